@@ -13,6 +13,11 @@ __host__ __device__ constexpr unsigned idesc_bf16(int M, int N, bool b_mn_major)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
 }
 
+// ... of an e4m3 x e4m3 -> float32 product, both operands K-major.
+__host__ __device__ constexpr unsigned idesc_e4m3(int M, int N) {
+    return (1u << 4) | ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
+}
+
 // Operand tile with 128-byte swizzle: rows of 128 bytes, atoms of 8 rows (1024 bytes) one after another.  K-major:
 // a row holds 64 k of one row of the operand; MN-major (B only): a row holds 64 columns of one k.  In both, the next
 // atom (8 more rows) lies 1024 bytes further (the stride offset).  The leading offset is not used by K-major swizzled
@@ -32,6 +37,12 @@ __device__ __forceinline__ unsigned long long desc_sw128(const void* smem, unsig
 __device__ __forceinline__ void mma_bf16(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate) {
     asm volatile(
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)accumulate) : "memory");
+}
+// e4m3 operands in shared memory, 32 k an instruction.
+__device__ __forceinline__ void mma_e4m3(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)accumulate) : "memory");
 }
 // The same product with the A operand in tensor memory: row m of A in lane m, its k values along the columns from

@@ -92,6 +92,11 @@ _SIGNATURES = {
     "llm_route_topk": [_vp, _i, _vp, _vp, _i, _i, _i, _f, _i, _i, _vp],
     "llm_expert_act_scale": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "llm_branch_sum_norm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _f, _vp],
+    "llm_quantize_blocks": [_vp, _i, _ll, _vp, _vp, _i, _i, _i, _vp],
+    "llm_linear8_few": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "llm_gemm8_tcgen05": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
+    "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
 }
 
@@ -2298,3 +2303,168 @@ def delta_rule(y: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor, a_log: 
     add_launches(1)
     _check(code, "delta_rule")
     return head_norm_gate(o, gate[:, :vv], eps, "silu", out_dtype=out_dtype, weight=weight)
+
+
+# ------------------------------------------------------------------------------------------------
+# Numbers in 8 bits: matrices of e4m3 values with a scale for every block of 128 (csrc/fp8.cuh, quantize_blocks.cu,
+# linear8_few.cu, gemm8_tcgen05.cu), and pages of keys and values with one for every head's vector (rope_kv_write8.cu, attention8.cu).
+_E4M3 = torch.float8_e4m3fn
+_BLOCK8 = 128
+_FEW8_MAX_ROWS = 64  # up to this many rows a product with 8-bit weights streams the weights through mma.sync; more go to tcgen05
+_ATTENTION8_HEAD_DIMS = (64, 128)
+
+
+def _here(*tensors) -> None:
+    """Kernels run on the current device's current stream: their operands have to lie there."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        _need(t.is_cuda and t.get_device() == device, f"a tensor lies on {t.device}, the current device is cuda:{device}")
+
+
+class Quantized:
+    """A matrix ``[M, K]`` in 8 bits: ``values`` (float8_e4m3fn, contiguous) times a float32 scale for every block of ``rows`` (1 or 128)
+    rows and 128 columns, ``scales [ceil(M / rows), ceil(K / 128)]``.  A weight (``rows`` 128) may carry any positive scales, such as
+    a checkpoint's; :func:`quantize_blocks` makes powers of two."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int = 1):
+        _need(rows in (1, _BLOCK8), f"Quantized: a scale is for 1 or {_BLOCK8} rows, not {rows}")
+        _need(values.dtype == _E4M3 and values.dim() == 2 and values.is_contiguous(), "Quantized: values are a contiguous float8_e4m3fn matrix")
+        blocks = (-(-values.shape[0] // rows), -(-values.shape[1] // _BLOCK8))
+        _need(scales.dtype == torch.float32 and tuple(scales.shape) == blocks and scales.is_contiguous(), f"Quantized: scales are contiguous float32 {list(blocks)}")
+        _need(scales.device == values.device, "Quantized: values and scales lie on one device")
+        self.values, self.scales, self.rows = values, scales, rows
+        self.shape, self.device = values.shape, values.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        m, k = self.shape
+        each = self.scales.repeat_interleave(self.rows, 0)[:m].repeat_interleave(_BLOCK8, 1)[:, :k]
+        return (self.values.float() * each).to(dtype)
+
+    def nbytes(self) -> int:
+        return self.values.numel() + 4 * self.scales.numel()
+
+
+def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Quantized:
+    """``x [M, K]`` (float32 or bfloat16, unit inner stride) in 8 bits: for every block of ``rows`` (1: activations, 128: weights) rows
+    and 128 columns the scale is ``2^e`` with the smallest ``e >= -126`` such that the block's largest finite ``|x|`` is at most ``448 * 2^e`` (1
+    for a block of zeros), and a value is ``x / 2^e`` rounded to the nearest e4m3 (ties to even).  NaN and infinities become NaN."""
+    _need(rows in (1, _BLOCK8), f"quantize_blocks: a scale is for 1 or {_BLOCK8} rows, not {rows}")
+    _need(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] <= 1), "quantize_blocks: x is a matrix with unit inner stride")
+    code = _code(x.dtype)
+    _here(x)
+    m, k = x.shape
+    values = torch.empty((m, k), dtype=_E4M3, device=x.device)
+    scales = torch.empty((-(-m // rows), -(-k // _BLOCK8)), dtype=torch.float32, device=x.device)
+    if m and k:
+        _check(_launch("llm_quantize_blocks", _ptr(x), code, x.stride(0), _ptr(values), _ptr(scales), m, k, rows, _stream()), "quantize_blocks")
+    return Quantized(values, scales, rows)
+
+
+def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x [M, K] @ w [N, K]^T -> [M, N]`` in 8 bits: ``x`` is quantised row by row in blocks of 128 (:func:`quantize_blocks`; it may
+    come as a :class:`Quantized` already), ``w`` has a scale for every block of 128 x 128.  Every block's products are summed on
+    the tensor cores and enter 32-bit sums times both scales: up to 64 rows through a kernel that streams the weights,
+    more on tcgen05.  ``K`` is a multiple of 16.  ``out_dtype``: float32 or bfloat16 (default: that of ``x``, bfloat16 for a quantised one)."""
+    _need(isinstance(w, Quantized) and w.rows == _BLOCK8, "linear8: w is a Quantized matrix with a scale for every 128 rows")
+    if isinstance(x, NormedInput):
+        x = x.materialize()
+    given = isinstance(x, Quantized)
+    _need(not given or x.rows == 1, "linear8: a quantised x has a scale for every row")
+    _need(len(x.shape) == 2 and x.shape[1] == w.shape[1], f"linear8: shapes {tuple(x.shape)} and {tuple(w.shape)} do not match")
+    (m, k), n = x.shape, w.shape[0]
+    _need(k >= 16 and k % 16 == 0, f"linear8: rows of {k} values; a multiple of 16 is needed")
+    out_dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
+    code = _code(out_dtype)
+    _here(w.values)
+    xq = x if given else quantize_blocks(x)
+    _here(xq.values)
+    _need(xq.values.data_ptr() % 16 == 0 and w.values.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
+    out = torch.empty((m, n), dtype=out_dtype, device=w.device)
+    if m == 0 or n == 0:
+        return out
+    operands = (_ptr(xq.values), _ptr(xq.scales), _ptr(w.values), _ptr(w.scales), _ptr(out), code, m, n, k, n)
+    if m <= _FEW8_MAX_ROWS:
+        # the weights may be asked for early only if the kernel in front is the one that quantised x here: it began when all
+        # before it had ended, whoever wrote the weights among them
+        _check(_launch("llm_linear8_few", *operands, int(not given), _stream()), "linear8 (few rows)")
+    else:
+        _check(_launch("llm_gemm8_tcgen05", *operands, _error_flag_ptr(), _stream()), "linear8 (tcgen05)")
+    return out
+
+
+def _pages8(pool: torch.Tensor, exponents: torch.Tensor, kv_heads: int, dim: int, what: str) -> None:
+    _need(pool.dtype == _E4M3 and pool.dim() == 5 and pool.is_contiguous() and pool.shape[1] == 2 and pool.shape[2] == kv_heads and pool.shape[4] == dim,
+          f"{what}: the pool plane is contiguous float8_e4m3fn [pages, 2, {kv_heads}, page_size, {dim}]")
+    _need(exponents.dtype == torch.uint8 and exponents.is_contiguous() and exponents.shape == pool.shape[:4],
+          f"{what}: exponents are contiguous uint8 {list(pool.shape[:4])}")
+    _need(dim in _ATTENTION8_HEAD_DIMS, f"{what}: 8-bit pages are built for heads of {_ATTENTION8_HEAD_DIMS} lanes, not {dim}")
+
+
+def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor | None, slot_map: torch.Tensor, pool: torch.Tensor,
+                   exponents: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
+    """:func:`rope_kv_write` into 8-bit pages: the query heads of each bfloat16 ``qkv`` row are rotated in place by its position's row of
+    ``table`` (None: no rotation); the rotated key heads, from their 32-bit values, and the value heads go to the row's slot of
+    ``pool`` (float8_e4m3fn ``[pages, 2, kv_heads, page_size, head_dim]``), each head's vector divided by a power of two (the rule of
+    :func:`quantize_blocks` with ``head_dim`` lanes a block) whose biased exponent goes to ``exponents`` (uint8 ``[pages, 2, kv_heads,
+    page_size]``): a number is ``e4m3 * 2^(exponent - 127)``.  Rows whose slot is no place of the pool are not stored."""
+    n, width = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
+    _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, f"rope_kv_write8: qkv rows hold {width} bfloat16 elements")
+    _need(qkv.stride(0) % 4 == 0 and qkv.data_ptr() % 8 == 0, "rope_kv_write8: qkv rows start on 8 bytes")
+    _i32(slot_map, "slot_map")
+    _need(slot_map.numel() == n, "rope_kv_write8: a slot for every row")
+    _pages8(pool, exponents, num_kv_heads, head_dim, "rope_kv_write8")
+    rows = 0
+    if table is not None:
+        _i32(positions, "positions")
+        _need(positions.numel() == n, "rope_kv_write8: a position for every row")
+        _need(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 2 and table.shape[1] == head_dim and table.shape[0] > 0, "the rotary table must be float32 [positions, head_dim]")
+        rows = table.shape[0]
+        _here(positions, table)
+    _here(qkv, slot_map, pool, exponents)
+    if n == 0:
+        return
+    code = _launch("llm_rope_kv_write8", _ptr(qkv), qkv.stride(0), _ptr(positions) if rows else None, _ptr(table), rows, _ptr(slot_map), _ptr(pool),
+                   _ptr(exponents), n, num_heads, num_kv_heads, head_dim, pool.shape[3], pool.shape[0], _stream())
+    _check(code, "rope_kv_write8")
+
+
+def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tensor, page_table: torch.Tensor, ctx, *, num_heads: int,
+                     num_kv_heads: int, head_dim: int, scale: float, window: int | None = None) -> torch.Tensor:
+    """:func:`paged_attention` over 8-bit pages as :func:`rope_kv_write8` leaves them.  ``q`` rows (bfloat16) start with the rotated query
+    heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  The keys of a request are split
+    over CTAs where the step has few rows, and joined by a second kernel.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
+    n = q.shape[0]
+    _need(q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= num_heads * head_dim, "paged_attention8: rows of q start with the query heads, bfloat16")
+    _need(q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0, "paged_attention8: rows of q start on 8 bytes")
+    _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, f"paged_attention8: {num_heads} query heads over {num_kv_heads} key heads")
+    _need(window is None or window >= 1, "paged_attention8: a window holds a key at least")
+    _pages8(pool, exponents, num_kv_heads, head_dim, "paged_attention8")
+    _i32(page_table, "page_table")
+    _i32(ctx.cu_tokens, "cu_tokens")
+    _i32(ctx.context_lens, "context_lens")
+    requests = ctx.context_lens.numel()
+    _need(page_table.dim() == 2 and page_table.shape[0] == requests and ctx.cu_tokens.numel() == requests + 1, "paged_attention8: a row of the page table and a length for every request")
+    _here(q, pool, exponents, page_table, ctx.cu_tokens, ctx.context_lens)
+    out = torch.empty((n, num_heads * head_dim), dtype=torch.bfloat16, device=q.device)
+    if n == 0 or requests == 0:
+        return out
+    longest = getattr(ctx, "max_query_len", None) or max(_token_counts(ctx))
+    keys = getattr(ctx, "max_context_len", None) or int(ctx.context_lens.max())
+    splits = _attention8_splits(requests * num_kv_heads * -(-longest * (num_heads // num_kv_heads) // 16), keys if window is None else min(keys, window + longest), n * num_heads * head_dim)
+    part_o = part_stat = None
+    if splits > 1:
+        part_o = torch.empty((n * num_heads * splits * head_dim,), dtype=torch.float32, device=q.device)
+        part_stat = torch.empty((n * num_heads * splits * 3,), dtype=torch.float32, device=q.device)
+    code = _launch("llm_attention8", _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(pool), _ptr(exponents), _ptr(page_table), page_table.shape[1],
+                   _ptr(ctx.cu_tokens), _ptr(ctx.context_lens), requests, n, longest, num_heads, num_kv_heads, head_dim, pool.shape[3],
+                   pool.shape[0], int(window or 0), float(scale), splits, _ptr(part_o), _ptr(part_stat), _stream())
+    add_launches(splits > 1)
+    _check(code, "paged_attention8")
+    return out
+
+
+def _attention8_splits(tiles: int, keys: int, elements: int) -> int:
+    """CTAs that share the keys of a row tile: as many as there is room for at once, none with fewer than 64 keys, and their
+    partial results bounded."""
+    splits = min(2 * _sm_count() // tiles, -(-keys // 64), _SPLIT_SCRATCH_BYTES // (4 * elements))
+    return max(1, splits)
