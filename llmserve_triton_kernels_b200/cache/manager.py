@@ -11,6 +11,9 @@ given back when the sequence ends) with two additions the reference has no use f
 * state slots: every request holds one slot id; an entry whose mixer keeps a ``StateSpec``
   has a tensor ``[slots, *shape]`` indexed by it, zeroed when the request starts.
 
+With ``dtype`` float8_e4m3fn the pages hold 8-bit keys and values and, beside the pool, a byte for every head's vector: the
+biased exponent of the power of two that it was divided by (``ops.rope_kv_write8``).
+
 Reservation and commit are separate: ``reserve`` finds pages for the new tokens of a whole
 step or raises ``OutOfPages`` with nothing changed; ``commit`` advances the lengths once the
 step has run and releases what the windows have passed.
@@ -38,6 +41,7 @@ class PagedKVView:
     slot_map: torch.Tensor  # [tokens] int32: page * page_size + offset of each new token
     page_size: int
     spec: PagedKVSpec | PagedRowSpec
+    exponents: torch.Tensor | None = None  # 8-bit pages: [pages, 2, kv_heads, page_size] uint8, a head's vector is e4m3 * 2^(exponent - 127)
 
 
 @dataclass
@@ -78,7 +82,14 @@ class PageGroup:
         else:
             self.place_elements = 2 * spec.kv_heads * spec.head_dim
             shape = (len(entries), self.num_pages, 2, spec.kv_heads, self.page_size, spec.head_dim)
-        self.pool = torch.zeros(shape, dtype=dtype, device=device)
+        self.exponents: torch.Tensor | None = None
+        if dtype == torch.float8_e4m3fn:
+            if isinstance(spec, PagedRowSpec):
+                raise ValueError("pages in 8 bits are built for keys and values of heads, not for rows of a latent")
+            self.pool = torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
+            self.exponents = torch.full(shape[:-1], 127, dtype=torch.uint8, device=device)
+        else:
+            self.pool = torch.zeros(shape, dtype=dtype, device=device)
         self.allocator = IdAllocator(self.num_pages, "page")
         self.tables: dict[object, list[int]] = {}
         # the same tables as int32 arrays with room to grow (released pages as 0), so that a step's table is put
@@ -141,7 +152,8 @@ class PageGroup:
         return max(0, last + 1 - len(table))
 
     def bytes_per_page(self) -> int:
-        return len(self.entries) * self.place_elements * self.page_size * self.pool.element_size()
+        scales = 0 if self.exponents is None else 2 * self.spec.kv_heads
+        return len(self.entries) * (self.place_elements * self.pool.element_size() + scales) * self.page_size
 
 
 class CacheManager:
@@ -230,7 +242,7 @@ class CacheManager:
         return 1.0 - used / held
 
     def nbytes(self) -> int:
-        total = sum(g.pool.numel() * g.pool.element_size() for g in self.groups)
+        total = sum(g.num_pages * g.bytes_per_page() for g in self.groups)
         return total + sum(t.numel() * t.element_size() for t in self._state_entries.values())
 
     # ------------------------------------------------------------------ lifecycle
@@ -347,7 +359,8 @@ class CacheManager:
                 g, plane = self._entry_group[key]
                 group = self.groups[g]
                 table, slot_map = group_tensors[g]
-                return PagedKVView(group.pool[plane], table, slot_map, group.page_size, group.spec)
+                exponents = None if group.exponents is None else group.exponents[plane]
+                return PagedKVView(group.pool[plane], table, slot_map, group.page_size, group.spec, exponents)
             if key in self._state_entries:
                 return StateView(self._state_entries[key], state_slots, host_slots)
             return None

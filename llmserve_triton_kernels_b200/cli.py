@@ -32,6 +32,8 @@ def parse_args(argv=None):
     ap.add_argument("--seed", type=int, default=None, help="sampling seed (and the weights' seed for a preset; default 0 there)")
     ap.add_argument("--device", default="cuda", help="a CUDA device; there is no CPU path")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--weight-dtype", choices=["float8"], default=None, help="the layers' matrices in 8 bits (default: as --dtype)")
+    ap.add_argument("--cache-dtype", choices=["float8"], default=None, help="keys and values in 8-bit pages (default: as --dtype)")
     ap.add_argument("--block-size", type=int, default=16)
     ap.add_argument("--num-blocks", type=int, default=None)
     ap.add_argument("--kv-mem-mib", type=float, default=None, help="size the cache by memory instead of --num-blocks")
@@ -49,6 +51,7 @@ def main(argv=None) -> None:
         args.model, dtype=args.dtype, device=device, seed=args.seed or 0, block_size=args.block_size,
         num_blocks=args.num_blocks, kv_mem_mib=args.kv_mem_mib, max_batch_size=args.max_batch_size,
         max_num_batched_tokens=args.max_num_batched_tokens, chunk_size=args.chunk_size, policy=args.policy,
+        weight_dtype=args.weight_dtype, cache_dtype=args.cache_dtype,
     )
     tok = llm.tokenizer
     if args.prompt_ids is not None:

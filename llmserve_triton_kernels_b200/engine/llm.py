@@ -21,7 +21,7 @@ from .. import models as _models  # noqa: F401  registers the built-in architect
 from ..cache import CacheManager, num_pages_for_budget
 from ..config.presets import PRESETS
 from ..config.registry import architecture_of
-from ..models.load import load_model, random_model, resolve_dtype
+from ..models.load import load_model, random_model, resolve_cache_dtype, resolve_dtype
 from ..parts.base import PagedKVSpec, PagedRowSpec, flat_specs
 from ..sampling import Sampler, SamplingParams
 from .scheduler import Scheduler
@@ -63,9 +63,15 @@ class LLM:
         policy: str = "continuous",
         tokenizer=None,
         freeze_gc: bool = True,
+        weight_dtype: str | None = None,
+        cache_dtype: str | None = None,
     ):
         """``model``: a folder with config.json and ``*.safetensors``; or the name of a preset or a
         config.json dictionary, for random weights drawn from ``seed``.
+
+        ``weight_dtype`` "float8": the layers' matrices in 8 bits (e4m3, a scale for every 128 x 128; the activations are quantised row
+        by row in front of every product).  ``cache_dtype`` "float8": keys and values in 8-bit pages (e4m3, a power of two for
+        every head's vector).  None: the compute type.  Both go with bfloat16 and the Llama architecture's layers.
 
         ``freeze_gc``: once the engine stands, collect garbage and move everything that is alive to the collector's
         permanent generation (``gc.freeze()``).  A full collection otherwise walks the some 170,000 objects that the
@@ -77,9 +83,9 @@ class LLM:
         if isinstance(model, dict) or (isinstance(model, str) and model in PRESETS and not Path(model).exists()):
             cfg_dict = PRESETS[model] if isinstance(model, str) else model
             self.config = architecture_of(cfg_dict).config_class.from_dict(cfg_dict)
-            self.model = random_model(self.config, seed, self.dtype, self.device)
+            self.model = random_model(self.config, seed, self.dtype, self.device, weight_dtype=weight_dtype)
         else:
-            self.model, self.config = load_model(model, self.dtype, self.device)
+            self.model, self.config = load_model(model, self.dtype, self.device, weight_dtype=weight_dtype)
             if tokenizer is None:
                 tokenizer = _maybe_tokenizer(model)
         self.tokenizer = tokenizer
@@ -87,7 +93,8 @@ class LLM:
         # a model without a position limit of its own: a request may be as long as the scheduler's token budget
         # allows it to be taken in, and the pool is sized for that
         model_limit = self.model.plan.max_positions or max(max_num_batched_tokens, 2048)
-        element = torch.empty(0, dtype=self.dtype).element_size()
+        pages_dtype = resolve_cache_dtype(cache_dtype, self.dtype, self.model)
+        element = torch.empty(0, dtype=pages_dtype).element_size()
         if num_blocks is None:
             if kv_mem_mib is not None:
                 num_blocks = num_pages_for_budget(specs, block_size, element, int(kv_mem_mib * 2**20))
@@ -101,7 +108,7 @@ class LLM:
                 num_blocks = max(1, min(want, cap))
         self.cache = CacheManager(
             specs, self.model.plan.schedule, page_size=block_size, num_pages=num_blocks,
-            max_requests=max_batch_size, dtype=self.dtype, device=self.device,
+            max_requests=max_batch_size, dtype=pages_dtype, device=self.device,
         )
         self.step_function = StepFunction(self.model, self.cache)
         self.sampler = Sampler(self.device)

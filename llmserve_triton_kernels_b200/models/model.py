@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from ..parts.base import Block, CompositeSpec, PagedKVSpec, PagedRowSpec, StateSpec, TensorSpec, build_part, part_factory
+from ..parts.base import Block, CompositeSpec, PagedKVSpec, PagedRowSpec, StateSpec, TensorSpec, build_part, flat_specs, part_factory
 from .plan import ModelPlan
 
 
@@ -91,13 +91,30 @@ class Model:
         for name, _ in plan.extra_tensors:
             self._vectors[name] = tensors[name].to(device=self.device, dtype=torch.float32).contiguous()
 
+    def quantize_weights(self) -> None:
+        """The layers' matrices in 8 bits, after :meth:`bind` (the token table, the output matrix and everything that is no matrix stay as
+        they are).  ValueError if a part's kernels read bfloat16 matrices only: then the model is not to be used, some parts may
+        have changed."""
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"8-bit weights go with bfloat16 activations, not {self.dtype}")
+        for _, part in self._named_parts:
+            part.quantize_weights()
+
+    def takes_eight_bit_pages(self) -> bool:
+        """Whether every layer that keeps or reads pages can do with 8-bit ones."""
+        mixers = [m for m in (getattr(self.blocks[run.layer], "mixer", None) for run in self.plan.schedule) if m is not None]
+        return self.dtype == torch.bfloat16 and all(
+            m.eight_bit_pages or not any(isinstance(s, (PagedKVSpec, PagedRowSpec)) for s in flat_specs([m.cache_spec()])) for m in mixers)
+
     def weight_bytes(self) -> int:
         """Bytes of every distinct weight tensor a step reads (the token table only if it is also the head)."""
         seen: dict[int, int] = {}
 
         def visit(obj):
             for value in vars(obj).values():
-                if isinstance(value, torch.Tensor):
+                if isinstance(value, ops.Quantized):
+                    seen[value.values.data_ptr()] = value.nbytes()
+                elif isinstance(value, torch.Tensor):
                     seen[value.data_ptr()] = value.numel() * value.element_size()
                 elif hasattr(value, "bind") and hasattr(value, "tensors"):
                     visit(value)

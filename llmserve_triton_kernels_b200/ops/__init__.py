@@ -483,7 +483,7 @@ class ResidualSink:
         takes the operands (then nothing was changed)."""
         m, k = x.shape
         n = w.shape[0]
-        if not (x.dtype == torch.bfloat16 and x.stride(1) == 1 and w.is_contiguous() and self.resid.is_contiguous()):
+        if isinstance(w, Quantized) or not (x.dtype == torch.bfloat16 and x.stride(1) == 1 and w.is_contiguous() and self.resid.is_contiguous()):
             return None
         if m <= _DECODE_LINEAR_MAX_ROWS and self.weight is not None and self.alpha == 1.0:
             parts = -(-n // 16)
@@ -563,7 +563,10 @@ def linear(x, w: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Te
     (fixed summation order); bfloat16 operands accumulate in 32-bit on the tensor cores: up to 16 rows
     through the weight-streaming kernel, more through the vendor's library (or, where ``_GEMM_POLICY`` says so,
     the own tcgen05 kernel from 128 rows on).  ``x`` may be a :class:`NormedInput`.  In 32 bits ``w`` may be what the kernel in
-    front writes; in bfloat16 it is a weight, which the kernels ask for before the one in front has ended."""
+    front writes; in bfloat16 it is a weight, which the kernels ask for before the one in front has ended.  A :class:`Quantized`
+    ``w`` goes to :func:`linear8`."""
+    if isinstance(w, Quantized):
+        return linear8(x, w, out_dtype)
     if isinstance(x, NormedInput):
         if x.shape[0] >= _TCGEN05_MIN_ROWS:
             out = _tcgen05_linear(x, w, out_dtype or x.dtype, 0, w.shape[0])
@@ -660,7 +663,7 @@ def linear_qkv_rope(
     scaled = isinstance(x, NormedInput)
     xt = x.xw if scaled else x
     m, k = xt.shape
-    if not (xt.dtype == torch.bfloat16 and m <= _DECODE_LINEAR_MAX_ROWS and xt.stride(1) == 1 and w_in.is_contiguous()):
+    if isinstance(w_in, Quantized) or not (xt.dtype == torch.bfloat16 and m <= _DECODE_LINEAR_MAX_ROWS and xt.stride(1) == 1 and w_in.is_contiguous()):
         return None
     if head_dim % 16 or (table is not None and (table.dtype != torch.float32 or table.shape[1] != head_dim)):
         return None
@@ -687,6 +690,8 @@ def linear_swiglu(x, w_gate_up: torch.Tensor) -> torch.Tensor:
     """``silu(x @ gate^T) * (x @ up^T)`` for ``w_gate_up = [gate rows | up rows]``: one kernel for
     few bfloat16 rows, else a product followed by the activation kernel."""
     inter = w_gate_up.shape[0] // 2
+    if isinstance(w_gate_up, Quantized):
+        return swiglu(linear8(x, w_gate_up, torch.bfloat16))
     xt = x.xw if isinstance(x, NormedInput) else x
     if xt.dtype == torch.bfloat16 and xt.shape[0] <= _DECODE_LINEAR_MAX_ROWS:
         out = _decode_linear(x, w_gate_up, torch.bfloat16, 1, inter, up_offset=inter)
@@ -2311,7 +2316,7 @@ def delta_rule(y: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor, a_log: 
 _E4M3 = torch.float8_e4m3fn
 _BLOCK8 = 128
 _FEW8_MAX_ROWS = 64  # up to this many rows a product with 8-bit weights streams the weights through mma.sync; more go to tcgen05
-_ATTENTION8_HEAD_DIMS = (64, 128)
+ATTENTION8_HEAD_DIMS = (64, 128)
 
 
 def _here(*tensors) -> None:
@@ -2360,6 +2365,12 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Quantized:
     return Quantized(values, scales, rows)
 
 
+def quantize_weight(w: torch.Tensor) -> Quantized:
+    """A product's matrix ``[N, K]`` as :func:`linear8` takes it: a scale for every block of 128 x 128."""
+    _need(w.dim() == 2 and w.shape[1] >= 16 and w.shape[1] % 16 == 0, f"quantize_weight: a matrix with rows of a multiple of 16 values, not {list(w.shape)}")
+    return quantize_blocks(w, rows=_BLOCK8)
+
+
 def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x [M, K] @ w [N, K]^T -> [M, N]`` in 8 bits: ``x`` is quantised row by row in blocks of 128 (:func:`quantize_blocks`; it may
     come as a :class:`Quantized` already), ``w`` has a scale for every block of 128 x 128.  Every block's products are summed on
@@ -2397,7 +2408,7 @@ def _pages8(pool: torch.Tensor, exponents: torch.Tensor, kv_heads: int, dim: int
           f"{what}: the pool plane is contiguous float8_e4m3fn [pages, 2, {kv_heads}, page_size, {dim}]")
     _need(exponents.dtype == torch.uint8 and exponents.is_contiguous() and exponents.shape == pool.shape[:4],
           f"{what}: exponents are contiguous uint8 {list(pool.shape[:4])}")
-    _need(dim in _ATTENTION8_HEAD_DIMS, f"{what}: 8-bit pages are built for heads of {_ATTENTION8_HEAD_DIMS} lanes, not {dim}")
+    _need(dim in ATTENTION8_HEAD_DIMS, f"{what}: 8-bit pages are built for heads of {ATTENTION8_HEAD_DIMS} lanes, not {dim}")
 
 
 def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor | None, slot_map: torch.Tensor, pool: torch.Tensor,
@@ -2410,9 +2421,9 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
     n, width = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
     _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, f"rope_kv_write8: qkv rows hold {width} bfloat16 elements")
     _need(qkv.stride(0) % 4 == 0 and qkv.data_ptr() % 8 == 0, "rope_kv_write8: qkv rows start on 8 bytes")
+    _pages8(pool, exponents, num_kv_heads, head_dim, "rope_kv_write8")
     _i32(slot_map, "slot_map")
     _need(slot_map.numel() == n, "rope_kv_write8: a slot for every row")
-    _pages8(pool, exponents, num_kv_heads, head_dim, "rope_kv_write8")
     rows = 0
     if table is not None:
         _i32(positions, "positions")

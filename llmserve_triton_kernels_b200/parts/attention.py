@@ -6,7 +6,8 @@ src/llmserve/kvcache/paged.py:81-110 (key j is visible to the query at position 
 consecutive query heads share a key/value head; softmax scale 1/sqrt(head_dim), which arrives
 here as the parameter ``scale``).  ``window`` (None in Llama) limits a query to the last
 ``window`` keys, itself included.  With ``own_kv=False`` the layer has no key and value
-projections and reads the cache that an earlier layer of the order wrote.  ``qkv_bias`` and
+projections and reads the cache that an earlier layer of the order wrote.  Over 8-bit pages (``cache.exponents``) the projection,
+the rotation with the write, and the attention are kernels of their own.  ``qkv_bias`` and
 ``out_bias`` (both off in Llama; the reference's projections take the first as a flag,
 src/llmserve/model/llama.py:64-66) give the projections bias vectors ``*_proj.bias``: such a layer
 runs its products and the bias sums as kernels of their own, not the fused decode kernels.
@@ -112,6 +113,15 @@ class PagedAttention(Mixer):
         if self.position is not None:
             self.position.bind({}, dtype, device)
 
+    def quantize_weights(self) -> None:
+        if self.general:
+            raise ValueError("8-bit weights are not built for attention with value_dim, qk_norm_eps or distance_bias")
+        self.w_in, self.w_out = ops.quantize_weight(self.w_in), ops.quantize_weight(self.w_out)
+
+    @property
+    def eight_bit_pages(self) -> bool:
+        return not self.general and self.head_dim in ops.ATTENTION8_HEAD_DIMS
+
     def cache_spec(self) -> PagedKVSpec:
         return PagedKVSpec(self.num_kv_heads, max(self.head_dim, self.value_dim), self.window)
 
@@ -135,24 +145,19 @@ class PagedAttention(Mixer):
             return self._forward_general(x, ctx, cache, sink)
         table = self._rotary_table()
         qkv = None
-        if (self.position is None or table is not None) and self.b_in is None:
+        eight_bit = getattr(cache, "exponents", None) is not None
+        if (self.position is None or table is not None) and self.b_in is None and not eight_bit:
             # few rows: projection, rotation and the cache write in one kernel
             qkv = ops.linear_qkv_rope(
                 x, self.w_in, ctx.positions, table, cache.slot_map, cache.pool, H, KV, D, write_kv=self.own_kv
             )
         if qkv is None:
             qkv = self._project_rotate_store(x, ctx, cache, table)
-        out = ops.paged_attention(
-            qkv,
-            cache.pool,
-            cache.page_table,
-            ctx,
-            num_heads=H,
-            num_kv_heads=KV,
-            head_dim=D,
-            scale=self.scale,
-            window=self.window,
-        )
+        heads = {"num_heads": H, "num_kv_heads": KV, "head_dim": D, "scale": self.scale, "window": self.window}
+        if eight_bit:
+            out = ops.paged_attention8(qkv, cache.pool, cache.exponents, cache.page_table, ctx, **heads)
+        else:
+            out = ops.paged_attention(qkv, cache.pool, cache.page_table, ctx, **heads)
         # the contribution to the 32-bit residual stream leaves the product in 32-bit: it is the sum's largest addend
         if self.b_out is not None:
             return ops.add_bias(ops.linear(out, self.w_out, out_dtype=torch.float32), self.b_out.float())
@@ -188,6 +193,9 @@ class PagedAttention(Mixer):
             q = qkv[:, : H * D].unflatten(1, (H, D))
             k = qkv[:, H * D : (H + KV) * D].unflatten(1, (KV, D)) if self.own_kv else qkv.new_empty((n, 0, D))
             self.position.apply(q, k, ctx.positions)
+        if self.own_kv and getattr(cache, "exponents", None) is not None:
+            ops.rope_kv_write8(qkv, ctx.positions, table, cache.slot_map, cache.pool, cache.exponents, H, KV, D)
+            return qkv
         ops.rope_kv_write(
             qkv, ctx.positions, table, cache.slot_map, cache.pool, H, KV, D, write_kv=self.own_kv
         )

@@ -113,8 +113,17 @@ class Part:
     # (``ops.Biased``), for a kernel that takes the result up anyway
     leaves_bias = False
 
+    # True for a mixer that can keep its keys and values in 8-bit pages (``PagedKVView.exponents``)
+    eight_bit_pages = False
+
     def tensors(self) -> dict[str, TensorSpec]:
         return {}
+
+    def quantize_weights(self) -> None:
+        """Put the matrices of this part's products, once bound, into 8 bits (``ops.quantize_blocks`` with a scale for every 128 x 128).  A
+        part without matrices has nothing to do; one whose kernels read bfloat16 matrices only refuses."""
+        if any(len(spec.shape) >= 2 for spec in self.tensors().values()):
+            raise ValueError(f"8-bit weights are not built for {type(self).__name__}")
 
     def bind(self, tensors: dict[str, torch.Tensor], dtype: torch.dtype, device: torch.device) -> None:
         """Take ownership of the loaded tensors (keyed by local name), in the compute dtype."""

@@ -34,6 +34,8 @@ def parse_args(argv=None):
     ap.add_argument("--random", metavar="PRESET", help="instead of --model: random weights of a named configuration (config/presets.py)")
     ap.add_argument("--seed", type=int, default=0, help="seed of the random weights (with --random)")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--weight-dtype", choices=["float8"], default=None, help="the layers' matrices in 8 bits")
+    ap.add_argument("--cache-dtype", choices=["float8"], default=None, help="keys and values in 8-bit pages")
     ap.add_argument("--out", required=True, help="folder for <step>.f32 files")
     ap.add_argument("--max-tokens", type=int, required=True, help="most tokens that live requests hold at any time")
     ap.add_argument("--page-size", type=int, default=16, help="tokens per page of the cache")
@@ -54,7 +56,7 @@ def main(argv=None) -> int:
     from .engine.step import StepFunction
     from .config.presets import PRESETS
     from .config.registry import architecture_of
-    from .models.load import load_model, random_model, resolve_dtype
+    from .models.load import load_model, random_model, resolve_cache_dtype, resolve_dtype
 
     out_dir = Path(args.out)
     out_dir.mkdir(parents=True, exist_ok=True)
@@ -66,13 +68,13 @@ def main(argv=None) -> int:
         if args.random not in PRESETS:
             raise SystemExit(f"trace_run: no configuration named {args.random!r}; known: {sorted(PRESETS)}")
         cfg_dict = PRESETS[args.random]
-        model = random_model(architecture_of(cfg_dict).config_class.from_dict(cfg_dict), args.seed, dtype, device)
+        model = random_model(architecture_of(cfg_dict).config_class.from_dict(cfg_dict), args.seed, dtype, device, weight_dtype=args.weight_dtype)
     else:
-        model, _ = load_model(args.model, dtype, device)
+        model, _ = load_model(args.model, dtype, device, weight_dtype=args.weight_dtype)
     num_pages = max(1, -(-args.max_tokens // args.page_size))
     cache = CacheManager(
         model.cache_specs(), model.plan.schedule, page_size=args.page_size, num_pages=num_pages,
-        max_requests=args.max_requests, dtype=dtype, device=device,
+        max_requests=args.max_requests, dtype=resolve_cache_dtype(args.cache_dtype, dtype, model), device=device,
     )
     step_function = StepFunction(model, cache)
     for line in sys.stdin:
