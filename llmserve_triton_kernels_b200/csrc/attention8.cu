@@ -2,26 +2,36 @@
 //
 //   s_j = scale * 2^(ek_j) * q . k_j        out = sum_j 2^(s_j) 2^(ev_j) v_j / sum_j 2^(s_j)     (scale holds log2 e)
 //
-// Rows are (token, query head of the key head's group): 16 a CTA, the height of an mma.sync tile, so that one new token of a
-// request whose group has up to 16 heads is one tile.  What bounds it is the pages' bytes; everything between them and the
-// products is registers: with the lanes of a head permuted alike in q and k (a dot product does not notice) a thread's 16-byte
-// load of a key holds the B elements of four products, and since the output's columns may come in any order, a thread's 16
-// bytes of four values are the B elements of sixteen.  e4m3 becomes half precision (one instruction for two values, exact) on the
-// way; q becomes half precision too, its row divided by a power of two so that it neither overflows nor loses bits.
+// Rows are (token, query head of the key head's group).  They ride along as the narrow side of both products: a tile of mma.sync is 16
+// keys (then: 16 lanes of the output) high and 8 rows wide, so that a group of up to 8 heads wastes nothing; a CTA takes one or two
+// such tiles of rows.  What bounds it is the pages' bytes, and behind them the instructions that unpack them, so there are few: with
+// the lanes of a head permuted alike in q and k (a dot product does not notice) a thread's 16-byte load of a key is the A operand of
+// two e4m3 products as it lies there.  q takes part as the sum of two e4m3 numbers, its row scaled to [128, 256): the first has a
+// value's upper 4 bits, the second the next 4, which is all that bfloat16 has (2^-18 of the row's largest value is what may be lost
+// of small ones).  Values become half precision (exact; one instruction for two): since the output's lanes may come in any order, a
+// thread's bytes of four values are the A elements of the second product.  Its weights stay in half precision, not in e4m3, whose
+// 18 powers of two would drop the many small weights of a long context.  They turn from the first product's result into the
+// second's operand by a transposition of 8 x 8 (movmatrix).
 //
 // A value's weight 2^(s_j + ev_j) has a running maximum of its own, apart from that of 2^(s_j): whatever the values' scales, the
 // weights that enter the half-precision product are at most one and the largest is one.
 //
-// The keys of a row tile are shared out over `splits` CTAs and their warps, 16 keys at a time; the warps meet in shared memory, the
-// CTAs in a second kernel, through scratch memory of the call's own: nothing is kept from call to call.
+// Work is counted in tiles of 16 keys for one tile of rows: a step's tiles, request after request, form one list, and every CTA takes an
+// equal stretch of it, wherever requests begin and end (their lengths are the device's business: a captured step is replayed at any
+// lengths).  A CTA's stretch is cut into segments, one for each tile of rows that it touches; a segment that holds all keys of its
+// rows writes their outputs, one that holds some leaves its sums in the call's scratch memory, and a second kernel joins those.
+// Within a segment the tiles go round the CTA's warps; a warp's tiles come through a ring of its own in shared memory (cp.async, a
+// thread reads back what it asked for itself, so nobody waits for anybody), and the warps meet once, in shared memory.
 //
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
 // Where rows differ in what they see, NaN among the values is counted apart, so that it reaches the rows that see it alone.
-#include "common.cuh"
+#include "fp8.cuh"
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 16;
+constexpr int WARPS = 8, THREADS = WARPS * 32, TILE = 16, STAGES = 3;
+constexpr int JOIN_THREADS = 512;
+constexpr int MAX_REQUESTS = 1024;  // of a step whose work is counted tile by tile
 
 struct Attn8Params {
     const __nv_bfloat16* q;
@@ -34,14 +44,19 @@ struct Attn8Params {
     int table_width;
     const int* cu_tokens;
     const int* context_lens;
-    int H, KV, G, page_size, pages, window, splits;
-    float scale;      // times log2 e
-    float* part_o;    // [rows of the step, splits, D]
-    float* part_stat; // [rows of the step, splits, 3]: largest score, largest score with the value's scale, sum
+    int requests, H, KV, G, page_size, pages, window;
+    int ranges;         // stretches of the step's list of tiles at most; 0: a CTA takes a tile of rows with all its keys
+    float scale;        // times log2 e
+    float* part_sums;   // [ranges][2][ROWS][D + 4]: what a stretch holds of the rows at its beginning and at its end,
+    float* part_stats;  // [ranges][2][ROWS][3]      as warps leave it to one another
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned half2_of(unsigned short v) {
@@ -59,405 +74,636 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float quad_max(float v) {
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// Over the eight lanes that hold the same row.
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// An 8 x 8 matrix of half-precision numbers, row g's elements 2 t and 2 t + 1 in lane (g, t), turned round.
+__device__ __forceinline__ unsigned transpose(unsigned v) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
 }
 
-// What a thread holds of 16 keys: 16-byte pieces of keys g and g + 8, and of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+// A stage of a warp's ring, 16 keys: [piece][lane] of what the threads hold (D / 4 bytes of keys g and g + 8, D / 8 bytes of the values
+// 2 t, 2 t + 1, 2 t + 8, 2 t + 9), then the exponents of the keys and of the values.
 template <int D>
-struct Keys {
-    static constexpr int KW = D / 16;  // words of a key a thread: D / 4 bytes
-    static constexpr int VW = D / 32;  // words of a value: D / 8 bytes
-    unsigned k[2][KW], v[4][VW];
-    unsigned ek[2], ev[2];  // exponents of keys / values (2 t | 2 t + 1), (2 t + 8 | 2 t + 9), a byte each
+struct Stage {
+    static constexpr int K_PIECES = D / 32, V_BYTES = D / 8;  // 16-byte pieces of both keys; bytes of a value
+    static constexpr int KEYS = K_PIECES * 512, VALUES = 4 * 32 * V_BYTES, BYTES = KEYS + VALUES + 2 * TILE;
 };
 
-template <int WORDS>
-__device__ __forceinline__ void load_words(unsigned (&w)[WORDS], const unsigned char* p) {
-    if constexpr (WORDS >= 4) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        if constexpr (WORDS == 8) {
-            const uint4 b = __ldg(reinterpret_cast<const uint4*>(p + 64));
-            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-        }
-    } else {
-        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = a.x; w[1] = a.y;
-    }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
-// ALIGNED: a page holds whole tiles of 16 keys.
-template <int D, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS)
+// References start below every score; a row whose weights' sum is zero has seen nothing.
+constexpr float NOTHING = -3.4028234e38f;
+
+// Two lanes of a row's output, columns c and c + 1 of the sums: its sum over the weights' sum; zeros for a row that saw no key.
+template <int D>
+__device__ __forceinline__ void finish(const Attn8Params& p, int first, int h, int rho, int c, float a, float b, float total, float y0, float y1) {
+    const float f = total == 0.f ? 0.f : exp2f(b - a) / total;
+    const int token = rho / p.G, lane = (D / 8) * ((c & 15) >> 1) + 2 * (c >> 4);
+    __nv_bfloat16* at = p.out + (first + token) * p.out_stride + (long long)(h * p.G + rho - token * p.G) * D + lane;
+    *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(y0 * f, y1 * f);
+}
+
+// A request's share of the list: tiles of rows for every key head, and the tiles of keys that any of its rows sees.
+struct Share {
+    int row_tiles, first_tile, tiles;
+};
+template <int ROWS>
+__device__ __forceinline__ Share share_of(const Attn8Params& p, int r) {
+    const int n = p.cu_tokens[r + 1] - p.cu_tokens[r], ctx = p.context_lens[r];
+    const int end = min(ctx, p.table_width * p.page_size), begin = p.window > 0 ? max(0, ctx - n - p.window + 1) : 0;
+    Share s;
+    s.row_tiles = (n * p.G + ROWS - 1) / ROWS;
+    s.first_tile = begin / TILE;
+    s.tiles = n > 0 ? max(0, (end + TILE - 1) / TILE - s.first_tile) : 0;
+    return s;
+}
+
+// Where the requests' shares begin in the list, [requests + 1], by the whole block.
+template <int ROWS>
+__device__ __forceinline__ void lay_out(const Attn8Params& p, long long* begins) {
+    for (int r = threadIdx.x; r < p.requests; r += blockDim.x) {
+        const Share s = share_of<ROWS>(p, r);
+        begins[r + 1] = (long long)p.KV * s.row_tiles * s.tiles;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        long long run = 0;
+        for (int r0 = 0; r0 < p.requests; r0 += 32) {
+            const int r = r0 + threadIdx.x;
+            long long v = r < p.requests ? begins[r + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                if ((int)threadIdx.x >= o) v += u;
+            }
+            if (r < p.requests) begins[r + 1] = run + v;
+            run += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (threadIdx.x == 0) begins[0] = 0;
+    }
+    __syncthreads();
+}
+
+// Stretches of a list of `total` tiles: no more than there are CTAs, none (but the last) shorter than a tile a warp.
+__device__ __forceinline__ int stretches(const Attn8Params& p, long long total) {
+    return (int)max(1LL, min((long long)p.ranges, total / WARPS));
+}
+
+// EIGHTS: pages hold whole runs of eight keys, so that a tile is two runs with one place each.
+template <int D, int NT, bool EIGHTS>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
 attention8_kernel(const Attn8Params p) {
-    constexpr int KSTEPS = D / 16, NTILES = D / 8;
-    extern __shared__ __align__(16) float merge[];  // [WARPS][16][D + 4], then [WARPS][16][3]
+    constexpr int KSTEPS = D / 32, MTILES = D / 16, ROWS = 8 * NT, PITCH = D + 4;
+    using S = Stage<D>;
+    extern __shared__ __align__(16) unsigned char smem[];  // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
+    __shared__ float stats[WARPS][ROWS][3];                // largest score, largest score with the value's scale, sum of weights
+    __shared__ long long begins[MAX_REQUESTS + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r = blockIdx.x / p.KV, h = blockIdx.x - r * p.KV, split = blockIdx.z;
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * STAGES * S::BYTES;
+    const unsigned char* ring_at = smem + warp * STAGES * S::BYTES;
     pdl_wait();
     pdl_trigger();
-    const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, ctx = p.context_lens[r];
-    const int row0 = blockIdx.y * 16, rows = n * p.G;
-    if (row0 >= rows) return;
-    const int start = ctx - n;  // position of the request's first new token
-    const int pos_min = start + row0 / p.G, pos_max = start + min(row0 + 15, rows - 1) / p.G;
-    const int key_end = min(pos_max + 1, p.table_width * p.page_size);
-    const int key_begin = p.window > 0 ? max(0, pos_min - p.window + 1) : 0;
-    const int tile_begin = key_begin / TILE, tile_count = max(0, (key_end + TILE - 1) / TILE - tile_begin);
-    const int per = (tile_count + p.splits - 1) / p.splits;
-    const int tile_lo = tile_begin + split * per, tile_hi = tile_begin + min(tile_count, (split + 1) * per);
-
-    // this thread's two rows
-    int pos[2], token[2], head[2];
-    bool live[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int rho = row0 + g + 8 * i;
-        live[i] = rho < rows;
-        token[i] = live[i] ? rho / p.G : 0;
-        head[i] = h * p.G + (live[i] ? rho - token[i] * p.G : 0);
-        pos[i] = live[i] ? start + token[i] : -1;
-        token[i] += first;
+    long long at = 0, end = 1;
+    if (p.ranges) {
+        lay_out<ROWS>(p, begins);
+        const long long total = begins[p.requests];
+        const int count = stretches(p, total);
+        if ((int)blockIdx.x >= count) return;
+        at = total * blockIdx.x / count;
+        end = total * (blockIdx.x + 1) / count;
     }
-    // q in half precision: product j of a key takes lanes (64 (j / 4) + 16 t + 4 (j % 4)) + 0 .. 3, or for D = 64 16 t + 4 j + 0 .. 3
-    unsigned qa[KSTEPS][4];
-    float factor[2];
+    while (at < end) {
+    // ---- the segment: request r, key head h, rows from row0 on, tiles tile_lo .. tile_hi - 1 ----
+    int r, h, row0, tile_lo, tile_hi, part = -1;  // part: the place in scratch memory of a segment without all keys
+    if (p.ranges) {
+        int lo = 0, hi = p.requests;  // the last request whose share begins at or before `at`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (begins[mid] <= at) lo = mid; else hi = mid;
+        }
+        r = lo;
+        const Share s = share_of<ROWS>(p, r);
+        const long long within = at - begins[r];
+        const int unit = (int)(within / s.tiles), off = (int)(within - (long long)unit * s.tiles);
+        const int take = (int)min((long long)(s.tiles - off), end - at);
+        h = unit / s.row_tiles;
+        row0 = (unit - h * s.row_tiles) * ROWS;
+        tile_lo = s.first_tile + off;
+        tile_hi = tile_lo + take;
+        if (take < s.tiles) part = blockIdx.x * 2 + (off == 0);
+        at += take;
+    } else {
+        r = blockIdx.x / p.KV;
+        h = blockIdx.x - r * p.KV;
+        row0 = blockIdx.y * ROWS;
+        const Share s = share_of<ROWS>(p, r);
+        tile_lo = s.first_tile;
+        tile_hi = tile_lo + s.tiles;
+        at = end;
+    }
+    const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = n * p.G;
+    if (row0 >= rows) return;
+    const int start = p.context_lens[r] - n;  // position of the request's first new token
+    const int pos_min = start + row0 / p.G, pos_max = start + min(row0 + ROWS - 1, rows - 1) / p.G;
+    // the request's tiles may reach further back or on than these rows see
+    const int key_end = min(pos_max + 1, p.table_width * p.page_size);
+    if (p.window > 0) tile_lo = max(tile_lo, max(0, pos_min - p.window + 1) / TILE);
+    tile_hi = min(tile_hi, (key_end + TILE - 1) / TILE);
+    const int mine = max(0, (tile_hi - tile_lo - warp + WARPS - 1) / WARPS);  // this warp's tiles: tile_lo + warp + i WARPS
+
+    // ---- the ring ----
+    const int* table = p.page_table + (long long)r * p.table_width;
+    // key `j` of the request as an index over [pages, 2, KV, page_size]
+    auto place = [&](int j) -> long long {
+        const int at = j / p.page_size;
+        const int page = min(max(table[at], 0), p.pages - 1);
+        return ((long long)page * 2 * p.KV + h) * p.page_size + (j - at * p.page_size);
+    };
+    const long long to_values = (long long)p.KV * p.page_size;
+    const unsigned char* my_keys = p.pool + (long long)g * D + 16 * t;  // what this thread holds of a run of eight keys, and of their values
+    const unsigned char* my_values = p.pool + (to_values + 2 * t) * D + S::V_BYTES * g;
+    unsigned run[2] = {0u, 0u};  // EIGHTS: this lane's tile of the next 32: the places of its two runs, in eights
+    auto issue = [&](int i, int slot) {
+        const int j0 = (tile_lo + warp + i * WARPS) * TILE;
+        const unsigned dst = ring + slot * S::BYTES;
+        // a place behind the request's end is some place of the pool: what lies there is masked
+        if constexpr (EIGHTS) {
+            if ((i & 31) == 0) {
+                const int j = j0 + lane * (WARPS * TILE);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        unsigned raw[KSTEPS][2];
-        unsigned top = 0;
-        const __nv_bfloat16* src = p.q + token[i] * p.q_stride + (long long)head[i] * D + 16 * t;
+                for (int x = 0; x < 2; ++x) run[x] = j + 8 * x < key_end ? (unsigned)(place(j + 8 * x) >> 3) : 0u;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const unsigned long long at = (unsigned long long)__shfl_sync(0xffffffffu, run[x], i & 31) * 8;
+                const unsigned char* kp = my_keys + at * D;
+                const unsigned char* vp = my_values + at * D;
+#pragma unroll
+                for (int c = 0; c < S::K_PIECES / 2; ++c) copy_async<16>(dst + (x * (S::K_PIECES / 2) + c) * 512 + lane * 16, kp + 64 * c);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) copy_async<S::V_BYTES>(dst + S::KEYS + (2 * x + e) * 32 * S::V_BYTES + lane * S::V_BYTES, vp + e * D);
+                if (lane < 2) copy_async<8>(dst + S::KEYS + S::VALUES + lane * TILE + 8 * x, p.exponents + at + lane * to_values);
+            }
+        } else {
+            // lane l finds key l's place
+            const bool is_there = j0 + (lane & 15) < key_end;
+            const long long own = is_there ? place(j0 + (lane & 15)) : 0;
+            const unsigned char exponent = is_there ? __ldg(p.exponents + own + (lane >> 4) * to_values) : 127;
+            asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(dst + S::KEYS + S::VALUES + lane), "r"((unsigned)exponent) : "memory");
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const long long kp = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, g + 8 * x);
+#pragma unroll
+                for (int c = 0; c < S::K_PIECES / 2; ++c) copy_async<16>(dst + (x * (S::K_PIECES / 2) + c) * 512 + lane * 16, p.pool + kp * D + 16 * t + 64 * c);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const long long vp = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, 2 * t + e + 8 * x) + to_values;
+                    copy_async<S::V_BYTES>(dst + S::KEYS + (2 * x + e) * 32 * S::V_BYTES + lane * S::V_BYTES, p.pool + vp * D + S::V_BYTES * g);
+                }
+            }
+        }
+    };
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (i < mine) issue(i, i);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+
+    // ---- q: product j of a key takes lanes 64 (j / 2) + 16 t + 8 (j % 2) + 0 .. 7 of a row, as the keys' bytes lie ----
+    unsigned qb[NT][KSTEPS][2][2];  // [upper, lower bits][first, second four lanes]
+    float factor[NT][2];  // of this thread's rows, which are 2 t and 2 t + 1 of every tile in the products' results
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int rho = row0 + 8 * nt + g;
+        const bool live = rho < rows;
+        const int token = live ? rho / p.G : 0, head = h * p.G + (live ? rho - token * p.G : 0);
+        const __nv_bfloat16* src = p.q + (first + token) * p.q_stride + (long long)head * D + 16 * t;
+        unsigned raw[KSTEPS][4], top = 0;
 #pragma unroll
         for (int j = 0; j < KSTEPS; ++j) {
-            const uint2 w = live[i] ? *reinterpret_cast<const uint2*>(src + 64 * (j / 4) + 4 * (j % 4)) : make_uint2(0u, 0u);
-            raw[j][0] = w.x;
-            raw[j][1] = w.y;
+            const __nv_bfloat16* at = src + 64 * (j / 2) + 8 * (j & 1);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                const uint2 w = live ? *reinterpret_cast<const uint2*>(at + 4 * e) : make_uint2(0u, 0u);
+                raw[j][2 * e] = w.x;
+                raw[j][2 * e + 1] = w.y;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
                 const unsigned a = raw[j][e] & 0x7fffu, b = (raw[j][e] >> 16) & 0x7fffu;
                 top = max(top, max(a < 0x7f80u ? a : 0u, b < 0x7f80u ? b : 0u));
             }
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest value to [2^14, 2^15): 2^shift, in two factors because either end may leave 32 bits' exponents
-        const int shift = top ? 141 - max((int)(top >> 7), 1) : 0;
+        // the row's largest value to [2^7, 2^8): 2^shift, in two factors because either end may leave 32 bits' exponents
+        const int shift = top ? 134 - max((int)(top >> 7), 1) : 0;
         const float f0 = __uint_as_float((unsigned)(127 + shift / 2) << 23), f1 = __uint_as_float((unsigned)(127 + shift - shift / 2) << 23);
-        factor[i] = p.scale / f0 / f1;
+        const float own = p.scale / f0 / f1;
+        const int own_pos = live ? start + token : -1;
 #pragma unroll
         for (int j = 0; j < KSTEPS; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float a = __uint_as_float(raw[j][e] << 16) * f0 * f1, b = __uint_as_float(raw[j][e] & 0xffff0000u) * f0 * f1;
-                qa[j][i + 2 * e] = pack_half(a, b);
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    v[2 * i] = __uint_as_float(raw[j][2 * e + i] << 16) * f0 * f1;
+                    v[2 * i + 1] = __uint_as_float(raw[j][2 * e + i] & 0xffff0000u) * f0 * f1;
+                }
+                const unsigned upper = fp8::pack4(v[0], v[1], v[2], v[3], 1.f);
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const unsigned h2 = half2_of((unsigned short)(upper >> (16 * i)));
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+                    w[2 * i] = v[2 * i] - back.x;
+                    w[2 * i + 1] = v[2 * i + 1] - back.y;
+                }
+                qb[nt][j][0][e] = upper;
+                qb[nt][j][1][e] = fp8::pack4(w[0], w[1], w[2], w[3], 1.f);
             }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            factor[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
+            pos[nt][e] = __shfl_sync(0xffffffffu, own_pos, (2 * t + e) * 4);
+        }
     }
 
-    const int* table = p.page_table + (long long)r * p.table_width;
-    const long long head_keys = (long long)p.page_size;  // keys of one head in a page
-    // key `j` of the request as an index over [pages, 2, KV, page_size]
-    auto place = [&](int j) -> long long {
-        j = min(j, key_end - 1);  // behind the end: some key that is there, masked later
-        const int at = j / p.page_size;
-        const int page = min(max(table[at], 0), p.pages - 1);
-        return ((long long)page * 2 * p.KV + h) * head_keys + (j - at * p.page_size);
-    };
-    const long long to_values = (long long)p.KV * head_keys;
-    auto fetch = [&](Keys<D>& x, int tile) {
-        const int j0 = tile * TILE;
-        if constexpr (ALIGNED) {
-            const long long base = place(j0);
-            const unsigned char* kp = p.pool + base * D;
-            const unsigned char* vp = kp + to_values * D;
+    // o[nt][x]: lanes (D / 8) g + 2 x (+ 1) of the head, rows 2 t, 2 t + 1 of tile nt: [lane][row]
+    float o[NT][MTILES][4], m1[NT][2], m2[NT][2], sum[NT][2];  // sum: this thread's keys alone
 #pragma unroll
-            for (int i = 0; i < 2; ++i) load_words(x.k[i], kp + (g + 8 * i) * D + 16 * t);
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_words(x.v[i], vp + (2 * t + (i & 1) + 8 * (i >> 1)) * D + (D / 8) * g);
-            const unsigned char* ep = p.exponents + base + 2 * t;
+        for (int x = 0; x < MTILES; ++x)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x.ek[i] = __ldg(reinterpret_cast<const unsigned short*>(ep + 8 * i));
-                x.ev[i] = __ldg(reinterpret_cast<const unsigned short*>(ep + to_values + 8 * i));
-            }
-        } else {
+            for (int e = 0; e < 4; ++e) o[nt][x][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) load_words(x.k[i], p.pool + place(j0 + g + 8 * i) * D + 16 * t);
+        for (int e = 0; e < 2; ++e) m1[nt][e] = m2[nt][e] = NOTHING, sum[nt][e] = 0.f;
+    }
+
+    // tiles that begin in here are seen whole by every row
+    const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
+    int slot = 0;  // i0 % STAGES
+    for (int i0 = 0; i0 < mine; ++i0) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();  // the exponents are other lanes' copies; and everyone has read the stage that is filled next
+        if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        const int j0 = (tile_lo + warp + i0 * WARPS) * TILE;
+        const unsigned char* stage = ring_at + slot * S::BYTES;
+        slot = slot == STAGES - 1 ? 0 : slot + 1;
+
+        // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
+        float s[NT][4], lower[NT][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                unsigned ek = 0, ev = 0;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const long long at = place(j0 + 2 * t + 8 * i + e);
-                    load_words(x.v[2 * i + e], p.pool + (at + to_values) * D + (D / 8) * g);
-                    ek |= (unsigned)__ldg(p.exponents + at) << (8 * e);
-                    ev |= (unsigned)__ldg(p.exponents + at + to_values) << (8 * e);
-                }
-                x.ek[i] = ek;
-                x.ev[i] = ev;
+            for (int e = 0; e < 4; ++e) s[nt][e] = lower[nt][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < S::K_PIECES / 2; ++c) {
+            const uint4 k0 = *reinterpret_cast<const uint4*>(stage + c * 512 + lane * 16);
+            const uint4 k1 = *reinterpret_cast<const uint4*>(stage + (S::K_PIECES / 2 + c) * 512 + lane * 16);
+            const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_e4m3(s[nt], a0, qb[nt][2 * c][0][0], qb[nt][2 * c][0][1]);
+                mma_e4m3(lower[nt], a0, qb[nt][2 * c][1][0], qb[nt][2 * c][1][1]);
+                mma_e4m3(s[nt], a1, qb[nt][2 * c + 1][0][0], qb[nt][2 * c + 1][0][1]);
+                mma_e4m3(lower[nt], a1, qb[nt][2 * c + 1][1][0], qb[nt][2 * c + 1][1][1]);
             }
         }
-    };
-
-    float o[NTILES][4];
+        unsigned v[4][S::V_BYTES / 4];
 #pragma unroll
-    for (int i = 0; i < NTILES; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m1[2] = {-INFINITY, -INFINITY}, m2[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // sum: this thread's keys alone
-
-    Keys<D> now, next;
-    int tile = tile_lo + warp;
-    if (tile < tile_hi) fetch(now, tile);
-    for (; tile < tile_hi; tile += WARPS) {
-        if (tile + WARPS < tile_hi) fetch(next, tile + WARPS);
-        const int j0 = tile * TILE;
-        // ---- scores: [row g | g + 8][key 2 t, 2 t + 1, 2 t + 8, 2 t + 9] ----
-        float s[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < KSTEPS; ++j)
-                mma_f16(c, qa[j], half2_of((unsigned short)now.k[i][j]), half2_of((unsigned short)(now.k[i][j] >> 16)));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float ks = __uint_as_float(((now.ek[i] >> (8 * e)) & 255u) << 23);
-                s[0][2 * i + e] = c[e] * (ks * factor[0]);
-                s[1][2 * i + e] = c[2 + e] * (ks * factor[1]);
+        for (int e = 0; e < 4; ++e) {
+            const unsigned char* at = stage + S::KEYS + e * 32 * S::V_BYTES + lane * S::V_BYTES;
+            if constexpr (S::V_BYTES == 16) {
+                const uint4 w = *reinterpret_cast<const uint4*>(at);
+                v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(at);
+                v[e][0] = w.x, v[e][1] = w.y;
             }
         }
-        const bool whole = j0 + TILE - 1 <= pos_min && j0 + TILE <= key_end && (p.window <= 0 || j0 > pos_max - p.window);
-        bool split_rows = false;  // some row sees a key of this tile that another does not
-        if (!whole) {
+        float ev[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* at = stage + S::KEYS + S::VALUES + g + 8 * x;
+            const float ks = __uint_as_float((unsigned)at[0] << 23);
+            ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) s[nt][2 * x + e] = (s[nt][2 * x + e] + lower[nt][2 * x + e]) * (ks * factor[nt][e]);
+        }
+        if (j0 < whole_from || j0 > whole_to) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int j = j0 + g + 8 * x;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (j > pos[nt][e] || j >= key_end || (p.window > 0 && j <= pos[nt][e] - p.window)) s[nt][2 * x + e] = -INFINITY;
+            }
+            // a value that no row of the tile sees is nobody's
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (j > pos[i] || j >= key_end || (p.window > 0 && j <= pos[i] - p.window)) s[i][e] = -INFINITY;
-                // a value that no row of the tile sees is nobody's
                 if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
 #pragma unroll
-                    for (int w = 0; w < Keys<D>::VW; ++w) now.v[e][w] = 0u;
+                    for (int w = 0; w < S::V_BYTES / 4; ++w) v[e][w] = 0u;
                 }
             }
-            split_rows = pos_min != pos_max;
-        }
-        // ---- running maxima and weights ----
-        unsigned pa[4];
-        float u[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float ev = (float)((now.ev[e >> 1] >> (8 * (e & 1))) & 255u) - 127.f;
-                u[i][e] = s[i][e] + ev;
-                a = fmaxf(a, s[i][e]);
-                b = fmaxf(b, u[i][e]);
-            }
-            a = fmaxf(m1[i], quad_max(a));
-            b = fmaxf(m2[i], quad_max(b));
-            const float a0 = a == -INFINITY ? 0.f : a, b0 = b == -INFINITY ? 0.f : b;
-            const float keep = exp2_fast(m2[i] - b0);
-            sum[i] *= exp2_fast(m1[i] - a0);
-            m1[i] = a;
-            m2[i] = b;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum[i] += exp2_fast(s[i][e] - a0);
-                u[i][e] = exp2_fast(u[i][e] - b0);
-            }
-#pragma unroll
-            for (int x = 0; x < NTILES; ++x) {
-                o[x][2 * i] *= keep;
-                o[x][2 * i + 1] *= keep;
-            }
-        }
-        pa[0] = pack_half(u[0][0], u[0][1]);
-        pa[1] = pack_half(u[1][0], u[1][1]);
-        pa[2] = pack_half(u[0][2], u[0][3]);
-        pa[3] = pack_half(u[1][2], u[1][3]);
-        // ---- values: column tile x takes lane (D / 8) g + x of every key ----
-        bool nan_here = false;
-        if (split_rows) {
-            unsigned any = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int w = 0; w < Keys<D>::VW; ++w) any |= __vcmpeq4(now.v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            nan_here = __any_sync(0xffffffffu, any != 0);
-        }
-        if (nan_here) {
-            // NaN times a weight of zero is NaN: its places are taken out and counted by a product of their own, of ones where a
-            // row sees a key and where a value is NaN
-            unsigned seen[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int i = q & 1, e = 2 * (q >> 1);
-                seen[q] = (s[i][e] == -INFINITY ? 0u : 0x3c00u) | (s[i][e + 1] == -INFINITY ? 0u : 0x3c000000u);
-            }
-#pragma unroll
-            for (int x = 0; x < NTILES; ++x) {
-                unsigned bad[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const unsigned lo = (now.v[2 * q][x / 4] >> (8 * (x & 3))) & 0x7fu, hi = (now.v[2 * q + 1][x / 4] >> (8 * (x & 3))) & 0x7fu;
-                    bad[q] = (lo == 0x7fu ? 0x3c00u : 0u) | (hi == 0x7fu ? 0x3c000000u : 0u);
-                }
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(c, seen, bad[0], bad[1]);
+            if (pos_min != pos_max) {
+                // Some row may see a key that another does not, and NaN times a weight of zero is NaN: NaN among the values is taken out and
+                // counted by a product of its own, of ones where a value is NaN and where a row sees a key.
+                unsigned any = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (c[e] > 0.f) o[x][e] = NAN;
+#pragma unroll
+                    for (int w = 0; w < S::V_BYTES / 4; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        unsigned seen[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            seen[x] = transpose((s[nt][2 * x] == -INFINITY ? 0u : 0x3c00u) | (s[nt][2 * x + 1] == -INFINITY ? 0u : 0x3c000000u));
+#pragma unroll
+                        for (int x = 0; x < MTILES; ++x) {
+                            unsigned bad[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {  // lane byte 2 x + (q & 1), keys 2 t + 8 (q >> 1) and the next
+                                const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
+                                bad[q] = (((v[e][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c00u : 0u) |
+                                         (((v[e + 1][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c000000u : 0u);
+                            }
+                            float c[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(c, bad, seen[0], seen[1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c[e] > 0.f) o[nt][x][e] = NAN;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int w = 0; w < S::V_BYTES / 4; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                }
+            }
+        }
+        // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
+        // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
+        unsigned pb[NT][2];
+        float u[NT][4];
+        bool behind = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[nt][e] = s[nt][e] + ev[e >> 1];
+                behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
+            }
+        if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
+                    const float keep = exp2_fast(m2[nt][e] - b);
+                    sum[nt][e] *= exp2_fast(m1[nt][e] - a);
+                    m1[nt][e] = a;
+                    m2[nt][e] = b;
+#pragma unroll
+                    for (int x = 0; x < MTILES; ++x) {
+                        o[nt][x][e] *= keep;
+                        o[nt][x][2 + e] *= keep;
+                    }
+                }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sum[nt][e] += exp2_fast(s[nt][e] - m1[nt][e]) + exp2_fast(s[nt][2 + e] - m1[nt][e]);
+                u[nt][e] = exp2_fast(u[nt][e] - m2[nt][e]);
+                u[nt][2 + e] = exp2_fast(u[nt][2 + e] - m2[nt][e]);
+            }
+            pb[nt][0] = transpose(pack_half(u[nt][0], u[nt][1]));
+            pb[nt][1] = transpose(pack_half(u[nt][2], u[nt][3]));
+        }
+        // ---- values: tile x takes bytes 2 x and 2 x + 1 of the thread's of every key ----
+#pragma unroll
+        for (int x = 0; x < MTILES; ++x) {
+            unsigned a[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
+                a[q] = half2_of((unsigned short)__byte_perm(v[e][b / 4], v[e + 1][b / 4], 0x0040u + 0x0011u * (b & 3)));
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int w = 0; w < Keys<D>::VW; ++w) now.v[e][w] &= ~__vcmpeq4(now.v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][x], a, pb[nt][0], pb[nt][1]);
         }
-#pragma unroll
-        for (int x = 0; x < NTILES; ++x) {
-            const unsigned pick = 0x0040u + 0x0011u * (x & 3);  // byte x of the first word, byte x of the second
-            const unsigned b0 = __byte_perm(now.v[0][x / 4], now.v[1][x / 4], pick), b1 = __byte_perm(now.v[2][x / 4], now.v[3][x / 4], pick);
-            mma_f16(o[x], pa, half2_of((unsigned short)b0), half2_of((unsigned short)b1));
-        }
-        now = next;
     }
 
-    // ---- the warps meet ----
-    float* mine = merge + (size_t)warp * 16 * (D + 4);
-    float* stats = merge + (size_t)WARPS * 16 * (D + 4);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        if (t == 0) {
-            float* at = stats + (warp * 16 + g + 8 * i) * 3;
-            at[0] = m1[i];
-            at[1] = m2[i];
-            at[2] = sum[i];
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < NTILES; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // column 2 t + (e & 1) of tile x is lane (D / 8) (2 t + (e & 1)) + x of the head
-            mine[(g + 8 * (e >> 1)) * (D + 4) + (D / 8) * (2 * t + (e & 1)) + x] = o[x][e];
+    // ---- the warps meet, where the rings were ----
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += THREADS) {
-        const int row = i / (D / 4), c = (i - row * (D / 4)) * 4;
-        const int rho = row0 + row;
-        if (rho >= rows) continue;
-        float a = -INFINITY, b = -INFINITY;
+    float* merge = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], x);
+            const int row = 8 * nt + 2 * t + e;
+            if (row0 + row >= rows) continue;
+            if (g == 0) {
+                stats[warp][row][0] = m1[nt][e];
+                stats[warp][row][1] = m2[nt][e];
+                stats[warp][row][2] = sum[nt][e];
+            }
+            // lanes (D / 8) g + 2 x, + 1 at columns 16 x + 2 g, + 1: the warp's stores meet in no bank
+            float* at = merge + ((size_t)warp * ROWS + row) * PITCH + 2 * g;
+#pragma unroll
+            for (int x = 0; x < MTILES; ++x) *reinterpret_cast<float2*>(at + 16 * x) = make_float2(o[nt][x][e], o[nt][x][2 + e]);
+        }
+    __syncthreads();
+    const int live_rows = min(ROWS, rows - row0);
+    for (int i = threadIdx.x; i < live_rows * (D / 2); i += THREADS) {
+        const int row = i / (D / 2), c = (i - row * (D / 2)) * 2;
+        float a = NOTHING, b = NOTHING;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            a = fmaxf(a, stats[(w * 16 + row) * 3]);
-            b = fmaxf(b, stats[(w * 16 + row) * 3 + 1]);
+            a = fmaxf(a, stats[w][row][0]);
+            b = fmaxf(b, stats[w][row][1]);
         }
-        const float a0 = a == -INFINITY ? 0.f : a, b0 = b == -INFINITY ? 0.f : b;
-        float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        float total = 0.f, y0 = 0.f, y1 = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float* st = stats + (w * 16 + row) * 3;
-            const float f = exp2_fast(st[1] - b0);
-            total += st[2] * exp2_fast(st[0] - a0);
-            const float4 x = *reinterpret_cast<const float4*>(merge + ((size_t)w * 16 + row) * (D + 4) + c);
-            v[0] = fmaf(x.x, f, v[0]);
-            v[1] = fmaf(x.y, f, v[1]);
-            v[2] = fmaf(x.z, f, v[2]);
-            v[3] = fmaf(x.w, f, v[3]);
+            total += stats[w][row][2] * exp2_fast(stats[w][row][0] - a);
+            const float f = exp2_fast(stats[w][row][1] - b);
+            const float2 x = *reinterpret_cast<const float2*>(merge + ((size_t)w * ROWS + row) * PITCH + c);
+            y0 = fmaf(x.x, f, y0);
+            y1 = fmaf(x.y, f, y1);
         }
-        const int tok = first + rho / p.G, hd = h * p.G + rho % p.G;
-        if (p.splits == 1) {
-            // a row that sees no key: zeros
-            const float f = a == -INFINITY && total == 0.f ? 0.f : exp2f(b0 - a0) / total;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= f;
-            store4(p.out + tok * p.out_stride + (long long)hd * D + c, v);
+        if (part < 0) {
+            finish<D>(p, first, h, row0 + row, c, a, b, total, y0, y1);
         } else {
-            const long long at = ((long long)tok * p.H + hd) * p.splits + split;
-            store4(p.part_o + at * D + c, v);
+            *reinterpret_cast<float2*>(p.part_sums + ((size_t)part * ROWS + row) * PITCH + c) = make_float2(y0, y1);
             if (c == 0) {
-                p.part_stat[at * 3] = a;
-                p.part_stat[at * 3 + 1] = b;
-                p.part_stat[at * 3 + 2] = total;
+                float* st = p.part_stats + ((size_t)part * ROWS + row) * 3;
+                st[0] = a;
+                st[1] = b;
+                st[2] = total;
             }
         }
+    }
+    __syncthreads();  // the rings are filled again
     }
 }
 
-// Joins the splits of every row: D / 4 threads a row.
-template <int D>
-__global__ void __launch_bounds__(128)
-attention8_join_kernel(const Attn8Params p, long long rows) {
-    constexpr int LANES = D / 4;
+// Joins what stretches left of a tile of rows that no stretch held alone: GROUPS groups of threads take every GROUPS-th stretch each.
+template <int D, int NT>
+__global__ void __launch_bounds__(JOIN_THREADS)
+attention8_join_kernel(const Attn8Params p) {
+    constexpr int ROWS = 8 * NT, PITCH = D + 4, COLS = ROWS * (D / 4), GROUPS = JOIN_THREADS / (8 * (D / 4));
+    __shared__ long long begins[MAX_REQUESTS + 1];
+    __shared__ float references[ROWS][2];
+    __shared__ float4 sums[GROUPS][8 * (D / 4)];
+    __shared__ float totals[GROUPS][ROWS];
+    const int r = blockIdx.x / p.KV, h = blockIdx.x - r * p.KV, row0 = blockIdx.y * ROWS;
+    // The step's arrays are older than the kernel in front, which began behind everything before it: where the parts are is worked
+    // out while that one runs.
+    const int first = p.cu_tokens[r], rows = (p.cu_tokens[r + 1] - first) * p.G, live_rows = min(ROWS, rows - row0);
+    const Share share = share_of<ROWS>(p, r);
+    lay_out<ROWS>(p, begins);
+    const long long total = begins[p.requests], from = begins[r] + (long long)(h * share.row_tiles + blockIdx.y) * share.tiles;
+    int c0 = 0, c1 = -1;  // the stretches that hold a tile of these rows
+    if (live_rows > 0 && share.tiles) {
+        const int count = stretches(p, total);
+        c0 = (int)(from * count / total);
+        while (total * (c0 + 1) / count <= from) ++c0;
+        c1 = c0;
+        while (total * (c1 + 1) / count < from + share.tiles) ++c1;
+    }
     pdl_wait();
     pdl_trigger();
-    const long long row = (long long)blockIdx.x * (128 / LANES) + threadIdx.x / LANES;
-    if (row >= rows) return;
-    const int c = (threadIdx.x % LANES) * 4;
-    const float* stat = p.part_stat + row * p.splits * 3;
-    float a = -INFINITY, b = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) {
-        a = fmaxf(a, stat[s * 3]);
-        b = fmaxf(b, stat[s * 3 + 1]);
+    if (live_rows <= 0 || (share.tiles && c0 == c1)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto place = [&](int k, int row) { return (size_t)(2 * k + (k == c0)) * ROWS + row; };
+    for (int row = warp; row < live_rows; row += JOIN_THREADS / 32) {
+        float a = NOTHING, b = NOTHING;
+        for (int k = c0 + lane; k <= c1; k += 32) {
+            a = fmaxf(a, p.part_stats[place(k, row) * 3]);
+            b = fmaxf(b, p.part_stats[place(k, row) * 3 + 1]);
+        }
+        a = warp_max(a);
+        b = warp_max(b);
+        if (lane == 0) {
+            references[row][0] = a;
+            references[row][1] = b;
+        }
     }
-    const float a0 = a == -INFINITY ? 0.f : a, b0 = b == -INFINITY ? 0.f : b;
-    float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2_fast(stat[s * 3 + 1] - b0);
-        total += stat[s * 3 + 2] * exp2_fast(stat[s * 3] - a0);
-        float x[4];
-        load4(p.part_o + (row * p.splits + s) * D + c, x);
+    __syncthreads();
+    const int group = threadIdx.x / (8 * (D / 4)), col = threadIdx.x - group * (8 * (D / 4));
+    for (int i0 = 0; i0 < COLS; i0 += 8 * (D / 4)) {
+        const int row = (i0 + col) / (D / 4), c = (i0 + col - row * (D / 4)) * 4;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float weights = 0.f;
+        if (row < live_rows) {
+            const float a = references[row][0], b = references[row][1];
+#pragma unroll 4
+            for (int k = c0 + group; k <= c1; k += GROUPS) {
+                const size_t at = place(k, row);
+                const float s0 = p.part_stats[at * 3], s1 = p.part_stats[at * 3 + 1], s2 = p.part_stats[at * 3 + 2];
+                const float4 x = *reinterpret_cast<const float4*>(p.part_sums + at * PITCH + c);
+                const float f = exp2_fast(s1 - b);
+                weights += s2 * exp2_fast(s0 - a);
+                y.x = fmaf(x.x, f, y.x);
+                y.y = fmaf(x.y, f, y.y);
+                y.z = fmaf(x.z, f, y.z);
+                y.w = fmaf(x.w, f, y.w);
+            }
+            sums[group][col] = y;
+            if (c == 0) totals[group][row] = weights;
+        }
+        __syncthreads();
+        if (group == 0 && row < live_rows) {
+            weights = totals[0][row];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+            for (int k = 1; k < GROUPS; ++k) {
+                const float4 x = sums[k][col];
+                y.x += x.x;
+                y.y += x.y;
+                y.z += x.z;
+                y.w += x.w;
+                weights += totals[k][row];
+            }
+            finish<D>(p, first, h, row0 + row, c, references[row][0], references[row][1], weights, y.x, y.y);
+            finish<D>(p, first, h, row0 + row, c + 2, references[row][0], references[row][1], weights, y.z, y.w);
+        }
+        __syncthreads();
     }
-    const float f = a == -INFINITY && total == 0.f ? 0.f : exp2f(b0 - a0) / total;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= f;
-    const long long tok = row / p.H;
-    store4(p.out + tok * p.out_stride + (row - tok * p.H) * D + c, v);
 }
 
-template <int D, bool ALIGNED>
-int launch(const Attn8Params& p, int requests, int n, int longest, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)WARPS * 16 * (D + 4 + 3) * sizeof(float);
-    const long long row_tiles = ((long long)longest * p.G + 15) / 16;
-    if (row_tiles > 65535 || p.splits > 65535 || (long long)requests * p.KV > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
-    auto kernel = attention8_kernel<D, ALIGNED>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-    }
-    const int code = launch_pdl(kernel, dim3(requests * p.KV, (unsigned)row_tiles, p.splits), dim3(THREADS), smem, stream, p);
-    if (code || p.splits == 1) return code;
-    const long long rows = (long long)n * p.H, per = 128 / (D / 4), blocks = (rows + per - 1) / per;
-    if (blocks > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
-    return launch_pdl(attention8_join_kernel<D>, dim3((unsigned)blocks), dim3(128), 0, stream, p, rows);
+template <int D, int NT, bool EIGHTS>
+int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
+    constexpr size_t ring = (size_t)WARPS * STAGES * Stage<D>::BYTES, merge = (size_t)WARPS * 8 * NT * (D + 4) * sizeof(float);
+    constexpr size_t smem = ring > merge ? ring : merge;
+    const long long row_tiles = ((long long)longest * p.G + 8 * NT - 1) / (8 * NT), pairs = (long long)p.requests * p.KV;
+    if (row_tiles > 65535 || pairs > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
+    const cudaError_t e = cudaFuncSetAttribute(attention8_kernel<D, NT, EIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
+    if (e != cudaSuccess) return (int)e;
+    const dim3 units((unsigned)pairs, (unsigned)row_tiles);
+    const int code = launch_pdl(attention8_kernel<D, NT, EIGHTS>, p.ranges ? dim3(p.ranges) : units, dim3(THREADS), smem, stream, p);
+    if (code || !p.ranges) return code;
+    return launch_pdl(attention8_join_kernel<D, NT>, units, dim3(JOIN_THREADS), 0, stream, p);
 }
 
 }  // namespace
 
-// q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them; request r's
-// new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the most tokens a request
-// brings.  out [n, H D].  splits > 1: part_o [n H splits D] and part_stat [n H splits 3] float32.  window 0: none.  D 64 or 128.
+// Rows of a tile for `longest` tokens a request and G query heads a key head: the sums that a stretch leaves are [2][rows][D + 4 + 3] floats.
+LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longest * G <= 8 ? 8 : 16; }
+
+// q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, on 16
+// bytes; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
+// most tokens a request brings.  out [n, H D].  window 0: none.  ranges: CTAs that share the step's keys evenly, with scratch memory of
+// ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and tile of rows.  D 64 or 128.
 LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long long out_stride, const void* pool, const void* exponents,
                               const int* page_table, int table_width, const int* cu_tokens, const int* context_lens, int requests, int n,
-                              int longest, int H, int KV, int D, int page_size, int pages, int window, float scale, int splits, float* part_o,
-                              float* part_stat, cudaStream_t stream) {
+                              int longest, int H, int KV, int D, int page_size, int pages, int window, float scale, int ranges, float* scratch,
+                              cudaStream_t stream) {
     if (n <= 0 || requests <= 0) return 0;
-    if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || splits <= 0 || window < 0 ||
-        (splits > 1 && (!part_o || !part_stat)) || (q_stride & 3) || ((uintptr_t)q & 7) || (out_stride & 3) || ((uintptr_t)out & 7) ||
-        ((uintptr_t)pool & 15) || ((uintptr_t)exponents & 15))
+    if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || ranges < 0 || window < 0 ||
+        (ranges && (!scratch || requests > MAX_REQUESTS || ((uintptr_t)scratch & 15))) || (q_stride & 3) || ((uintptr_t)q & 7) ||
+        (out_stride & 3) || ((uintptr_t)out & 7) || ((uintptr_t)pool & 15) || ((uintptr_t)exponents & 15) ||
+        (long long)table_width * page_size > 0x7fff0000)
         return LLM_ERR_BAD_ARGUMENT;
+    const int rows = llm_attention8_rows(longest, H / KV);
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
-                     page_table, table_width, cu_tokens, context_lens, H, KV, H / KV, page_size, pages, window, splits,
-                     scale * 1.4426950408889634f, part_o, part_stat};
-    const bool aligned = page_size % TILE == 0;
-    if (D == 64) return aligned ? launch<64, true>(p, requests, n, longest, stream) : launch<64, false>(p, requests, n, longest, stream);
-    if (D == 128) return aligned ? launch<128, true>(p, requests, n, longest, stream) : launch<128, false>(p, requests, n, longest, stream);
+                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, ranges,
+                     scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};
+    // places are counted in eights, in 32 bits
+    const bool eights = page_size % 8 == 0 && (long long)pages * 2 * KV * (page_size / 8) <= 0xffffffffLL;
+#define ATTENTION8(D_) \
+    (eights ? rows == 8 ? launch<D_, 1, true>(p, longest, stream) : launch<D_, 2, true>(p, longest, stream) \
+            : rows == 8 ? launch<D_, 1, false>(p, longest, stream) : launch<D_, 2, false>(p, longest, stream))
+    if (D == 64) return ATTENTION8(64);
+    if (D == 128) return ATTENTION8(128);
+#undef ATTENTION8
     return LLM_ERR_UNSUPPORTED;
 }

@@ -96,7 +96,7 @@ _SIGNATURES = {
     "llm_linear8_few": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "llm_gemm8_tcgen05": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
+    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
 }
 
@@ -2442,8 +2442,8 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
 def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tensor, page_table: torch.Tensor, ctx, *, num_heads: int,
                      num_kv_heads: int, head_dim: int, scale: float, window: int | None = None) -> torch.Tensor:
     """:func:`paged_attention` over 8-bit pages as :func:`rope_kv_write8` leaves them.  ``q`` rows (bfloat16) start with the rotated query
-    heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  The keys of a request are split
-    over CTAs where the step has few rows, and joined by a second kernel.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
+    heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  Where requests may be
+    long their keys are spread evenly over the CTAs, wherever requests begin and end, and joined by a second kernel.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
     n = q.shape[0]
     _need(q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= num_heads * head_dim, "paged_attention8: rows of q start with the query heads, bfloat16")
     _need(q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0, "paged_attention8: rows of q start on 8 bytes")
@@ -2461,21 +2461,27 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
         return out
     longest = getattr(ctx, "max_query_len", None) or max(_token_counts(ctx))
     keys = getattr(ctx, "max_context_len", None) or int(ctx.context_lens.max())
-    splits = _attention8_splits(requests * num_kv_heads * -(-longest * (num_heads // num_kv_heads) // 16), keys if window is None else min(keys, window + longest), n * num_heads * head_dim)
-    part_o = part_stat = None
-    if splits > 1:
-        part_o = torch.empty((n * num_heads * splits * head_dim,), dtype=torch.float32, device=q.device)
-        part_stat = torch.empty((n * num_heads * splits * 3,), dtype=torch.float32, device=q.device)
+    group = num_heads // num_kv_heads
+    ranges = _attention8_ranges(requests, num_kv_heads, longest * group, keys if window is None else min(keys, window + longest))
+    scratch = None
+    if ranges:
+        scratch = torch.empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32, device=q.device)
+        add_launches(1)
     code = _launch("llm_attention8", _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(pool), _ptr(exponents), _ptr(page_table), page_table.shape[1],
                    _ptr(ctx.cu_tokens), _ptr(ctx.context_lens), requests, n, longest, num_heads, num_kv_heads, head_dim, pool.shape[3],
-                   pool.shape[0], int(window or 0), float(scale), splits, _ptr(part_o), _ptr(part_stat), _stream())
-    add_launches(splits > 1)
+                   pool.shape[0], int(window or 0), float(scale), ranges, _ptr(scratch), _stream())
     _check(code, "paged_attention8")
     return out
 
 
-def _attention8_splits(tiles: int, keys: int, elements: int) -> int:
-    """CTAs that share the keys of a row tile: as many as there is room for at once, none with fewer than 64 keys, and their
-    partial results bounded."""
-    splits = min(2 * _sm_count() // tiles, -(-keys // 64), _SPLIT_SCRATCH_BYTES // (4 * elements))
-    return max(1, splits)
+_ATTENTION8_RANGES: int | None = None  # for measurements: so many whatever the rule says
+
+
+def _attention8_ranges(requests: int, kv_heads: int, rows: int, keys: int) -> int:
+    """Over how many CTAs a step's keys are spread evenly (0: a CTA takes a tile of rows with all its keys): as many as there is room for at
+    once, where requests may be long."""
+    if _ATTENTION8_RANGES is not None:
+        return _ATTENTION8_RANGES
+    if keys <= 256 or requests > 1024:
+        return 0
+    return _sm_count() * (2 if rows <= 8 else 1)
