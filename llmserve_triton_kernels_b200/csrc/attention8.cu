@@ -20,12 +20,15 @@
 // equal stretch of it, wherever requests begin and end (their lengths are the device's business: a captured step is replayed at any
 // lengths).  A CTA's stretch is cut into segments, one for each tile of rows that it touches; a segment that holds all keys of its
 // rows writes their outputs, one that holds some leaves its sums in the call's scratch memory, and a second kernel joins those.
-// Within a segment the tiles go round the CTA's warps; a warp's tiles come through a ring of its own in shared memory (cp.async, a
-// thread reads back what it asked for itself, so nobody waits for anybody), and the warps meet once, in shared memory.
+// Within a segment the tiles go round the CTA's warps; a warp's tiles come through a ring of its own in shared memory, and the warps meet
+// once, in shared memory.  The ring is filled by TMA, swizzled so that neither keys nor values meet in a bank.  A page holds a head's keys
+// side by side, and their values a fixed distance behind, so one box is a tile's keys and values (where pages hold tiles whole; two
+// boxes of eight keys where they hold eights): four boxes, or copies by the threads, cost a warp some 600 cycles a tile to ask for.
 //
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
 // Where rows differ in what they see, NaN among the values is counted apart, so that it reaches the rows that see it alone.
 #include "fp8.cuh"
+#include "tma.cuh"
 
 namespace {
 
@@ -45,6 +48,7 @@ struct Attn8Params {
     const int* cu_tokens;
     const int* context_lens;
     int requests, H, KV, G, page_size, pages, window;
+    int* error_flag;
     int ranges;         // stretches of the step's list of tiles at most; 0: a CTA takes a tile of rows with all its keys
     float scale;        // times log2 e
     float* part_sums;   // [ranges][2][ROWS][D + 4]: what a stretch holds of the rows at its beginning and at its end,
@@ -87,12 +91,14 @@ __device__ __forceinline__ unsigned transpose(unsigned v) {
     return r;
 }
 
-// A stage of a warp's ring, 16 keys: [piece][lane] of what the threads hold (D / 4 bytes of keys g and g + 8, D / 8 bytes of the values
-// 2 t, 2 t + 1, 2 t + 8, 2 t + 9), then the exponents of the keys and of the values.
-template <int D>
+// A stage of a warp's ring: a tile's keys and values in runs of RUN keys (8 or 16): [run][keys, values][RUN][D bytes], the 16-byte chunks
+// of a row swizzled as TMA does it.
+template <int D, int RUN>
 struct Stage {
-    static constexpr int K_PIECES = D / 32, V_BYTES = D / 8;  // 16-byte pieces of both keys; bytes of a value
-    static constexpr int KEYS = K_PIECES * 512, VALUES = 4 * 32 * V_BYTES, BYTES = KEYS + VALUES + 2 * TILE;
+    static constexpr int BYTES = 2 * TILE * D, VALUES = RUN * D, SECOND = RUN == 8 ? 16 * D : 8 * D;  // to the values; to keys 8 .. 15
+    static constexpr CUtensorMapSwizzle SWIZZLE = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    static __device__ __forceinline__ int chunk(int row, int c) { return (D == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) * 16; }
+    static __device__ __forceinline__ int key(int row, int c) { return (row >> 3) * SECOND + (row & 7) * D + chunk(row, c); }
 };
 
 template <int BYTES>
@@ -161,18 +167,28 @@ __device__ __forceinline__ int stretches(const Attn8Params& p, long long total) 
     return (int)max(1LL, min((long long)p.ranges, total / WARPS));
 }
 
-// EIGHTS: pages hold whole runs of eight keys, so that a tile is two runs with one place each.
-template <int D, int NT, bool EIGHTS>
+// RUN: pages hold whole runs of 8 or 16 keys; 0: they do not, and the threads copy every key from its own place.
+template <int D, int NT, int RUN>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
-attention8_kernel(const Attn8Params p) {
+attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) {
     constexpr int KSTEPS = D / 32, MTILES = D / 16, ROWS = 8 * NT, PITCH = D + 4;
-    using S = Stage<D>;
-    extern __shared__ __align__(16) unsigned char smem[];  // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
-    __shared__ float stats[WARPS][ROWS][3];                // largest score, largest score with the value's scale, sum of weights
+    using S = Stage<D, RUN ? RUN : TILE>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
+    __shared__ float stats[WARPS][ROWS][3];  // largest score, largest score with the value's scale, sum of weights
     __shared__ long long begins[MAX_REQUESTS + 1];
+    __shared__ __align__(16) unsigned char scales[WARPS][STAGES][2 * TILE];  // exponents of a stage's keys and values
+    __shared__ __align__(8) unsigned long long full[WARPS][STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * STAGES * S::BYTES;
-    const unsigned char* ring_at = smem + warp * STAGES * S::BYTES;
+    unsigned char* ring = smem + warp * STAGES * S::BYTES;
+    if (RUN && lane == 0) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) tma::mbar_init(&full[warp][i], 1);
+        tma::mbar_fence_init();
+    }
+    __syncwarp();
+    int filled = 0;  // stages this warp has asked for: the barriers' phases go on from segment to segment
+    bool broken = false;
     pdl_wait();
     pdl_trigger();
     long long at = 0, end = 1;
@@ -232,55 +248,49 @@ attention8_kernel(const Attn8Params p) {
         return ((long long)page * 2 * p.KV + h) * p.page_size + (j - at * p.page_size);
     };
     const long long to_values = (long long)p.KV * p.page_size;
-    const unsigned char* my_keys = p.pool + (long long)g * D + 16 * t;  // what this thread holds of a run of eight keys, and of their values
-    const unsigned char* my_values = p.pool + (to_values + 2 * t) * D + S::V_BYTES * g;
-    unsigned run[2] = {0u, 0u};  // EIGHTS: this lane's tile of the next 32: the places of its two runs, in eights
+    int run[2] = {0, 0};  // this lane's tile of the next 32: the places of its runs
+    // a place behind the request's end is some place of the pool: what lies there is masked
     auto issue = [&](int i, int slot) {
         const int j0 = (tile_lo + warp + i * WARPS) * TILE;
-        const unsigned dst = ring + slot * S::BYTES;
-        // a place behind the request's end is some place of the pool: what lies there is masked
-        if constexpr (EIGHTS) {
+        unsigned char* dst = ring + slot * S::BYTES;
+        const unsigned scale_dst = tma::smem_addr(scales[warp][slot]);
+        if constexpr (RUN != 0) {
             if ((i & 31) == 0) {
                 const int j = j0 + lane * (WARPS * TILE);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) run[x] = j + 8 * x < key_end ? (unsigned)(place(j + 8 * x) >> 3) : 0u;
+                for (int x = 0; x < TILE / RUN; ++x) run[x] = j + 8 * x < key_end ? (int)place(j + 8 * x) : 0;
             }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const unsigned long long at = (unsigned long long)__shfl_sync(0xffffffffu, run[x], i & 31) * 8;
-                const unsigned char* kp = my_keys + at * D;
-                const unsigned char* vp = my_values + at * D;
-#pragma unroll
-                for (int c = 0; c < S::K_PIECES / 2; ++c) copy_async<16>(dst + (x * (S::K_PIECES / 2) + c) * 512 + lane * 16, kp + 64 * c);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) copy_async<S::V_BYTES>(dst + S::KEYS + (2 * x + e) * 32 * S::V_BYTES + lane * S::V_BYTES, vp + e * D);
-                if (lane < 2) copy_async<8>(dst + S::KEYS + S::VALUES + lane * TILE + 8 * x, p.exponents + at + lane * to_values);
+            // lanes 0 to 3 ask for the exponents of the keys' and the values' eights, lane 0 for the boxes
+            const int at0 = __shfl_sync(0xffffffffu, run[0], i & 31), at1 = RUN == 8 ? __shfl_sync(0xffffffffu, run[1], i & 31) : at0 + 8;
+            if (lane < 4) copy_async<8>(scale_dst + 8 * lane, p.exponents + ((lane & 1) ? at1 : at0) + (lane >> 1) * to_values);
+            if (lane == 0) {
+                tma::mbar_expect_tx(&full[warp][slot], S::BYTES);
+                tma::load_3d(dst, &map, 0, at0, 0, &full[warp][slot]);
+                if (RUN == 8) tma::load_3d(dst + S::SECOND, &map, 0, at1, 0, &full[warp][slot]);
             }
         } else {
             // lane l finds key l's place
             const bool is_there = j0 + (lane & 15) < key_end;
             const long long own = is_there ? place(j0 + (lane & 15)) : 0;
             const unsigned char exponent = is_there ? __ldg(p.exponents + own + (lane >> 4) * to_values) : 127;
-            asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(dst + S::KEYS + S::VALUES + lane), "r"((unsigned)exponent) : "memory");
+            asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(scale_dst + lane), "r"((unsigned)exponent) : "memory");
+            constexpr int CHUNKS = D / 16, AT_ONCE = 32 / CHUNKS;  // of a row; rows a copy
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const long long kp = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, g + 8 * x);
-#pragma unroll
-                for (int c = 0; c < S::K_PIECES / 2; ++c) copy_async<16>(dst + (x * (S::K_PIECES / 2) + c) * 512 + lane * 16, p.pool + kp * D + 16 * t + 64 * c);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const long long vp = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, 2 * t + e + 8 * x) + to_values;
-                    copy_async<S::V_BYTES>(dst + S::KEYS + (2 * x + e) * 32 * S::V_BYTES + lane * S::V_BYTES, p.pool + vp * D + S::V_BYTES * g);
-                }
+            for (int k = 0; k < TILE / AT_ONCE; ++k) {
+                const int row = k * AT_ONCE + lane / CHUNKS, c = lane % CHUNKS;
+                const long long key = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, row);
+                const unsigned to = tma::smem_addr(dst) + S::key(row, c);
+                copy_async<16>(to, p.pool + key * D + 16 * c);
+                copy_async<16>(to + S::VALUES, p.pool + (key + to_values) * D + 16 * c);
             }
         }
     };
     for (int i = 0; i < STAGES - 1; ++i) {
-        if (i < mine) issue(i, i);
+        if (i < mine) issue(i, (filled + i) % STAGES);
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     }
 
-    // ---- q: product j of a key takes lanes 64 (j / 2) + 16 t + 8 (j % 2) + 0 .. 7 of a row, as the keys' bytes lie ----
+    // ---- q: product j of a key takes lanes (D / 4) t + 8 j + 0 .. 7 of a row, as the keys' bytes lie ----
     unsigned qb[NT][KSTEPS][2][2];  // [upper, lower bits][first, second four lanes]
     float factor[NT][2];  // of this thread's rows, which are 2 t and 2 t + 1 of every tile in the products' results
     int pos[NT][2];
@@ -289,11 +299,11 @@ attention8_kernel(const Attn8Params p) {
         const int rho = row0 + 8 * nt + g;
         const bool live = rho < rows;
         const int token = live ? rho / p.G : 0, head = h * p.G + (live ? rho - token * p.G : 0);
-        const __nv_bfloat16* src = p.q + (first + token) * p.q_stride + (long long)head * D + 16 * t;
+        const __nv_bfloat16* src = p.q + (first + token) * p.q_stride + (long long)head * D + (D / 4) * t;
         unsigned raw[KSTEPS][4], top = 0;
 #pragma unroll
         for (int j = 0; j < KSTEPS; ++j) {
-            const __nv_bfloat16* at = src + 64 * (j / 2) + 8 * (j & 1);
+            const __nv_bfloat16* at = src + 8 * j;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const uint2 w = live ? *reinterpret_cast<const uint2*>(at + 4 * e) : make_uint2(0u, 0u);
@@ -356,57 +366,67 @@ attention8_kernel(const Attn8Params p) {
 
     // tiles that begin in here are seen whole by every row
     const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
-    int slot = 0;  // i0 % STAGES
-    for (int i0 = 0; i0 < mine; ++i0) {
+    for (int i0 = 0; i0 < mine; ++i0, ++filled) {
+        const int slot = filled % STAGES;
         asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
-        __syncwarp();  // the exponents are other lanes' copies; and everyone has read the stage that is filled next
+        if (RUN && !broken && !tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1)) broken = true;
+        __syncwarp();  // copies by other lanes have arrived; and everyone has read the stage that is filled next
         if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
         asm volatile("cp.async.commit_group;\n" ::: "memory");
         const int j0 = (tile_lo + warp + i0 * WARPS) * TILE;
-        const unsigned char* stage = ring_at + slot * S::BYTES;
-        slot = slot == STAGES - 1 ? 0 : slot + 1;
+        const unsigned char* stage = ring + slot * S::BYTES;
 
         // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
-        float s[NT][4], lower[NT][4];
+        // (four sums of products each, so that none waits for another for long)
+        float s[NT][4];
+        {
+            float c[NT][4][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = lower[nt][e] = 0.f;
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int c = 0; c < S::K_PIECES / 2; ++c) {
-            const uint4 k0 = *reinterpret_cast<const uint4*>(stage + c * 512 + lane * 16);
-            const uint4 k1 = *reinterpret_cast<const uint4*>(stage + (S::K_PIECES / 2 + c) * 512 + lane * 16);
-            const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+                    for (int e = 0; e < 4; ++e) c[nt][k][e] = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma_e4m3(s[nt], a0, qb[nt][2 * c][0][0], qb[nt][2 * c][0][1]);
-                mma_e4m3(lower[nt], a0, qb[nt][2 * c][1][0], qb[nt][2 * c][1][1]);
-                mma_e4m3(s[nt], a1, qb[nt][2 * c + 1][0][0], qb[nt][2 * c + 1][0][1]);
-                mma_e4m3(lower[nt], a1, qb[nt][2 * c + 1][1][0], qb[nt][2 * c + 1][1][1]);
+            for (int x = 0; x < D / 64; ++x) {
+                const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
+                const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
+                const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_e4m3(c[nt][0], a0, qb[nt][2 * x][0][0], qb[nt][2 * x][0][1]);
+                    mma_e4m3(c[nt][1], a0, qb[nt][2 * x][1][0], qb[nt][2 * x][1][1]);
+                    mma_e4m3(c[nt][2], a1, qb[nt][2 * x + 1][0][0], qb[nt][2 * x + 1][0][1]);
+                    mma_e4m3(c[nt][3], a1, qb[nt][2 * x + 1][1][0], qb[nt][2 * x + 1][1][1]);
+                }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = (c[nt][0][e] + c[nt][2][e]) + (c[nt][1][e] + c[nt][3][e]);
         }
-        unsigned v[4][S::V_BYTES / 4];
+        unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const unsigned char* at = stage + S::KEYS + e * 32 * S::V_BYTES + lane * S::V_BYTES;
-            if constexpr (S::V_BYTES == 16) {
-                const uint4 w = *reinterpret_cast<const uint4*>(at);
+            const int row = 2 * t + (e & 1) + 8 * (e >> 1);
+            if constexpr (D == 128) {
+                const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(row, g));
                 v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
             } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(at);
+                const uint2 w = *reinterpret_cast<const uint2*>(stage + S::VALUES + S::key(row, g >> 1) + (g & 1) * 8);
                 v[e][0] = w.x, v[e][1] = w.y;
             }
         }
         float ev[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const unsigned char* at = stage + S::KEYS + S::VALUES + g + 8 * x;
+            const unsigned char* at = scales[warp][slot] + g + 8 * x;
             const float ks = __uint_as_float((unsigned)at[0] << 23);
             ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) s[nt][2 * x + e] = (s[nt][2 * x + e] + lower[nt][2 * x + e]) * (ks * factor[nt][e]);
+                for (int e = 0; e < 2; ++e) s[nt][2 * x + e] *= ks * factor[nt][e];
         }
         if (j0 < whole_from || j0 > whole_to) {
 #pragma unroll
@@ -424,7 +444,7 @@ attention8_kernel(const Attn8Params p) {
                 const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
                 if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
 #pragma unroll
-                    for (int w = 0; w < S::V_BYTES / 4; ++w) v[e][w] = 0u;
+                    for (int w = 0; w < D / 32; ++w) v[e][w] = 0u;
                 }
             }
             if (pos_min != pos_max) {
@@ -434,7 +454,7 @@ attention8_kernel(const Attn8Params p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int w = 0; w < S::V_BYTES / 4; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    for (int w = 0; w < D / 32; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
                 if (__any_sync(0xffffffffu, any != 0)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -461,7 +481,7 @@ attention8_kernel(const Attn8Params p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int w = 0; w < S::V_BYTES / 4; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        for (int w = 0; w < D / 32; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
                 }
             }
         }
@@ -521,6 +541,12 @@ attention8_kernel(const Attn8Params p) {
 
     // ---- the warps meet, where the rings were ----
     asm volatile("cp.async.wait_all;\n" ::: "memory");
+    if (broken) {  // a wait gave up: the result is void; what is still on its way must land before the memory serves another end
+        if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
+        for (int i = max(0, filled - STAGES); i < filled; ++i) (void)tma::mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
+    }
+    // the rings were written by the other proxy too, and will be: order what threads do to the same places
+    if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     __syncthreads();
     float* merge = reinterpret_cast<float*>(smem);
 #pragma unroll
@@ -572,6 +598,7 @@ attention8_kernel(const Attn8Params p) {
             }
         }
     }
+    if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     __syncthreads();  // the rings are filled again
     }
 }
@@ -660,16 +687,19 @@ attention8_join_kernel(const Attn8Params p) {
     }
 }
 
-template <int D, int NT, bool EIGHTS>
+template <int D, int NT, int RUN>
 int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
-    constexpr size_t ring = (size_t)WARPS * STAGES * Stage<D>::BYTES, merge = (size_t)WARPS * 8 * NT * (D + 4) * sizeof(float);
-    constexpr size_t smem = ring > merge ? ring : merge;
+    constexpr size_t ring = (size_t)WARPS * STAGES * 2 * TILE * D, merge = (size_t)WARPS * 8 * NT * (D + 4) * sizeof(float);
+    constexpr size_t smem = (ring > merge ? ring : merge) + 1024;
     const long long row_tiles = ((long long)longest * p.G + 8 * NT - 1) / (8 * NT), pairs = (long long)p.requests * p.KV;
     if (row_tiles > 65535 || pairs > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
-    const cudaError_t e = cudaFuncSetAttribute(attention8_kernel<D, NT, EIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
+    const cudaError_t e = cudaFuncSetAttribute(attention8_kernel<D, NT, RUN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
+    CUtensorMap map = {};
+    const uint64_t values = (uint64_t)p.KV * p.page_size, keys = p.pages * 2 * values;  // a key's value lies so many places behind it
+    if (RUN && !tma::make_map_2d_u8_twice(&map, p.pool, keys - values, D, D, values * D, RUN, D, Stage<D, RUN ? RUN : TILE>::SWIZZLE)) return LLM_ERR_UNSUPPORTED;
     const dim3 units((unsigned)pairs, (unsigned)row_tiles);
-    const int code = launch_pdl(attention8_kernel<D, NT, EIGHTS>, p.ranges ? dim3(p.ranges) : units, dim3(THREADS), smem, stream, p);
+    const int code = launch_pdl(attention8_kernel<D, NT, RUN>, p.ranges ? dim3(p.ranges) : units, dim3(THREADS), smem, stream, p, map);
     if (code || !p.ranges) return code;
     return launch_pdl(attention8_join_kernel<D, NT>, units, dim3(JOIN_THREADS), 0, stream, p);
 }
@@ -686,7 +716,7 @@ LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longe
 LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long long out_stride, const void* pool, const void* exponents,
                               const int* page_table, int table_width, const int* cu_tokens, const int* context_lens, int requests, int n,
                               int longest, int H, int KV, int D, int page_size, int pages, int window, float scale, int ranges, float* scratch,
-                              cudaStream_t stream) {
+                              int* error_flag, cudaStream_t stream) {
     if (n <= 0 || requests <= 0) return 0;
     if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || ranges < 0 || window < 0 ||
         (ranges && (!scratch || requests > MAX_REQUESTS || ((uintptr_t)scratch & 15))) || (q_stride & 3) || ((uintptr_t)q & 7) ||
@@ -695,15 +725,13 @@ LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long
         return LLM_ERR_BAD_ARGUMENT;
     const int rows = llm_attention8_rows(longest, H / KV);
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
-                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, ranges,
+                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, error_flag, ranges,
                      scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};
-    // places are counted in eights, in 32 bits
-    const bool eights = page_size % 8 == 0 && (long long)pages * 2 * KV * (page_size / 8) <= 0xffffffffLL;
-#define ATTENTION8(D_) \
-    (eights ? rows == 8 ? launch<D_, 1, true>(p, longest, stream) : launch<D_, 2, true>(p, longest, stream) \
-            : rows == 8 ? launch<D_, 1, false>(p, longest, stream) : launch<D_, 2, false>(p, longest, stream))
-    if (D == 64) return ATTENTION8(64);
-    if (D == 128) return ATTENTION8(128);
+    // a tensor map's rows are counted in 32 bits
+    const int run = (long long)pages * 2 * KV * page_size > 0x7fffffffLL ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 0;
+#define ATTENTION8(D_, NT_) (run == 16 ? launch<D_, NT_, 16>(p, longest, stream) : run == 8 ? launch<D_, NT_, 8>(p, longest, stream) : launch<D_, NT_, 0>(p, longest, stream))
+    if (D == 64) return rows == 8 ? ATTENTION8(64, 1) : ATTENTION8(64, 2);
+    if (D == 128) return rows == 8 ? ATTENTION8(128, 1) : ATTENTION8(128, 2);
 #undef ATTENTION8
     return LLM_ERR_UNSUPPORTED;
 }

@@ -58,6 +58,20 @@ inline bool make_map_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, ui
               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// ... whose boxes hold the same rows of two such matrices, the second `apart` bytes (a multiple of 16) behind the first: laid down one
+// after the other.  Coordinates: (column, row, 0).
+inline bool make_map_2d_u8_twice(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t apart, uint32_t box_rows,
+                                 uint32_t box_cols, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {cols, rows, 2};
+    const cuuint64_t strides[2] = {ld, apart};
+    const cuuint32_t box[3] = {box_cols, box_rows, 2};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // A map over a row-major 16-bit matrix [rows, cols], cols a multiple of 64, seen as [cols / 64][rows][64]: a box is
 // `box_rows` rows of two consecutive 64-element pieces, laid down in shared memory as [2][box_rows][64] with the
 // 128-byte swizzle (the 16-byte chunk c of row r lies at chunk c ^ (r & 7)).  Coordinates: (0, row, piece).

@@ -96,7 +96,7 @@ _SIGNATURES = {
     "llm_linear8_few": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "llm_gemm8_tcgen05": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp],
+    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
 }
 
@@ -2469,7 +2469,7 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
         add_launches(1)
     code = _launch("llm_attention8", _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(pool), _ptr(exponents), _ptr(page_table), page_table.shape[1],
                    _ptr(ctx.cu_tokens), _ptr(ctx.context_lens), requests, n, longest, num_heads, num_kv_heads, head_dim, pool.shape[3],
-                   pool.shape[0], int(window or 0), float(scale), ranges, _ptr(scratch), _stream())
+                   pool.shape[0], int(window or 0), float(scale), ranges, _ptr(scratch), _error_flag_ptr(), _stream())
     _check(code, "paged_attention8")
     return out
 
