@@ -9,20 +9,11 @@
 // A block's four products start from zero and enter the 32-bit sums times both scales.  (The e4m3 product of mma.sync adds
 // its 32 terms without loss on this chip: 2,048 terms came out within 1.6e-7 of the 64-bit sum.)
 #include "common.cuh"
+#include "linear8.h"
 
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, BLOCK = 128;
-
-struct Few8Params {
-    const unsigned char* x;  // [M, K]
-    const float* sx;         // [M, kblocks]
-    const unsigned char* w;  // [N, K]
-    const float* sw;         // [ceil(N / 128), kblocks]
-    void* out;
-    int M, N, K, kblocks, ldo;
-    int early;  // the weights may be read before the kernel in front has ended
-};
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
@@ -44,7 +35,7 @@ struct Weights {
 
 template <int NT, int GROUP, typename TO>
 __global__ void __launch_bounds__(THREADS)
-linear8_few_kernel(const Few8Params p) {
+linear8_few_kernel(const linear8::Operands p, const int early) {
     extern __shared__ __align__(16) float red[];  // [2][WARPS][NT * 4][32]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int tiles = (p.N + 15) / 16;
@@ -66,10 +57,10 @@ linear8_few_kernel(const Few8Params p) {
 
     Weights<GROUP> now, next;
     int tile = blockIdx.x, group = 0, turn = 0;
-    if (p.early) fetch(now, tile, 0);
+    if (early) fetch(now, tile, 0);
     pdl_wait();
     pdl_trigger();
-    if (!p.early) fetch(now, tile, 0);
+    if (!early) fetch(now, tile, 0);
 
     float acc[NT][4];
 #pragma unroll
@@ -137,7 +128,7 @@ linear8_few_kernel(const Few8Params p) {
 }
 
 template <int NT, int GROUP, typename TO>
-int launch(const Few8Params& p, cudaStream_t stream) {
+int launch(const linear8::Operands& p, int early, cudaStream_t stream) {
     constexpr size_t smem = 2 * WARPS * NT * 128 * sizeof(float);
     auto kernel = linear8_few_kernel<NT, GROUP, TO>;
     if (smem > 48 * 1024) {
@@ -145,29 +136,19 @@ int launch(const Few8Params& p, cudaStream_t stream) {
         if (e != cudaSuccess) return (int)e;
     }
     const int tiles = (p.N + 15) / 16, most = device_sms() * 2;
-    return launch_pdl(kernel, dim3(tiles < most ? tiles : most), dim3(THREADS), smem, stream, p);
+    return launch_pdl(kernel, dim3(tiles < most ? tiles : most), dim3(THREADS), smem, stream, p, early);
 }
 
 template <typename TO>
-int by_rows(const Few8Params& p, cudaStream_t stream) {
-    if (p.M <= 8) return launch<1, 2, TO>(p, stream);
-    if (p.M <= 16) return launch<2, 2, TO>(p, stream);
-    if (p.M <= 32) return launch<4, 2, TO>(p, stream);
-    return launch<8, 1, TO>(p, stream);
+int by_rows(const linear8::Operands& p, int early, cudaStream_t stream) {
+    if (p.M <= 8) return launch<1, 2, TO>(p, early, stream);
+    if (p.M <= 16) return launch<2, 2, TO>(p, early, stream);
+    if (p.M <= 32) return launch<4, 2, TO>(p, early, stream);
+    return launch<8, 1, TO>(p, early, stream);
 }
 
 }  // namespace
 
-// x [M, K] and w [N, K] e4m3, contiguous, on 16 bytes, K a multiple of 16; sx [M, ceil(K / 128)], sw [ceil(N / 128), ceil(K / 128)] float32;
-// out [M, N] (row stride ldo), float32 or bfloat16.  M <= 64, otherwise LLM_ERR_UNSUPPORTED.  `early`: w and sw may be read while
-// the kernel in front still runs.
-LLM_EXPORT int llm_linear8_few(const void* x, const float* sx, const void* w, const float* sw, void* out, int out_dtype, int M, int N, int K,
-                               int ldo, int early, cudaStream_t stream) {
-    if (M <= 0 || N <= 0) return 0;
-    if (K < 16 || (K & 15) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15)) return LLM_ERR_BAD_ARGUMENT;
-    if (M > 64) return LLM_ERR_UNSUPPORTED;
-    Few8Params p = {(const unsigned char*)x, sx, (const unsigned char*)w, sw, out, M, N, K, (K + BLOCK - 1) / BLOCK, ldo, early};
-    if (out_dtype == LLM_F32) return by_rows<float>(p, stream);
-    if (out_dtype == LLM_BF16) return by_rows<__nv_bfloat16>(p, stream);
-    return LLM_ERR_BAD_ARGUMENT;
+int linear8::few(const Operands& p, bool early, cudaStream_t stream) {
+    return p.out_dtype == LLM_F32 ? by_rows<float>(p, early, stream) : by_rows<__nv_bfloat16>(p, early, stream);
 }

@@ -93,8 +93,7 @@ _SIGNATURES = {
     "llm_expert_act_scale": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "llm_branch_sum_norm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _f, _vp],
     "llm_quantize_blocks": [_vp, _i, _ll, _vp, _vp, _i, _i, _i, _vp],
-    "llm_linear8_few": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    "llm_gemm8_tcgen05": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
+    "llm_linear8": [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
@@ -2315,15 +2314,18 @@ def delta_rule(y: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor, a_log: 
 # linear8_few.cu, gemm8_tcgen05.cu), and pages of keys and values with one for every head's vector (rope_kv_write8.cu, attention8.cu).
 _E4M3 = torch.float8_e4m3fn
 _BLOCK8 = 128
-_FEW8_MAX_ROWS = 64  # up to this many rows a product with 8-bit weights streams the weights through mma.sync; more go to tcgen05
 ATTENTION8_HEAD_DIMS = (64, 128)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _here(*tensors) -> None:
     """Kernels run on the current device's current stream: their operands have to lie there."""
-    device = torch.cuda.current_device()
+    device = _current_device() if torch.cuda.is_initialized() else torch.cuda.current_device()
     for t in tensors:
-        _need(t.is_cuda and t.get_device() == device, f"a tensor lies on {t.device}, the current device is cuda:{device}")
+        if t.get_device() != device:  # -1: on the host
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
 
 
 class Quantized:
@@ -2332,13 +2334,19 @@ class Quantized:
     a checkpoint's; :func:`quantize_blocks` makes powers of two."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int = 1):
-        _need(rows in (1, _BLOCK8), f"Quantized: a scale is for 1 or {_BLOCK8} rows, not {rows}")
-        _need(values.dtype == _E4M3 and values.dim() == 2 and values.is_contiguous(), "Quantized: values are a contiguous float8_e4m3fn matrix")
-        blocks = (-(-values.shape[0] // rows), -(-values.shape[1] // _BLOCK8))
-        _need(scales.dtype == torch.float32 and tuple(scales.shape) == blocks and scales.is_contiguous(), f"Quantized: scales are contiguous float32 {list(blocks)}")
-        _need(scales.device == values.device, "Quantized: values and scales lie on one device")
-        self.values, self.scales, self.rows = values, scales, rows
-        self.shape, self.device = values.shape, values.device
+        shape = values.shape
+        # (one test of everything: a call's own time is of the order of the smallest kernels')
+        if not (rows in (1, _BLOCK8) and values.dtype == _E4M3 and len(shape) == 2 and values.is_contiguous() and scales.dtype == torch.float32
+                and scales.shape == (-(-shape[0] // rows), -(-shape[1] // _BLOCK8)) and scales.is_contiguous() and scales.get_device() == values.get_device()):
+            _need(rows in (1, _BLOCK8), f"Quantized: a scale is for 1 or {_BLOCK8} rows, not {rows}")
+            _need(values.dtype == _E4M3 and len(shape) == 2 and values.is_contiguous(), "Quantized: values are a contiguous float8_e4m3fn matrix")
+            _need(scales.device == values.device, "Quantized: values and scales lie on one device")
+            raise KernelError(f"Quantized: scales are contiguous float32 {[-(-shape[0] // rows), -(-shape[1] // _BLOCK8)]}")
+        self.values, self.scales, self.rows, self.shape = values, scales, rows, shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         m, k = self.shape
@@ -2353,16 +2361,23 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Quantized:
     """``x [M, K]`` (float32 or bfloat16, unit inner stride) in 8 bits: for every block of ``rows`` (1: activations, 128: weights) rows
     and 128 columns the scale is ``2^e`` with the smallest ``e >= -126`` such that the block's largest finite ``|x|`` is at most ``448 * 2^e`` (1
     for a block of zeros), and a value is ``x / 2^e`` rounded to the nearest e4m3 (ties to even).  NaN and infinities become NaN."""
-    _need(rows in (1, _BLOCK8), f"quantize_blocks: a scale is for 1 or {_BLOCK8} rows, not {rows}")
-    _need(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] <= 1), "quantize_blocks: x is a matrix with unit inner stride")
+    shape = x.shape
+    if not (rows in (1, _BLOCK8) and len(shape) == 2 and (shape[1] <= 1 or x.stride(1) == 1)):
+        _need(rows in (1, _BLOCK8), f"quantize_blocks: a scale is for 1 or {_BLOCK8} rows, not {rows}")
+        raise KernelError("quantize_blocks: x is a matrix with unit inner stride")
     code = _code(x.dtype)
     _here(x)
-    m, k = x.shape
-    values = torch.empty((m, k), dtype=_E4M3, device=x.device)
-    scales = torch.empty((-(-m // rows), -(-k // _BLOCK8)), dtype=torch.float32, device=x.device)
+    m, k = shape
+    values = x.new_empty(shape, dtype=_E4M3)
+    scales = x.new_empty((-(-m // rows), -(-k // _BLOCK8)), dtype=torch.float32)
     if m and k:
-        _check(_launch("llm_quantize_blocks", _ptr(x), code, x.stride(0), _ptr(values), _ptr(scales), m, k, rows, _stream()), "quantize_blocks")
+        _check8(_launch("llm_quantize_blocks", x.data_ptr(), code, x.stride(0), values.data_ptr(), scales.data_ptr(), m, k, rows, _stream()), "quantize_blocks")
     return Quantized(values, scales, rows)
+
+
+def _check8(code: int, what: str) -> None:
+    if code:
+        _check(code, what)
 
 
 def quantize_weight(w: torch.Tensor) -> Quantized:
@@ -2380,35 +2395,44 @@ def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tens
     if isinstance(x, NormedInput):
         x = x.materialize()
     given = isinstance(x, Quantized)
-    _need(not given or x.rows == 1, "linear8: a quantised x has a scale for every row")
-    _need(len(x.shape) == 2 and x.shape[1] == w.shape[1], f"linear8: shapes {tuple(x.shape)} and {tuple(w.shape)} do not match")
-    (m, k), n = x.shape, w.shape[0]
-    _need(k >= 16 and k % 16 == 0, f"linear8: rows of {k} values; a multiple of 16 is needed")
+    xt = x.values if given else x
+    n, k = w.shape
+    if not (len(x.shape) == 2 and x.shape[1] == k and k % 16 == 0 and k >= 16 and xt.stride(1) == 1 and (not given or x.rows == 1)):
+        _need(not given or x.rows == 1, "linear8: a quantised x has a scale for every row")
+        _need(len(x.shape) == 2 and x.shape[1] == k, f"linear8: shapes {tuple(x.shape)} and {tuple(w.shape)} do not match")
+        _need(k >= 16 and k % 16 == 0, f"linear8: rows of {k} values; a multiple of 16 is needed")
+        raise KernelError("linear8: x has unit inner stride")
+    m = x.shape[0]
+    x_code = 0 if given else _code(x.dtype)
     out_dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
     code = _code(out_dtype)
-    _here(w.values)
-    xq = x if given else quantize_blocks(x)
-    _here(xq.values)
-    _need(xq.values.data_ptr() % 16 == 0 and w.values.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
-    out = torch.empty((m, n), dtype=out_dtype, device=w.device)
+    _here(xt, w.values)
+    out = xt.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return out
-    operands = (_ptr(xq.values), _ptr(xq.scales), _ptr(w.values), _ptr(w.scales), _ptr(out), code, m, n, k, n)
-    if m <= _FEW8_MAX_ROWS:
-        # the weights may be asked for early only if the kernel in front is the one that quantised x here: it began when all
-        # before it had ended, whoever wrote the weights among them
-        _check(_launch("llm_linear8_few", *operands, int(not given), _stream()), "linear8 (few rows)")
-    else:
-        _check(_launch("llm_gemm8_tcgen05", *operands, _error_flag_ptr(), _stream()), "linear8 (tcgen05)")
+    if given:
+        xq = None
+        _need(xt.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
+    else:  # values and scales of the quantised x
+        blocks = -(-k // _BLOCK8)
+        xq = xt.new_empty((m * k + 4 * m * blocks,), dtype=torch.uint8)
+    _need(w.values.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
+    _check8(_launch("llm_linear8", xt.data_ptr(), x_code, 0 if given else xt.stride(0), x.scales.data_ptr() if given else None, None if given else xq.data_ptr(),
+                    w.values.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, m, n, k, n, _error_flag_ptr(), _stream()), "linear8")
+    if not given:
+        add_launches(1)
     return out
 
 
 def _pages8(pool: torch.Tensor, exponents: torch.Tensor, kv_heads: int, dim: int, what: str) -> None:
-    _need(pool.dtype == _E4M3 and pool.dim() == 5 and pool.is_contiguous() and pool.shape[1] == 2 and pool.shape[2] == kv_heads and pool.shape[4] == dim,
+    shape = pool.shape
+    if (pool.dtype == _E4M3 and len(shape) == 5 and shape[1] == 2 and shape[2] == kv_heads and shape[4] == dim and pool.is_contiguous()
+            and exponents.dtype == torch.uint8 and exponents.shape == shape[:4] and exponents.is_contiguous() and dim in ATTENTION8_HEAD_DIMS):
+        return
+    _need(pool.dtype == _E4M3 and len(shape) == 5 and pool.is_contiguous() and shape[1] == 2 and shape[2] == kv_heads and shape[4] == dim,
           f"{what}: the pool plane is contiguous float8_e4m3fn [pages, 2, {kv_heads}, page_size, {dim}]")
-    _need(exponents.dtype == torch.uint8 and exponents.is_contiguous() and exponents.shape == pool.shape[:4],
-          f"{what}: exponents are contiguous uint8 {list(pool.shape[:4])}")
     _need(dim in ATTENTION8_HEAD_DIMS, f"{what}: 8-bit pages are built for heads of {ATTENTION8_HEAD_DIMS} lanes, not {dim}")
+    raise KernelError(f"{what}: exponents are contiguous uint8 {list(shape[:4])}")
 
 
 def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor | None, slot_map: torch.Tensor, pool: torch.Tensor,
@@ -2418,13 +2442,14 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
     ``pool`` (float8_e4m3fn ``[pages, 2, kv_heads, page_size, head_dim]``), each head's vector divided by a power of two (the rule of
     :func:`quantize_blocks` with ``head_dim`` lanes a block) whose biased exponent goes to ``exponents`` (uint8 ``[pages, 2, kv_heads,
     page_size]``): a number is ``e4m3 * 2^(exponent - 127)``.  Rows whose slot is no place of the pool are not stored."""
-    n, width = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
-    _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, f"rope_kv_write8: qkv rows hold {width} bfloat16 elements")
-    _need(qkv.stride(0) % 4 == 0 and qkv.data_ptr() % 8 == 0, "rope_kv_write8: qkv rows start on 8 bytes")
+    width = (num_heads + 2 * num_kv_heads) * head_dim
+    if not (qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width and qkv.stride(0) % 4 == 0 and qkv.data_ptr() % 8 == 0):
+        _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, f"rope_kv_write8: qkv rows hold {width} bfloat16 elements")
+        raise KernelError("rope_kv_write8: qkv rows start on 8 bytes")
     _pages8(pool, exponents, num_kv_heads, head_dim, "rope_kv_write8")
+    n, rows = qkv.shape[0], 0
     _i32(slot_map, "slot_map")
     _need(slot_map.numel() == n, "rope_kv_write8: a slot for every row")
-    rows = 0
     if table is not None:
         _i32(positions, "positions")
         _need(positions.numel() == n, "rope_kv_write8: a position for every row")
@@ -2434,9 +2459,9 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
     _here(qkv, slot_map, pool, exponents)
     if n == 0:
         return
-    code = _launch("llm_rope_kv_write8", _ptr(qkv), qkv.stride(0), _ptr(positions) if rows else None, _ptr(table), rows, _ptr(slot_map), _ptr(pool),
-                   _ptr(exponents), n, num_heads, num_kv_heads, head_dim, pool.shape[3], pool.shape[0], _stream())
-    _check(code, "rope_kv_write8")
+    _check8(_launch("llm_rope_kv_write8", qkv.data_ptr(), qkv.stride(0), positions.data_ptr() if rows else None, table.data_ptr() if rows else None, rows,
+                    slot_map.data_ptr(), pool.data_ptr(), exponents.data_ptr(), n, num_heads, num_kv_heads, head_dim, pool.shape[3], pool.shape[0], _stream()),
+            "rope_kv_write8")
 
 
 def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tensor, page_table: torch.Tensor, ctx, *, num_heads: int,
@@ -2444,33 +2469,36 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     """:func:`paged_attention` over 8-bit pages as :func:`rope_kv_write8` leaves them.  ``q`` rows (bfloat16) start with the rotated query
     heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  Where requests may be
     long their keys are spread evenly over the CTAs, wherever requests begin and end, and joined by a second kernel.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
-    n = q.shape[0]
-    _need(q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= num_heads * head_dim, "paged_attention8: rows of q start with the query heads, bfloat16")
-    _need(q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0, "paged_attention8: rows of q start on 8 bytes")
-    _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, f"paged_attention8: {num_heads} query heads over {num_kv_heads} key heads")
-    _need(window is None or window >= 1, "paged_attention8: a window holds a key at least")
+    width = num_heads * head_dim
+    if not (q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= width and q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0
+            and num_kv_heads > 0 and num_heads % num_kv_heads == 0 and (window is None or window >= 1)):
+        _need(q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= width, "paged_attention8: rows of q start with the query heads, bfloat16")
+        _need(q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0, "paged_attention8: rows of q start on 8 bytes")
+        _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, f"paged_attention8: {num_heads} query heads over {num_kv_heads} key heads")
+        raise KernelError("paged_attention8: a window holds a key at least")
     _pages8(pool, exponents, num_kv_heads, head_dim, "paged_attention8")
+    cu_tokens, context_lens = ctx.cu_tokens, ctx.context_lens
     _i32(page_table, "page_table")
-    _i32(ctx.cu_tokens, "cu_tokens")
-    _i32(ctx.context_lens, "context_lens")
-    requests = ctx.context_lens.numel()
-    _need(page_table.dim() == 2 and page_table.shape[0] == requests and ctx.cu_tokens.numel() == requests + 1, "paged_attention8: a row of the page table and a length for every request")
-    _here(q, pool, exponents, page_table, ctx.cu_tokens, ctx.context_lens)
-    out = torch.empty((n, num_heads * head_dim), dtype=torch.bfloat16, device=q.device)
+    _i32(cu_tokens, "cu_tokens")
+    _i32(context_lens, "context_lens")
+    n, requests = q.shape[0], context_lens.numel()
+    _need(page_table.dim() == 2 and page_table.shape[0] == requests and cu_tokens.numel() == requests + 1, "paged_attention8: a row of the page table and a length for every request")
+    _here(q, pool, exponents, page_table, cu_tokens, context_lens)
+    out = q.new_empty((n, width))
     if n == 0 or requests == 0:
         return out
     longest = getattr(ctx, "max_query_len", None) or max(_token_counts(ctx))
-    keys = getattr(ctx, "max_context_len", None) or int(ctx.context_lens.max())
+    keys = getattr(ctx, "max_context_len", None) or int(context_lens.max())
     group = num_heads // num_kv_heads
     ranges = _attention8_ranges(requests, num_kv_heads, longest * group, keys if window is None else min(keys, window + longest))
     scratch = None
     if ranges:
-        scratch = torch.empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32, device=q.device)
+        scratch = q.new_empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32)
         add_launches(1)
-    code = _launch("llm_attention8", _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(pool), _ptr(exponents), _ptr(page_table), page_table.shape[1],
-                   _ptr(ctx.cu_tokens), _ptr(ctx.context_lens), requests, n, longest, num_heads, num_kv_heads, head_dim, pool.shape[3],
-                   pool.shape[0], int(window or 0), float(scale), ranges, _ptr(scratch), _error_flag_ptr(), _stream())
-    _check(code, "paged_attention8")
+    _check8(_launch("llm_attention8", q.data_ptr(), q.stride(0), out.data_ptr(), width, pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), page_table.shape[1],
+                    cu_tokens.data_ptr(), context_lens.data_ptr(), requests, n, longest, num_heads, num_kv_heads, head_dim, pool.shape[3],
+                    pool.shape[0], int(window or 0), float(scale), ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
+            "paged_attention8")
     return out
 
 
