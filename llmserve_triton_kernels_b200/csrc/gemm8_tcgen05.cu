@@ -7,10 +7,15 @@
 // that way, and no sum is longer than 128 terms before it is rounded to 32 bits.  Roles, by warp:
 //   warp 0     : TMA producer, a ring of STAGES slots;
 //   warp 1     : issues the products into one of NBUF accumulators of tensor memory, in turn;
-//   warps 4-11 : the sums.  A warp owns its 32 rows (lanes) and half of the tile's columns, two columns to an instruction
-//                (fma.rn.f32x2); it asks for 32 columns of tensor memory while it adds the 32 before.  128 sums and two times
-//                32 columns need more registers than a third of the SM has: the first four warps give theirs up.
-// One CTA per SM walks 128 x BN tiles, column tiles outermost, so that CTAs that run at the same time share their weights.  What lies beyond
+//   warps 4-19 : the sums.  A warp owns its 32 rows (lanes) and a quarter of the tile's columns, two columns to an instruction
+//                (fma.rn.f32x2).  The sums and 32 columns on their way need more registers than 640 threads are launched with: the
+//                first four warps give theirs up.
+// The sums are what bounds it: one multiplication and addition for every 128 of a product take an SM's arithmetic 280 cycles for a
+// 128 x 256 tile's k-block, the reading of tensor memory 200 and the products 512, and they overlap in part (without the sums'
+// additions 4,096 x 28,672 x 4,096 took 395 us, with them 525).  What it measured: 533 us there, 1,806 TFLOP/s; the framework's bfloat16
+// product of the vendor's library reaches 1,670 at most on this chip.  Scales are read where rows lie side by side (linear8.h): from
+// [rows, blocks] the same product took 640 us.
+// One CTA per SM walks 128 x 128 tiles, or a pair of CTAs 256 x 256, column tiles outermost, so that CTAs that run at the same time share their weights.  What lies beyond
 // the matrices arrives as zeros and is masked at the store.  Every wait is bounded; one that gives up sets *error_flag and the
 // roles run to their ends.
 #include "common.cuh"
@@ -18,12 +23,16 @@
 #include "tma.cuh"
 #include "umma.cuh"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int BM = 128, BK = 128, UMMA_K = 32, EPI_WARPS = 8, FIRST_EPI = 4;
+constexpr int BM = 128, BK = 128, UMMA_K = 32, EPI_WARPS = 16, FIRST_EPI = 4;
 constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
-// 384 threads are launched with 168 registers each: 3 x 168 = 40 + 2 x 232
-constexpr int FEW_REGISTERS = 40, MANY_REGISTERS = 232;
+// 640 threads are launched with 96 registers each: 5 x 96 = 32 + 4 x 112
+constexpr int FEW_REGISTERS = 32, MANY_REGISTERS = 112;
 
 __device__ __forceinline__ unsigned long long pair_of(unsigned lo, unsigned hi) {
     unsigned long long r;
@@ -37,49 +46,61 @@ __device__ __forceinline__ void add_columns(unsigned long long* sums, const unsi
     for (int j = 0; j < 16; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sums[j]) : "l"(pair_of(v[2 * j], v[2 * j + 1])), "l"(scale));
 }
 
+// 32 rows (the warp's lanes) x 32 columns of sums, turned round in shared memory so that lanes side by side write 16 bytes each of one row:
+// a thread's own row would be a sector of each of 32 rows a store, which the way to memory takes several times as long for.
 template <typename TO>
-__device__ __forceinline__ void store_row(TO* dst, const float* v, int valid);
-template <>
-__device__ __forceinline__ void store_row<float>(float* dst, const float* v, int valid) {
-    if (valid >= 32 && ((uintptr_t)dst & 15) == 0) {
+constexpr int PIECE_PITCH = 32 * sizeof(TO) + 16;
+template <typename TO>
+constexpr int PIECE_BYTES = 32 * PIECE_PITCH<TO>;
+template <typename TO>
+__device__ __forceinline__ void store_piece(const linear8::Operands& p, unsigned char* piece, const unsigned long long* sums, int m0, int n0, int lane) {
+    constexpr int EACH = 16 / sizeof(TO), LANES = 32 / EACH;  // columns of 16 bytes; lanes of a row
+    unsigned char* mine = piece + lane * PIECE_PITCH<TO>;
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) dst[i] = v[i];
-    }
-}
-template <>
-__device__ __forceinline__ void store_row<__nv_bfloat16>(__nv_bfloat16* dst, const float* v, int valid) {
-    if (valid >= 32 && ((uintptr_t)dst & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+    for (int j = 0; j < 32; j += EACH) {
+        if constexpr (sizeof(TO) == 4) {
+            *reinterpret_cast<ulonglong2*>(mine + j * 4) = make_ulonglong2(sums[j / 2], sums[j / 2 + 1]);
+        } else {
             unsigned u[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __nv_bfloat162 a = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                u[j] = *reinterpret_cast<const unsigned*>(&a);
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(__uint_as_float((unsigned)sums[j / 2 + i]), __uint_as_float((unsigned)(sums[j / 2 + i] >> 32)));
+                u[i] = *reinterpret_cast<const unsigned*>(&a);
             }
-            *reinterpret_cast<uint4*>(dst + i) = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(mine + j * 2) = make_uint4(u[0], u[1], u[2], u[3]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) dst[i] = __float2bfloat16_rn(v[i]);
     }
+    __syncwarp();
+    const int c = (lane % LANES) * EACH, valid = p.N - n0 - c;
+    TO* out = reinterpret_cast<TO*>(p.out) + n0 + c;
+    const bool wide = valid >= EACH && ((uintptr_t)out & 15) == 0 && (p.ldo * sizeof(TO)) % 16 == 0;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 32 / LANES) {
+        const int row = r0 + lane / LANES, m = m0 + row;
+        if (m >= p.M) continue;
+        const unsigned char* from = piece + row * PIECE_PITCH<TO> + c * sizeof(TO);
+        if (wide) {
+            *reinterpret_cast<uint4*>(out + (size_t)m * p.ldo) = *reinterpret_cast<const uint4*>(from);
+        } else {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                if (i < valid) out[(size_t)m * p.ldo + i] = reinterpret_cast<const TO*>(from)[i];
+        }
+    }
+    __syncwarp();  // the piece is written again
 }
 
 template <int BN, int STAGES, typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
     constexpr int A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN * BK;
-    constexpr int NBUF = BN == 256 ? 2 : 4, TMEM_COLS = NBUF * BN;
-    static_assert(TMEM_COLS == 512 || TMEM_COLS == 256, "columns of tensor memory come in powers of two");
-    constexpr int COLS = BN / 2;  // of an epilogue warp
+    constexpr int NBUF = 4, TMEM_COLS = NBUF * BN;
+    static_assert(TMEM_COLS == 512, "all columns of tensor memory");
+    constexpr int COLS = BN / (EPI_WARPS / 4);  // of an epilogue warp
     constexpr unsigned IDESC = umma::idesc_e4m3(BM, BN);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
@@ -125,7 +146,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
     if (warp >= FIRST_EPI) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(MANY_REGISTERS));
         // ---- sums: warp w may touch the 32 lanes (warp % 4) * 32 .. of tensor memory ----
-        const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
+        const int quarter = warp & 3, part = (warp - FIRST_EPI) >> 2;
         int it = 0;
         bool ok = true;
         auto release = [&](int buf) {  // this warp has read its part: the accumulator may be filled again
@@ -134,9 +155,8 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
             if (lane == 0) tma::mbar_arrive(&acc_empty[buf]);
         };
         for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-            const int m0 = (tile % row_tiles) * BM, n0 = (tile / row_tiles) * BN + half * COLS;
-            const int row = m0 + quarter * 32 + lane;
-            const float* sx = p.sx + (size_t)min(row, p.M - 1) * kblocks;
+            const int m0 = (tile % row_tiles) * BM, n0 = (tile / row_tiles) * BN + part * COLS;
+            const float* sx = p.sx + (size_t)min(m0 + quarter * 32 + lane, p.M - 1) * p.sx_row;
             const float* sw = p.sw + (size_t)(min(n0, p.N - 1) >> 7) * kblocks;  // the warp's columns lie in one block of 128
             unsigned long long acc[COLS / 2];  // two 32-bit sums each
 #pragma unroll
@@ -144,52 +164,41 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
             // the scales of four k-blocks are asked for four k-blocks ahead
             float sx_now[4], sw_now[4], sx_next[4], sw_next[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sx_next[i] = sx[min(i, kblocks - 1)], sw_next[i] = sw[min(i, kblocks - 1)];
+            for (int i = 0; i < 4; ++i) sx_next[i] = sx[(size_t)min(i, kblocks - 1) * p.sx_block], sw_next[i] = sw[min(i, kblocks - 1)];
             for (int k0 = 0; k0 < kblocks && ok; k0 += 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sx_now[i] = sx_next[i], sw_now[i] = sw_next[i];
-                sx_next[i] = sx[min(k0 + 4 + i, kblocks - 1)], sw_next[i] = sw[min(k0 + 4 + i, kblocks - 1)];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (k0 + i >= kblocks) break;
-                const int buf = it % NBUF;
-                const float scale = sx_now[i] * sw_now[i];
-                ok = __all_sync(0xffffffffu, !failed() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
-                if (!ok) {
-                    if (lane == 0) fail();
-                    break;
+                for (int i = 0; i < 4; ++i) {
+                    sx_now[i] = sx_next[i], sw_now[i] = sw_next[i];
+                    sx_next[i] = sx[(size_t)min(k0 + 4 + i, kblocks - 1) * p.sx_block], sw_next[i] = sw[min(k0 + 4 + i, kblocks - 1)];
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const unsigned base = tmem_base + buf * BN + half * COLS + ((unsigned)(quarter * 32) << 16);
-                const unsigned long long both = pair_of(__float_as_uint(scale), __float_as_uint(scale));
-                unsigned v0[32], v1[32];
-                umma::tmem_ask32(base, v0);
 #pragma unroll
-                for (int c = 0; c < COLS; c += 64) {
-                    umma::tmem_have32(v0);
-                    if (c + 32 < COLS) umma::tmem_ask32(base + c + 32, v1); else release(buf);
-                    add_columns(acc + c / 2, v0, both);
-                    if (c + 32 >= COLS) break;
-                    umma::tmem_have32(v1);
-                    if (c + 64 < COLS) umma::tmem_ask32(base + c + 64, v0); else release(buf);
-                    add_columns(acc + c / 2 + 16, v1, both);
+                for (int i = 0; i < 4; ++i) {
+                    if (k0 + i >= kblocks) break;
+                    const int buf = it % NBUF;
+                    const float scale = sx_now[i] * sw_now[i];
+                    ok = __all_sync(0xffffffffu, !failed() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
+                    if (!ok) {
+                        if (lane == 0) fail();
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
+                    const unsigned long long both = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 32) {
+                        unsigned v[32];
+                        umma::tmem_ask32(base + c, v);
+                        umma::tmem_have32(v);
+                        if (c + 32 == COLS) release(buf);
+                        add_columns(acc + c / 2, v, both);
+                    }
+                    ++it;
                 }
-                ++it;
             }
-            }
-            if (ok && row < p.M) {
+            if (ok) {
 #pragma unroll
                 for (int c = 0; c < COLS; c += 32) {
-                    if (n0 + c >= p.N) continue;
-                    float v[32];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        v[2 * j] = __uint_as_float((unsigned)acc[c / 2 + j]);
-                        v[2 * j + 1] = __uint_as_float((unsigned)(acc[c / 2 + j] >> 32));
-                    }
-                    store_row<TO>(reinterpret_cast<TO*>(p.out) + (size_t)row * p.ldo + n0 + c, v, p.N - n0 - c);
+                    if (n0 + c < p.N) store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
                 }
             }
         }
@@ -259,9 +268,191 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
     }
 }
 
+// The same by a pair of CTAs (a cluster of two) on tiles of 256 x 256: each CTA loads and keeps its 128 rows of x, half the tile's rows of w and
+// its 128 rows of the result; the first CTA issues the products for both.  A single CTA's 128 x 256 tile needs 48 KB a k-block, which
+// the way from L2 to an SM does not bring in the products' time; a pair's needs 32 KB an SM.
+template <int STAGES, typename TO>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    constexpr int BN = 256, A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN / 2 * BK;  // of one CTA
+    constexpr int NBUF = 2, TMEM_COLS = NBUF * BN;
+    constexpr int COLS = BN / (EPI_WARPS / 4);  // of an epilogue warp
+    constexpr unsigned IDESC = umma::idesc_e4m3(2 * BM, BN);
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
+    __shared__ unsigned tmem_base;
+    __shared__ int gave_up;
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int kblocks = p.kblocks;
+    const int place = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int row_tiles = (p.M + 2 * BM - 1) / (2 * BM), col_tiles = (p.N + BN - 1) / BN, tiles = row_tiles * col_tiles;
+
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+            tma::mbar_init(&full[s], 1);
+            tma::mbar_init(&empty[s], 1);
+        }
+#pragma unroll
+        for (int b = 0; b < NBUF; ++b) {
+            tma::mbar_init(&acc_full[b], 1);
+            tma::mbar_init(&acc_empty[b], 2 * EPI_WARPS);  // the first CTA's is waited for, by both CTAs' warps
+        }
+        tma::mbar_init(&drained, 1);
+        gave_up = 0;
+        tma::mbar_fence_init();
+        tma::prefetch_map(&xmap);
+        tma::prefetch_map(&wmap);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tma::smem_addr(&tmem_base)), "n"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    cg::this_cluster().sync();  // both CTAs' barriers and tensor memory are there
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    pdl_wait();  // x comes from the kernel before
+    pdl_trigger();
+
+    auto fail = [&]() {
+        *(volatile int*)&gave_up = 1;
+        if (error_flag) atomicExch(error_flag, 1);
+    };
+    auto failed = [&]() { return *(volatile int*)&gave_up != 0; };
+
+    // (each role's share of the registers is set where the role begins: what follows a smaller share is compiled for it)
+    if (warp >= FIRST_EPI) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(MANY_REGISTERS));
+        // ---- sums: warp w may touch the 32 lanes (warp % 4) * 32 .. of tensor memory ----
+        const int quarter = warp & 3, part = (warp - FIRST_EPI) >> 2;
+        int it = 0;
+        bool ok = true;
+        auto release = [&](int buf) {  // this warp has read its part: the accumulator may be filled again
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive_at(&acc_empty[buf], 0);
+        };
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + part * COLS;
+            const float* sx = p.sx + (size_t)min(m0 + quarter * 32 + lane, p.M - 1) * p.sx_row;
+            const float* sw = p.sw + (size_t)(min(n0, p.N - 1) >> 7) * kblocks;  // the warp's columns lie in one block of 128
+            unsigned long long acc[COLS / 2];  // two 32-bit sums each
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
+            // the scales of four k-blocks are asked for four k-blocks ahead
+            float sx_now[4], sw_now[4], sx_next[4], sw_next[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sx_next[i] = sx[(size_t)min(i, kblocks - 1) * p.sx_block], sw_next[i] = sw[min(i, kblocks - 1)];
+            for (int k0 = 0; k0 < kblocks && ok; k0 += 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sx_now[i] = sx_next[i], sw_now[i] = sw_next[i];
+                    sx_next[i] = sx[(size_t)min(k0 + 4 + i, kblocks - 1) * p.sx_block], sw_next[i] = sw[min(k0 + 4 + i, kblocks - 1)];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (k0 + i >= kblocks) break;
+                    const int buf = it % NBUF;
+                    const float scale = sx_now[i] * sw_now[i];
+                    ok = __all_sync(0xffffffffu, !failed() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
+                    if (!ok) {
+                        if (lane == 0) fail();
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
+                    const unsigned long long both = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 32) {
+                        unsigned v[32];
+                        umma::tmem_ask32(base + c, v);
+                        umma::tmem_have32(v);
+                        if (c + 32 == COLS) release(buf);
+                        add_columns(acc + c / 2, v, both);
+                    }
+                    ++it;
+                }
+            }
+            if (ok) {
+#pragma unroll
+                for (int c = 0; c < COLS; c += 32) {
+                    if (n0 + c < p.N) store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(FEW_REGISTERS));
+        auto there = [&](unsigned long long* bar, unsigned parity) {  // for the whole warp
+            if (__all_sync(0xffffffffu, tma::mbar_wait(bar, parity))) return true;
+            fail();
+            return false;
+        };
+        if (warp == 0) {
+            // ---- producer ----
+            int it = 0, s = 0, turn = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += pairs) {
+                const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + place * (BN / 2);
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                    if (!ok) break;
+                    unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                    if (umma::elect_one()) {
+                        if (place == 0) tma::mbar_expect_tx(&full[s], 2 * SLOT_BYTES);  // both CTAs' bytes
+                        tma::load_2d_pair(slot, &xmap, kb * BK, m0, &full[s]);
+                        tma::load_2d_pair(slot + A_BYTES, &wmap, kb * BK, n0, &full[s]);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) s = 0, ++turn;
+                }
+            }
+            // nobody waits for the copies on their way any more (they are counted at the first CTA, which outlives them: the CTAs leave together)
+            if (!ok && place == 0)
+                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        } else if (warp == 1 && place == 0) {
+            // ---- tensor-core issuer, for both CTAs ----
+            int it = 0, s = 0, turn = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += pairs) {
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    const int buf = it % NBUF;
+                    ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                    const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
+                    const unsigned d = tmem_base + buf * BN;
+                    if (umma::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
+                            umma::mma_e4m3_pair(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
+                        umma::commit_pair(&empty[s]);
+                        umma::commit_pair(&acc_full[buf]);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) s = 0, ++turn;
+                }
+            }
+            if (!ok) {  // nor for the products
+                if (umma::elect_one()) umma::commit_pair(&drained);
+                (void)tma::mbar_wait(&drained, 0);
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
+    }
+}
+
 template <int BN, int STAGES, typename TO>
 int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024;
+    constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
     auto kernel = gemm8_tcgen05_kernel<BN, STAGES, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
@@ -276,18 +467,44 @@ int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
 }
 
 template <typename TO>
+int launch_pair(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
+    constexpr int STAGES = 4;
+    constexpr size_t smem = (size_t)STAGES * 2 * BM * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
+    auto kernel = gemm8_pair_kernel<STAGES, TO>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap xmap, wmap;
+    if (!tma::make_map_2d_u8(&xmap, p.x, p.M, p.K, p.K, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !tma::make_map_2d_u8(&wmap, p.w, p.N, p.K, p.K, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B))
+        return LLM_ERR_UNSUPPORTED;
+    const long long tiles = (long long)((p.N + 255) / 256) * ((p.M + 255) / 256);
+    if (tiles > 0x3fffffffLL) return LLM_ERR_UNSUPPORTED;
+    const int pairs = device_sms() / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles < pairs ? tiles : pairs) * 2);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, error_flag, xmap, wmap);
+}
+
+// A pair's tile of 256 x 256 takes 0.66 us a k-block, a CTA's of 128 x 128 0.45: pairs are faster (4,096 x 28,672 x 4,096: 533 us against
+// 714) but where their tiles leave most of them without work (512 x 4,096 x 4,096, 32 tiles for 74 pairs: 25.3 us against 20.2).
+template <typename TO>
 int by_shape(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
-    const int sms = device_sms(), row_tiles = (p.M + BM - 1) / BM;
-    int best = 64;
-    double least = 1e30;
-    for (int bn : {256, 128, 64}) {
-        const long long tiles = (long long)((p.N + bn - 1) / bn) * row_tiles;
-        const double cost = (double)((tiles + sms - 1) / sms) * (bn + 40);
-        if (cost < least) least = cost, best = bn;
-    }
-    if (best == 256) return launch<256, 4, TO>(p, error_flag, stream);
-    if (best == 128) return launch<128, 6, TO>(p, error_flag, stream);
-    return launch<64, 8, TO>(p, error_flag, stream);
+    const long long sms = device_sms(), pairs = sms / 2;
+    auto rounds = [&](long long side, long long at_once) { return (((p.M + side - 1) / side) * ((p.N + side - 1) / side) + at_once - 1) / at_once; };
+    if (rounds(256, pairs) * 66 <= rounds(128, sms) * 45) return launch_pair<TO>(p, error_flag, stream);
+    return launch<128, 4, TO>(p, error_flag, stream);
 }
 
 }  // namespace

@@ -1,11 +1,8 @@
-// A product with 8-bit weights as one call: the rows of x are quantised (unless they come so), then go to the kernel for few rows or to
-// the one for many.
+// A product with 8-bit weights as one call: the rows of x are quantised (unless they come so), then go to the kernel for so
+// many of them.
 #include "linear8.h"
 
 #include "common.cuh"
-
-LLM_EXPORT int llm_quantize_blocks(const void* x, int dtype, long long ldx, unsigned char* values, float* scales, int M, int K, int rows,
-                                   cudaStream_t stream);
 
 // x [M, K]: float32 or bfloat16 (x_dtype; row stride ldx, unit inner stride), quantised into `scratch` (16-byte aligned, M K + 4 M ceil(K / 128)
 // bytes); or, with sx [M, ceil(K / 128)] float32 (not null), e4m3, contiguous, on 16 bytes.  w [N, K] e4m3, contiguous, on 16 bytes; sw
@@ -16,16 +13,20 @@ LLM_EXPORT int llm_linear8(const void* x, int x_dtype, long long ldx, const floa
     if (K < 16 || (K & 15) || ((uintptr_t)w & 15) || (out_dtype != LLM_F32 && out_dtype != LLM_BF16)) return LLM_ERR_BAD_ARGUMENT;
     const bool given = sx != nullptr;
     if (given ? ((uintptr_t)x & 15) != 0 : !scratch || ((uintptr_t)scratch & 15)) return LLM_ERR_BAD_ARGUMENT;
-    linear8::Operands p = {(const unsigned char*)x, sx, (const unsigned char*)w, sw, out, M, N, K, (K + 127) / 128, ldo, out_dtype};
+    linear8::Operands p = {(const unsigned char*)x, sx, given ? (K + 127) / 128 : 1, given ? 1 : M, (const unsigned char*)w, sw, out, M, N, K, (K + 127) / 128, ldo, out_dtype};
     if (!given) {
         unsigned char* values = (unsigned char*)scratch;
         float* scales = reinterpret_cast<float*>(values + (size_t)M * K);  // K is a multiple of 16
-        const int code = llm_quantize_blocks(x, x_dtype, ldx, values, scales, M, K, 1, stream);
+        const int code = linear8::quantize_rows(x, x_dtype, ldx, values, scales, M, K, stream);
         if (code) return code;
         p.x = values;
         p.sx = scales;
     }
     // The weights may be asked for early only if the kernel in front is the one that quantised x here: it began when all before it
     // had ended, whoever wrote the weights among them.
-    return M <= linear8::FEW_ROWS ? linear8::few(p, !given, stream) : linear8::many(p, error_flag, stream);
+    if (M <= linear8::FEW_ROWS) return linear8::few(p, !given, stream);
+    // The weights as the tall operand where x fills no tile of 128 rows by half, and where there are so few tiles that several CTAs may
+    // share one's k-blocks (which that kernel does).
+    const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
+    return M <= 64 || tiles * 2 <= device_sms() ? linear8::some(p, error_flag, stream) : linear8::many(p, error_flag, stream);
 }

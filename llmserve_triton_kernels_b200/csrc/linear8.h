@@ -5,19 +5,23 @@
 
 namespace linear8 {
 
-constexpr int FEW_ROWS = 64;  // up to this many rows of x the weights are streamed through mma.sync; more go to tcgen05
+constexpr int FEW_ROWS = 8;  // up to this many rows of x the weights are streamed through mma.sync
 
 struct Operands {
     const unsigned char* x;  // [M, K] e4m3
-    const float* sx;         // [M, kblocks]
+    const float* sx;         // row m's scale of block b at m * sx_row + b * sx_block: warps read those of many rows at once, which lie side by
+    int sx_row, sx_block;    // side where they were made for this, [kblocks, M]; a caller's are [M, kblocks]
     const unsigned char* w;  // [N, K] e4m3
     const float* sw;         // [ceil(N / 128), kblocks]
     void* out;               // [M, N], row stride ldo
     int M, N, K, kblocks, ldo, out_dtype;
 };
 
+// The rows of x [M, K] (float32 or bfloat16, row stride ldx) in 8 bits; scales [kblocks, M].
+int quantize_rows(const void* x, int dtype, long long ldx, unsigned char* values, float* scales, int M, int K, cudaStream_t stream);
 // `early`: w and sw may be read while the kernel in front still runs.
 int few(const Operands& p, bool early, cudaStream_t stream);
+int some(const Operands& p, int* error_flag, cudaStream_t stream);
 int many(const Operands& p, int* error_flag, cudaStream_t stream);
 
 }  // namespace linear8

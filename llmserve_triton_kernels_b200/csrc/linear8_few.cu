@@ -90,8 +90,8 @@ linear8_few_kernel(const linear8::Operands p, const int early) {
                 mma_e4m3(c, a0.z, a1.z, a0.w, a1.w, b0.z, b0.w);
                 mma_e4m3(c, a2.x, a3.x, a2.y, a3.y, b1.x, b1.y);
                 mma_e4m3(c, a2.z, a3.z, a2.w, a3.w, b1.z, b1.w);
-                const float s0 = sw * p.sx[(size_t)min(8 * i + 2 * t, p.M - 1) * p.kblocks + kb];
-                const float s1 = sw * p.sx[(size_t)min(8 * i + 2 * t + 1, p.M - 1) * p.kblocks + kb];
+                const float s0 = sw * p.sx[(size_t)min(8 * i + 2 * t, p.M - 1) * p.sx_row + (size_t)kb * p.sx_block];
+                const float s1 = sw * p.sx[(size_t)min(8 * i + 2 * t + 1, p.M - 1) * p.sx_row + (size_t)kb * p.sx_block];
                 acc[i][0] = fmaf(c[0], s0, acc[i][0]);
                 acc[i][1] = fmaf(c[1], s1, acc[i][1]);
                 acc[i][2] = fmaf(c[2], s0, acc[i][2]);

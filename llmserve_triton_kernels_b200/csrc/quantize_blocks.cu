@@ -2,6 +2,7 @@
 // (weights); see fp8.cuh for the scale.  One pass: a block's values stay in registers between its maximum and its rounding, so
 // every input byte is read once and every output byte written once.
 #include "fp8.cuh"
+#include "linear8.h"
 
 namespace {
 
@@ -35,10 +36,10 @@ __device__ __forceinline__ void store8(unsigned char* p, const float (&v)[8], fl
 }
 
 // Rows on their own, K a multiple of 8 and rows on 16 bytes: half a warp a block, eight values a lane.  UNROLL blocks a
-// half warp are on their way at once.
+// half warp are on their way at once.  `across`: the scales are laid down block by block, [blocks][M], as products read them.
 template <typename T, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
-quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ values, float* __restrict__ scales, int M, int K) {
+quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ values, float* __restrict__ scales, int M, int K, int across) {
     pdl_wait();
     pdl_trigger();  // after the wait: whoever starts behind this kernel starts when everything in front of it has ended
     const int kblocks = (K + BLOCK - 1) / BLOCK, lane = threadIdx.x & 15;
@@ -63,7 +64,7 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __re
             const long long b = b0 + u * step;
             if (b >= blocks) continue;
             if (col[u] < K) store8(values + row[u] * K + col[u], v[u], fp8::inverse(e));
-            if (lane == 0) scales[b] = fp8::power(e);
+            if (lane == 0) scales[across ? (b - row[u] * kblocks) * M + row[u] : b] = fp8::power(e);
         }
     }
 }
@@ -71,7 +72,7 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __re
 // ... any K, any layout: a warp a block.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-quantize_rows_any_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ values, float* __restrict__ scales, int M, int K) {
+quantize_rows_any_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ values, float* __restrict__ scales, int M, int K, int across) {
     pdl_wait();
     pdl_trigger();
     const int kblocks = (K + BLOCK - 1) / BLOCK, lane = threadIdx.x & 31;
@@ -91,7 +92,7 @@ quantize_rows_any_kernel(const T* __restrict__ x, long long ldx, unsigned char* 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (k0 + 32 * i < K) values[row * K + k0 + 32 * i] = (unsigned char)fp8::pack2(v[i], 0.f, inv);
-        if (lane == 0) scales[b] = fp8::power(e);
+        if (lane == 0) scales[across ? (b - row * kblocks) * M + row : b] = fp8::power(e);
     }
 }
 
@@ -147,7 +148,7 @@ quantize_tiles_kernel(const T* __restrict__ x, long long ldx, unsigned char* __r
 }
 
 template <typename T>
-int launch(const void* x, long long ldx, unsigned char* values, float* scales, int M, int K, int rows, cudaStream_t stream) {
+int launch(const void* x, long long ldx, unsigned char* values, float* scales, int M, int K, int rows, int across, cudaStream_t stream) {
     const T* p = (const T*)x;
     const long long kblocks = (K + BLOCK - 1) / BLOCK;
     const bool vector = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (ldx * sizeof(T)) % 16 == 0 && ((uintptr_t)values & 7) == 0;
@@ -161,8 +162,8 @@ int launch(const void* x, long long ldx, unsigned char* values, float* scales, i
     const long long per = vector ? THREADS / 16 : THREADS / 32;
     const long long want = (blocks + per - 1) / per;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    if (!vector) return launch_pdl(quantize_rows_any_kernel<T>, dim3(grid), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K);
-    return launch_pdl(quantize_rows_kernel<T, 2>, dim3(grid), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K);
+    if (!vector) return launch_pdl(quantize_rows_any_kernel<T>, dim3(grid), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K, across);
+    return launch_pdl(quantize_rows_kernel<T, 2>, dim3(grid), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K, across);
 }
 
 }  // namespace
@@ -173,7 +174,13 @@ LLM_EXPORT int llm_quantize_blocks(const void* x, int dtype, long long ldx, unsi
                                    cudaStream_t stream) {
     if (M <= 0 || K <= 0) return 0;
     if (rows != 1 && rows != BLOCK) return LLM_ERR_BAD_ARGUMENT;
-    if (dtype == LLM_F32) return launch<float>(x, ldx, values, scales, M, K, rows, stream);
-    if (dtype == LLM_BF16) return launch<__nv_bfloat16>(x, ldx, values, scales, M, K, rows, stream);
+    if (dtype == LLM_F32) return launch<float>(x, ldx, values, scales, M, K, rows, 0, stream);
+    if (dtype == LLM_BF16) return launch<__nv_bfloat16>(x, ldx, values, scales, M, K, rows, 0, stream);
+    return LLM_ERR_BAD_ARGUMENT;
+}
+
+int linear8::quantize_rows(const void* x, int dtype, long long ldx, unsigned char* values, float* scales, int M, int K, cudaStream_t stream) {
+    if (dtype == LLM_F32) return launch<float>(x, ldx, values, scales, M, K, 1, 1, stream);
+    if (dtype == LLM_BF16) return launch<__nv_bfloat16>(x, ldx, values, scales, M, K, 1, 1, stream);
     return LLM_ERR_BAD_ARGUMENT;
 }

@@ -159,6 +159,18 @@ __device__ __forceinline__ void load_2d(void* smem, const CUtensorMap* map, int 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
                  ::"r"(smem_addr(smem)), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
 }
+// For a pair of CTAs whose products one of them issues: the box goes to this CTA's shared memory, its bytes are counted on the first
+// CTA's barrier (bit 24 of a shared-memory address is the CTA's place in the pair).
+__device__ __forceinline__ void load_2d_pair(void* smem, const CUtensorMap* map, int x, int y, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+                 ::"r"(smem_addr(smem)), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar) & 0xfeffffffu) : "memory");
+}
+// Arrives at the same barrier of the cluster's CTA `rank`.
+__device__ __forceinline__ void mbar_arrive_at(unsigned long long* bar, unsigned rank) {
+    asm volatile(
+        "{\n.reg .b32 there;\nmapa.shared::cluster.u32 there, %0, %1;\nmbarrier.arrive.shared::cluster.b64 _, [there];\n}\n"
+        ::"r"(smem_addr(bar)), "r"(rank) : "memory");
+}
 __device__ __forceinline__ void load_3d(void* smem, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
                  ::"r"(smem_addr(smem)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");

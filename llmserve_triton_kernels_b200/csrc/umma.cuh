@@ -45,6 +45,18 @@ __device__ __forceinline__ void mma_e4m3(unsigned d_tmem, unsigned long long a, 
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)accumulate) : "memory");
 }
+// ... of a pair of CTAs (a cluster of two): M = 256, each CTA holds 128 rows of A and of the result, and half the rows of B.  Issued
+// by the pair's first CTA, for shared-memory and tensor-memory addresses that are the same in both.
+__device__ __forceinline__ void mma_e4m3_pair(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)accumulate) : "memory");
+}
+// Arrives at this barrier of both CTAs once the pair's products issued so far have ended.
+__device__ __forceinline__ void commit_pair(unsigned long long* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+                 ::"r"(tma::smem_addr(bar)), "h"((unsigned short)3) : "memory");
+}
 // The same product with the A operand in tensor memory: row m of A in lane m, its k values along the columns from
 // a_tmem on, two 16-bit values to a 32-bit column (the lower k in the lower half).
 __device__ __forceinline__ void mma_bf16_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b, unsigned idesc, bool accumulate) {
