@@ -29,6 +29,31 @@ __device__ __forceinline__ unsigned scale_exponent(unsigned bits) {
 __device__ __forceinline__ float power(unsigned biased) { return __uint_as_float(biased << 23); }
 __device__ __forceinline__ float inverse(unsigned biased) { return __uint_as_float((254u - biased) << 23); }
 
+// Eight consecutive values, 16-byte aligned.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 t = *reinterpret_cast<const uint4*>(p);
+    const unsigned w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    unsigned u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        u[i] = *reinterpret_cast<const unsigned*>(&a);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
 // Two values times the scale's inverse, rounded to e4m3 (the first in the low byte).  v * 0 + v is v, and NaN for an infinity:
 // what was not finite is NaN in 8 bits too.
 __device__ __forceinline__ unsigned short pack2(float a, float b, float inv) {

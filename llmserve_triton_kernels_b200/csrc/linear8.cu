@@ -24,7 +24,7 @@ LLM_EXPORT int llm_linear8(const void* x, int x_dtype, long long ldx, const floa
     }
     // The weights may be asked for early only if the kernel in front is the one that quantised x here: it began when all before it
     // had ended, whoever wrote the weights among them.
-    if (M <= linear8::FEW_ROWS) return linear8::few(p, !given, stream);
+    if (M <= linear8::FEW_ROWS || (M <= 2 * linear8::FEW_ROWS && (long long)N * K <= linear8::FEW_BYTES)) return linear8::few(p, !given, stream);
     // The weights as the tall operand where x fills no tile of 128 rows by half, and where there are so few tiles that several CTAs may
     // share one's k-blocks (which that kernel does).
     const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);

@@ -5,7 +5,9 @@
 
 namespace linear8 {
 
-constexpr int FEW_ROWS = 8;  // up to this many rows of x the weights are streamed through mma.sync
+// Up to FEW_ROWS rows of x the weights are streamed through mma.sync, up to twice as many where the weights are FEW_BYTES at most.
+constexpr int FEW_ROWS = 8;
+constexpr long long FEW_BYTES = 20 << 20;
 
 struct Operands {
     const unsigned char* x;  // [M, K] e4m3

@@ -265,7 +265,7 @@ int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
     if (tiles > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
     const int sms = device_sms();
     int split = 1;  // doubled while all CTAs still run at once and none has fewer than four k-blocks
-    while (split < 8 && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
+    while (split < 4 && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms));
     cfg.blockDim = dim3(THREADS);

@@ -6,23 +6,9 @@
 
 namespace {
 
-constexpr int THREADS = 256, BLOCK = 128;
+constexpr int THREADS = 256, TILE_THREADS = 512, BLOCK = 128;
 
-// Eight consecutive values, 16-byte aligned.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 t = *reinterpret_cast<const uint4*>(p);
-    const unsigned w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
+using fp8::load8;
 
 __device__ __forceinline__ unsigned top_of(const float (&v)[8]) {
     unsigned top = 0;
@@ -96,21 +82,22 @@ quantize_rows_any_kernel(const T* __restrict__ x, long long ldx, unsigned char* 
     }
 }
 
-// Blocks of 128 x 128, one a CTA: 64 values a thread.  VECTOR: K a multiple of 8 and rows on 16 bytes.
+// Blocks of 128 x 128, one a CTA: 32 values a thread.  VECTOR: K a multiple of 8 and rows on 16 bytes.
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
 quantize_tiles_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ values, float* __restrict__ scales, int M, int K) {
-    __shared__ unsigned tops[THREADS / 32];
+    constexpr int PER = BLOCK / (TILE_THREADS / 16);  // rows a thread
+    __shared__ unsigned tops[TILE_THREADS / 32];
     pdl_wait();
     pdl_trigger();
     const int kblocks = (K + BLOCK - 1) / BLOCK;
     const int tile_row = blockIdx.x / kblocks, tile_col = blockIdx.x - tile_row * kblocks;
     const int r0 = tile_row * BLOCK + (threadIdx.x >> 4), c0 = tile_col * BLOCK + (threadIdx.x & 15) * 8;
-    float v[8][8];
+    float v[PER][8];
     unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = r0 + 16 * i;
+    for (int i = 0; i < PER; ++i) {
+        const int r = r0 + (TILE_THREADS / 16) * i;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
         if (r < M && c0 < K) {
@@ -124,17 +111,17 @@ quantize_tiles_kernel(const T* __restrict__ x, long long ldx, unsigned char* __r
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, top_of(v[i]));
+    for (int i = 0; i < PER; ++i) top = max(top, top_of(v[i]));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) top = max(top, tops[w]);
+    for (int w = 0; w < TILE_THREADS / 32; ++w) top = max(top, tops[w]);
     const unsigned e = fp8::scale_exponent(top);
     const float inv = fp8::inverse(e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = r0 + 16 * i;
+    for (int i = 0; i < PER; ++i) {
+        const int r = r0 + (TILE_THREADS / 16) * i;
         if (r >= M || c0 >= K) continue;
         if (VECTOR) {
             store8(values + (long long)r * K + c0, v[i], inv);
@@ -155,8 +142,8 @@ int launch(const void* x, long long ldx, unsigned char* values, float* scales, i
     if (rows == BLOCK) {
         const long long tiles = (long long)((M + BLOCK - 1) / BLOCK) * kblocks;
         if (tiles > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
-        return vector ? launch_pdl(quantize_tiles_kernel<T, true>, dim3((unsigned)tiles), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K)
-                      : launch_pdl(quantize_tiles_kernel<T, false>, dim3((unsigned)tiles), dim3(THREADS), 0, stream, p, ldx, values, scales, M, K);
+        return vector ? launch_pdl(quantize_tiles_kernel<T, true>, dim3((unsigned)tiles), dim3(TILE_THREADS), 0, stream, p, ldx, values, scales, M, K)
+                      : launch_pdl(quantize_tiles_kernel<T, false>, dim3((unsigned)tiles), dim3(TILE_THREADS), 0, stream, p, ldx, values, scales, M, K);
     }
     const long long blocks = (long long)M * kblocks, most = (long long)device_sms() * 8;
     const long long per = vector ? THREADS / 16 : THREADS / 32;

@@ -2443,9 +2443,9 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
     :func:`quantize_blocks` with ``head_dim`` lanes a block) whose biased exponent goes to ``exponents`` (uint8 ``[pages, 2, kv_heads,
     page_size]``): a number is ``e4m3 * 2^(exponent - 127)``.  Rows whose slot is no place of the pool are not stored."""
     width = (num_heads + 2 * num_kv_heads) * head_dim
-    if not (qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width and qkv.stride(0) % 4 == 0 and qkv.data_ptr() % 8 == 0):
+    if not (qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0):
         _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, f"rope_kv_write8: qkv rows hold {width} bfloat16 elements")
-        raise KernelError("rope_kv_write8: qkv rows start on 8 bytes")
+        raise KernelError("rope_kv_write8: qkv rows start on 16 bytes")
     _pages8(pool, exponents, num_kv_heads, head_dim, "rope_kv_write8")
     n, rows = qkv.shape[0], 0
     _i32(slot_map, "slot_map")

@@ -79,7 +79,7 @@ def test_attention_refuses():
     good = dict(qkv=qkv, positions=pos, table=torch.zeros(9, 64), slot_map=slots, pool=pool, exponents=exps, num_heads=4, num_kv_heads=2, head_dim=64)
     for change, why in (
         (dict(qkv=qkv.float()), "bfloat16"), (dict(num_heads=5), "512|576"), (dict(exponents=exps[:, :1].contiguous()), "exponents"),
-        (dict(qkv=torch.zeros(2, 515, dtype=BF16)), "8 bytes"), (dict(pool=pool.transpose(2, 3)), "pool plane"),
+        (dict(qkv=torch.zeros(2, 515, dtype=BF16)), "16 bytes"), (dict(pool=pool.transpose(2, 3)), "pool plane"),
     ):
         with pytest.raises(ops.KernelError, match=why):
             ops.rope_kv_write8(**{**good, **change})

@@ -216,7 +216,7 @@ def rotary(d, places):
 def test_write_is_its_definition(H, KV, D, page_size):
     ctx, table, slots, pages = a_step([1, 19, 3], [40, 19, 7], page_size, H * 10 + D)
     n, width = ctx.num_tokens, (H + 2 * KV) * D
-    wide = torch.randn(n, width + 12, generator=gen(7), device=DEV).to(BF16)
+    wide = torch.randn(n, width + 16, generator=gen(7), device=DEV).to(BF16)
     wide[3, H * D + 5], wide[4, (H + KV) * D + 1] = torch.nan, torch.inf  # a key and a value that are not finite
     wide[5, H * D :] = 0.0
     wide[6, H * D :] *= 1e30
