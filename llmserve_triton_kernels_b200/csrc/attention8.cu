@@ -48,6 +48,7 @@ struct Attn8Params {
     const int* cu_tokens;
     const int* context_lens;
     int requests, H, KV, G, page_size, pages, window;
+    int below;          // requests that bring so many tokens or more are left out (0: none)
     int* error_flag;
     int ranges;         // stretches of the step's list of tiles at most; 0: a CTA takes a tile of rows with all its keys
     float scale;        // times log2 e
@@ -127,7 +128,9 @@ struct Share {
 };
 template <int ROWS>
 __device__ __forceinline__ Share share_of(const Attn8Params& p, int r) {
-    const int n = p.cu_tokens[r + 1] - p.cu_tokens[r], ctx = p.context_lens[r];
+    int n = p.cu_tokens[r + 1] - p.cu_tokens[r];
+    if (p.below && n >= p.below) n = 0;
+    const int ctx = p.context_lens[r];
     const int end = min(ctx, p.table_width * p.page_size), begin = p.window > 0 ? max(0, ctx - n - p.window + 1) : 0;
     Share s;
     s.row_tiles = (n * p.G + ROWS - 1) / ROWS;
@@ -230,7 +233,7 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
         at = end;
     }
     const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = n * p.G;
-    if (row0 >= rows) return;
+    if (row0 >= rows || (p.below && n >= p.below)) return;
     const int start = p.context_lens[r] - n;  // position of the request's first new token
     const int pos_min = start + row0 / p.G, pos_max = start + min(row0 + ROWS - 1, rows - 1) / p.G;
     // the request's tiles may reach further back or on than these rows see
@@ -615,7 +618,7 @@ attention8_join_kernel(const Attn8Params p) {
     const int r = blockIdx.x / p.KV, h = blockIdx.x - r * p.KV, row0 = blockIdx.y * ROWS;
     // The step's arrays are older than the kernel in front, which began behind everything before it: where the parts are is worked
     // out while that one runs.
-    const int first = p.cu_tokens[r], rows = (p.cu_tokens[r + 1] - first) * p.G, live_rows = min(ROWS, rows - row0);
+    const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = p.below && n >= p.below ? 0 : n * p.G, live_rows = min(ROWS, rows - row0);
     const Share share = share_of<ROWS>(p, r);
     lay_out<ROWS>(p, begins);
     const long long total = begins[p.requests], from = begins[r] + (long long)(h * share.row_tiles + blockIdx.y) * share.tiles;
@@ -711,12 +714,12 @@ LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longe
 
 // q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, on 16
 // bytes; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
-// most tokens a request brings.  out [n, H D].  window 0: none.  ranges: CTAs that share the step's keys evenly, with scratch memory of
+// most tokens a request brings; with `below` requests that bring so many or more are left out, and their rows of out as they are.  out [n, H D].  window 0: none.  ranges: CTAs that share the step's keys evenly, with scratch memory of
 // ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and tile of rows.  D 64 or 128.
 LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long long out_stride, const void* pool, const void* exponents,
                               const int* page_table, int table_width, const int* cu_tokens, const int* context_lens, int requests, int n,
-                              int longest, int H, int KV, int D, int page_size, int pages, int window, float scale, int ranges, float* scratch,
-                              int* error_flag, cudaStream_t stream) {
+                              int longest, int below, int H, int KV, int D, int page_size, int pages, int window, float scale, int ranges,
+                              float* scratch, int* error_flag, cudaStream_t stream) {
     if (n <= 0 || requests <= 0) return 0;
     if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || ranges < 0 || window < 0 ||
         (ranges && (!scratch || requests > MAX_REQUESTS || ((uintptr_t)scratch & 15))) || (q_stride & 3) || ((uintptr_t)q & 7) ||
@@ -725,7 +728,7 @@ LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long
         return LLM_ERR_BAD_ARGUMENT;
     const int rows = llm_attention8_rows(longest, H / KV);
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
-                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, error_flag, ranges,
+                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, below, error_flag, ranges,
                      scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};
     // a tensor map's rows are counted in 32 bits
     const int run = (long long)pages * 2 * KV * page_size > 0x7fffffffLL ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 0;

@@ -1,0 +1,74 @@
+// Pages in 8 bits as bfloat16 pages, for requests that bring so many tokens that the products bound their attention: there the tcgen05
+// kernel over bfloat16 pages does it, and what every tile of rows would unpack anew is unpacked once.  A number e4m3 * 2^e is a bfloat16
+// number (but for the smallest of all), so nothing is rounded.
+//
+// Request r's pages lie one after another from page rank(r) * width on, rank counting the requests that bring at least `least` tokens.
+// Places behind a request's end become zeros.  One CTA a page: 16 values a thread at a time, a 16-byte read and two 16-byte writes.
+#include "fp8.cuh"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+template <int D>
+__global__ void __launch_bounds__(THREADS)
+expand_pages8_kernel(const unsigned char* __restrict__ pool, const unsigned char* __restrict__ exponents, const int* __restrict__ page_table, int width,
+                     const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int KV, int page_size, int pages, int window, int least,
+                     __nv_bfloat16* __restrict__ out, int* __restrict__ out_table) {
+    const int r = blockIdx.y, at = blockIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    const int n = cu_tokens[r + 1] - cu_tokens[r];
+    int before = 0;
+    for (int r0 = 0; r0 < r; r0 += THREADS) {
+        const int i = r0 + threadIdx.x;
+        before += __syncthreads_count(i < r && cu_tokens[min(i, r) + 1] - cu_tokens[min(i, r)] >= least);
+    }
+    const int ctx = context_lens[r], first = window > 0 ? max(0, ctx - n - window + 1) : 0;
+    const bool needed = n >= least && at * page_size < ctx && (at + 1) * page_size > first;
+    const int to = before * width + at;
+    if (threadIdx.x == 0) out_table[(long long)r * width + at] = needed ? to : 0;
+    if (!needed) return;
+    const long long from = min(max(page_table[(long long)r * width + at], 0), pages - 1);
+    const long long keys = 2LL * KV * page_size;
+    constexpr int PIECES = D / 16;
+    for (int i = threadIdx.x; i < keys * PIECES; i += THREADS) {
+        const int key = i / PIECES, c = (i - key * PIECES) * 16;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        float scale = 0.f;
+        if (at * page_size + key % page_size < ctx) {
+            w = *reinterpret_cast<const uint4*>(pool + (from * keys + key) * D + c);
+            scale = fp8::power(exponents[from * keys + key]);
+        }
+        const unsigned words[4] = {w.x, w.y, w.z, w.w};
+        float v[2][8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 f = fp8::unpack2((unsigned short)(words[k] >> (16 * e)));
+                v[k >> 1][(k & 1) * 4 + 2 * e] = f.x * scale;
+                v[k >> 1][(k & 1) * 4 + 2 * e + 1] = f.y * scale;
+            }
+        __nv_bfloat16* dst = out + (to * keys + key) * D + c;
+        fp8::store8(dst, v[0]);
+        fp8::store8(dst + 8, v[1]);
+    }
+}
+
+}  // namespace
+
+// pool and exponents as rope_kv_write8.cu leaves them (16-byte aligned).  out: bfloat16 [requests with at least `least` tokens x width pages, 2, KV,
+// page_size, D]; out_table [requests, width].  window 0: none; else pages that no token's window reaches are left as they are.  D 64 or 128.
+LLM_EXPORT int llm_expand_pages8(const void* pool, const void* exponents, const int* page_table, int width, const int* cu_tokens,
+                                 const int* context_lens, int requests, int KV, int D, int page_size, int pages, int window, int least, void* out,
+                                 int* out_table, cudaStream_t stream) {
+    if (requests <= 0 || width <= 0) return 0;
+    if (KV <= 0 || page_size <= 0 || pages <= 0 || least <= 0 || window < 0 || ((uintptr_t)pool & 15) || ((uintptr_t)out & 15) ||
+        2LL * KV * page_size * (D / 16) > 0x7fffffffLL)
+        return LLM_ERR_BAD_ARGUMENT;
+    if (requests > 65535 || (D != 64 && D != 128)) return LLM_ERR_UNSUPPORTED;
+    return launch_pdl(D == 64 ? expand_pages8_kernel<64> : expand_pages8_kernel<128>, dim3(width, requests), dim3(THREADS), 0, stream,
+                      (const unsigned char*)pool, (const unsigned char*)exponents, page_table, width, cu_tokens, context_lens, KV, page_size, pages,
+                      window, least, (__nv_bfloat16*)out, out_table);
+}

@@ -9,6 +9,7 @@
 
 #include "common.cuh"
 
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 namespace fp8 {
@@ -28,6 +29,12 @@ __device__ __forceinline__ unsigned scale_exponent(unsigned bits) {
 }
 __device__ __forceinline__ float power(unsigned biased) { return __uint_as_float(biased << 23); }
 __device__ __forceinline__ float inverse(unsigned biased) { return __uint_as_float((254u - biased) << 23); }
+
+// The two numbers of a pair (the first in the low byte); by way of half precision, which holds every e4m3 number.
+__device__ __forceinline__ float2 unpack2(unsigned short v) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
 
 // Eight consecutive values, 16-byte aligned.
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {

@@ -297,6 +297,31 @@ def test_attention_is_its_definition(H, KV, D, page_size, case, window):
         assert not got[0].any()
 
 
+@pytest.mark.parametrize("window", [None, 70])
+@pytest.mark.parametrize("counts,held", [([130], [130]), ([300, 1, 40, 200, 5], [301, 700, 40, 260, 5]), ([1, 128], [0, 900]), ([129, 0, 31], [400, 9, 31])], ids=str)
+@pytest.mark.parametrize("H,KV,D,page_size", [(8, 2, 64, 16), (4, 1, 128, 8), (3, 3, 64, 64), (4, 2, 128, 24)])
+def test_attention_of_prompt_portions(H, KV, D, page_size, counts, held, window):
+    """Requests of many tokens, over unpacked pages, beside others that are not; weights are rounded to bfloat16 there, which has 7 bits behind
+    the leading one: half a step is 2^-8 of a weight."""
+    ctx, table, _, pages = a_step(counts, held, page_size, H + D + page_size)
+    pool, exps = pages8(pages, KV, page_size, D, 11)
+    needed = torch.zeros(pages, page_size, dtype=torch.bool, device=DEV)
+    for r, n in enumerate(held):
+        j = torch.arange(n, device=DEV)
+        needed[table[r].long()[j // page_size], j % page_size] = True
+    pool.view(torch.uint8).permute(0, 3, 1, 2, 4)[~needed] = 0x7F
+    exps.permute(0, 3, 1, 2)[~needed] = 255
+    q = torch.randn(ctx.num_tokens, H * D + 8, generator=gen(3), device=DEV).to(BF16)
+    got = ops().paged_attention8(q, pool, exps, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.05, window=window)
+    cu = ctx.host_cu_tokens
+    for r, n in enumerate(held):
+        rows = q[cu[r] : cu[r + 1], : H * D].view(-1, H, D)
+        k, v = request_rows(pool, exps, table[r], n)
+        want, size = (plain.attention(rows, k, x, n - rows.shape[0], 0.05, window) for x in (v, v.abs()))
+        off = (got[cu[r] : cu[r + 1]].view_as(want).to(F64) - want).abs()
+        assert (off <= (2.0**-8 + 2.0**-14) * size + 2.0**-8 * want.abs()).all(), r
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_reaches_the_rows_that_see(D):
     """NaN in a value or a key spoils the rows that see it and no other, also inside a tile of 16 keys that others see in part."""
