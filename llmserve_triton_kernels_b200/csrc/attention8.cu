@@ -25,6 +25,12 @@
 // side by side, and their values a fixed distance behind, so one box is a tile's keys and values (where pages hold tiles whole; two
 // boxes of eight keys where they hold eights): four boxes, or copies by the threads, cost a warp some 600 cycles a tile to ask for.
 //
+// Cutting and joining cost 8 us and more, so short or many units of work go without: a CTA takes a tile of rows with all its keys, of two
+// warps instead of eight where there are many units of few keys, whose time is a CTA's 4 us of loads that wait for one another (q and
+// the page table, the pages, the warps' meeting) and not the bytes.  The host picks, from the longest context it is told.
+// Heads of 128 lanes, 32 over 8, requests of random lengths: 32 of up to 16,000 keys 137 us, 5.0 TB/s of pages; 64 of up to 4,000 93 us, 3.7
+// TB/s; 8 of up to 4,000 23 us, of which 10 are laying out, cutting and joining.
+//
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
 // Where rows differ in what they see, NaN among the values is counted apart, so that it reaches the rows that see it alone.
 #include "fp8.cuh"
@@ -32,7 +38,7 @@
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32, TILE = 16, STAGES = 3;
+constexpr int TILE = 16, STAGES = 3;
 constexpr int JOIN_THREADS = 512;
 constexpr int MAX_REQUESTS = 1024;  // of a step whose work is counted tile by tile
 
@@ -50,6 +56,7 @@ struct Attn8Params {
     int requests, H, KV, G, page_size, pages, window;
     int below;          // requests that bring so many tokens or more are left out (0: none)
     int* error_flag;
+    int warps;          // of a CTA
     int ranges;         // stretches of the step's list of tiles at most; 0: a CTA takes a tile of rows with all its keys
     float scale;        // times log2 e
     float* part_sums;   // [ranges][2][ROWS][D + 4]: what a stretch holds of the rows at its beginning and at its end,
@@ -167,17 +174,19 @@ __device__ __forceinline__ void lay_out(const Attn8Params& p, long long* begins)
 
 // Stretches of a list of `total` tiles: no more than there are CTAs, none (but the last) shorter than a tile a warp.
 __device__ __forceinline__ int stretches(const Attn8Params& p, long long total) {
-    return (int)max(1LL, min((long long)p.ranges, total / WARPS));
+    return (int)max(1LL, min((long long)p.ranges, total / p.warps));
 }
 
 // RUN: pages hold whole runs of 8 or 16 keys; 0: they do not, and the threads copy every key from its own place.
-template <int D, int NT, int RUN>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
+template <int D, int NT, int RUN, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (NT == 1 ? 16 : 8) / WARPS)
 attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) {
+    constexpr int THREADS = WARPS * 32;
     constexpr int KSTEPS = D / 32, MTILES = D / 16, ROWS = 8 * NT, PITCH = D + 4;
     using S = Stage<D, RUN ? RUN : TILE>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
+    // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ float stats[WARPS][ROWS][3];  // largest score, largest score with the value's scale, sum of weights
     __shared__ long long begins[MAX_REQUESTS + 1];
     __shared__ __align__(16) unsigned char scales[WARPS][STAGES][2 * TILE];  // exponents of a stage's keys and values
@@ -204,405 +213,412 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
         end = total * (blockIdx.x + 1) / count;
     }
     while (at < end) {
-    // ---- the segment: request r, key head h, rows from row0 on, tiles tile_lo .. tile_hi - 1 ----
-    int r, h, row0, tile_lo, tile_hi, part = -1;  // part: the place in scratch memory of a segment without all keys
-    if (p.ranges) {
-        int lo = 0, hi = p.requests;  // the last request whose share begins at or before `at`
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (begins[mid] <= at) lo = mid; else hi = mid;
-        }
-        r = lo;
-        const Share s = share_of<ROWS>(p, r);
-        const long long within = at - begins[r];
-        const int unit = (int)(within / s.tiles), off = (int)(within - (long long)unit * s.tiles);
-        const int take = (int)min((long long)(s.tiles - off), end - at);
-        h = unit / s.row_tiles;
-        row0 = (unit - h * s.row_tiles) * ROWS;
-        tile_lo = s.first_tile + off;
-        tile_hi = tile_lo + take;
-        if (take < s.tiles) part = blockIdx.x * 2 + (off == 0);
-        at += take;
-    } else {
-        r = blockIdx.x / p.KV;
-        h = blockIdx.x - r * p.KV;
-        row0 = blockIdx.y * ROWS;
-        const Share s = share_of<ROWS>(p, r);
-        tile_lo = s.first_tile;
-        tile_hi = tile_lo + s.tiles;
-        at = end;
-    }
-    const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = n * p.G;
-    if (row0 >= rows || (p.below && n >= p.below)) return;
-    const int start = p.context_lens[r] - n;  // position of the request's first new token
-    const int pos_min = start + row0 / p.G, pos_max = start + min(row0 + ROWS - 1, rows - 1) / p.G;
-    // the request's tiles may reach further back or on than these rows see
-    const int key_end = min(pos_max + 1, p.table_width * p.page_size);
-    if (p.window > 0) tile_lo = max(tile_lo, max(0, pos_min - p.window + 1) / TILE);
-    tile_hi = min(tile_hi, (key_end + TILE - 1) / TILE);
-    const int mine = max(0, (tile_hi - tile_lo - warp + WARPS - 1) / WARPS);  // this warp's tiles: tile_lo + warp + i WARPS
-
-    // ---- the ring ----
-    const int* table = p.page_table + (long long)r * p.table_width;
-    // key `j` of the request as an index over [pages, 2, KV, page_size]
-    auto place = [&](int j) -> long long {
-        const int at = j / p.page_size;
-        const int page = min(max(table[at], 0), p.pages - 1);
-        return ((long long)page * 2 * p.KV + h) * p.page_size + (j - at * p.page_size);
-    };
-    const long long to_values = (long long)p.KV * p.page_size;
-    int run[2] = {0, 0};  // this lane's tile of the next 32: the places of its runs
-    // a place behind the request's end is some place of the pool: what lies there is masked
-    auto issue = [&](int i, int slot) {
-        const int j0 = (tile_lo + warp + i * WARPS) * TILE;
-        unsigned char* dst = ring + slot * S::BYTES;
-        const unsigned scale_dst = tma::smem_addr(scales[warp][slot]);
-        if constexpr (RUN != 0) {
-            if ((i & 31) == 0) {
-                const int j = j0 + lane * (WARPS * TILE);
-#pragma unroll
-                for (int x = 0; x < TILE / RUN; ++x) run[x] = j + 8 * x < key_end ? (int)place(j + 8 * x) : 0;
+        // ---- the segment: request r, key head h, rows from row0 on, tiles tile_lo .. tile_hi - 1 ----
+        int r, h, row0, tile_lo, tile_hi, part = -1;  // part: the place in scratch memory of a segment without all keys
+        if (p.ranges) {
+            int lo = 0, hi = p.requests;  // the last request whose share begins at or before `at`
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (begins[mid] <= at) lo = mid; else hi = mid;
             }
-            // lanes 0 to 3 ask for the exponents of the keys' and the values' eights, lane 0 for the boxes
-            const int at0 = __shfl_sync(0xffffffffu, run[0], i & 31), at1 = RUN == 8 ? __shfl_sync(0xffffffffu, run[1], i & 31) : at0 + 8;
-            if (lane < 4) copy_async<8>(scale_dst + 8 * lane, p.exponents + ((lane & 1) ? at1 : at0) + (lane >> 1) * to_values);
-            if (lane == 0) {
-                tma::mbar_expect_tx(&full[warp][slot], S::BYTES);
-                tma::load_3d(dst, &map, 0, at0, 0, &full[warp][slot]);
-                if (RUN == 8) tma::load_3d(dst + S::SECOND, &map, 0, at1, 0, &full[warp][slot]);
-            }
+            r = lo;
+            const Share s = share_of<ROWS>(p, r);
+            const long long within = at - begins[r];
+            const int unit = (int)(within / s.tiles), off = (int)(within - (long long)unit * s.tiles);
+            const int take = (int)min((long long)(s.tiles - off), end - at);
+            h = unit / s.row_tiles;
+            row0 = (unit - h * s.row_tiles) * ROWS;
+            tile_lo = s.first_tile + off;
+            tile_hi = tile_lo + take;
+            if (take < s.tiles) part = blockIdx.x * 2 + (off == 0);
+            at += take;
         } else {
-            // lane l finds key l's place
-            const bool is_there = j0 + (lane & 15) < key_end;
-            const long long own = is_there ? place(j0 + (lane & 15)) : 0;
-            const unsigned char exponent = is_there ? __ldg(p.exponents + own + (lane >> 4) * to_values) : 127;
-            asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(scale_dst + lane), "r"((unsigned)exponent) : "memory");
-            constexpr int CHUNKS = D / 16, AT_ONCE = 32 / CHUNKS;  // of a row; rows a copy
-#pragma unroll
-            for (int k = 0; k < TILE / AT_ONCE; ++k) {
-                const int row = k * AT_ONCE + lane / CHUNKS, c = lane % CHUNKS;
-                const long long key = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, row);
-                const unsigned to = tma::smem_addr(dst) + S::key(row, c);
-                copy_async<16>(to, p.pool + key * D + 16 * c);
-                copy_async<16>(to + S::VALUES, p.pool + (key + to_values) * D + 16 * c);
-            }
+            r = blockIdx.x / p.KV;
+            h = blockIdx.x - r * p.KV;
+            row0 = blockIdx.y * ROWS;
+            const Share s = share_of<ROWS>(p, r);
+            tile_lo = s.first_tile;
+            tile_hi = tile_lo + s.tiles;
+            at = end;
         }
-    };
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (i < mine) issue(i, (filled + i) % STAGES);
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
-    }
+        const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = n * p.G;
+        if (row0 >= rows || (p.below && n >= p.below)) return;
+        const int start = p.context_lens[r] - n;  // position of the request's first new token
+        const int pos_min = start + row0 / p.G, pos_max = start + min(row0 + ROWS - 1, rows - 1) / p.G;
+        // the request's tiles may reach further back or on than these rows see
+        const int key_end = min(pos_max + 1, p.table_width * p.page_size);
+        if (p.window > 0) tile_lo = max(tile_lo, max(0, pos_min - p.window + 1) / TILE);
+        tile_hi = min(tile_hi, (key_end + TILE - 1) / TILE);
+        const int mine = max(0, (tile_hi - tile_lo - warp + WARPS - 1) / WARPS);  // this warp's tiles: tile_lo + warp + i WARPS
 
-    // ---- q: product j of a key takes lanes (D / 4) t + 8 j + 0 .. 7 of a row, as the keys' bytes lie ----
-    unsigned qb[NT][KSTEPS][2][2];  // [upper, lower bits][first, second four lanes]
-    float factor[NT][2];  // of this thread's rows, which are 2 t and 2 t + 1 of every tile in the products' results
-    int pos[NT][2];
+        // q's loads go out before the ring's, whose places take a trip to the page table first
+        unsigned raw[NT][KSTEPS][4];
+        int own_pos[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int rho = row0 + 8 * nt + g;
-        const bool live = rho < rows;
-        const int token = live ? rho / p.G : 0, head = h * p.G + (live ? rho - token * p.G : 0);
-        const __nv_bfloat16* src = p.q + (first + token) * p.q_stride + (long long)head * D + (D / 4) * t;
-        unsigned raw[KSTEPS][4], top = 0;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int rho = row0 + 8 * nt + g;
+            const bool live = rho < rows;
+            const int token = live ? rho / p.G : 0, head = h * p.G + (live ? rho - token * p.G : 0);
+            const __nv_bfloat16* src = p.q + (first + token) * p.q_stride + (long long)head * D + (D / 4) * t;
+            own_pos[nt] = live ? start + token : -1;
 #pragma unroll
-        for (int j = 0; j < KSTEPS; ++j) {
-            const __nv_bfloat16* at = src + 8 * j;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint2 w = live ? *reinterpret_cast<const uint2*>(at + 4 * e) : make_uint2(0u, 0u);
-                raw[j][2 * e] = w.x;
-                raw[j][2 * e + 1] = w.y;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned a = raw[j][e] & 0x7fffu, b = (raw[j][e] >> 16) & 0x7fffu;
-                top = max(top, max(a < 0x7f80u ? a : 0u, b < 0x7f80u ? b : 0u));
-            }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest value to [2^7, 2^8): 2^shift, in two factors because either end may leave 32 bits' exponents
-        const int shift = top ? 134 - max((int)(top >> 7), 1) : 0;
-        const float f0 = __uint_as_float((unsigned)(127 + shift / 2) << 23), f1 = __uint_as_float((unsigned)(127 + shift - shift / 2) << 23);
-        const float own = p.scale / f0 / f1;
-        const int own_pos = live ? start + token : -1;
-#pragma unroll
-        for (int j = 0; j < KSTEPS; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    v[2 * i] = __uint_as_float(raw[j][2 * e + i] << 16) * f0 * f1;
-                    v[2 * i + 1] = __uint_as_float(raw[j][2 * e + i] & 0xffff0000u) * f0 * f1;
-                }
-                const unsigned upper = fp8::pack4(v[0], v[1], v[2], v[3], 1.f);
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const unsigned h2 = half2_of((unsigned short)(upper >> (16 * i)));
-                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-                    w[2 * i] = v[2 * i] - back.x;
-                    w[2 * i + 1] = v[2 * i + 1] - back.y;
-                }
-                qb[nt][j][0][e] = upper;
-                qb[nt][j][1][e] = fp8::pack4(w[0], w[1], w[2], w[3], 1.f);
-            }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            factor[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
-            pos[nt][e] = __shfl_sync(0xffffffffu, own_pos, (2 * t + e) * 4);
-        }
-    }
-
-    // o[nt][x]: lanes (D / 8) g + 2 x (+ 1) of the head, rows 2 t, 2 t + 1 of tile nt: [lane][row]
-    float o[NT][MTILES][4], m1[NT][2], m2[NT][2], sum[NT][2];  // sum: this thread's keys alone
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int x = 0; x < MTILES; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][x][e] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) m1[nt][e] = m2[nt][e] = NOTHING, sum[nt][e] = 0.f;
-    }
-
-    // tiles that begin in here are seen whole by every row
-    const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
-    for (int i0 = 0; i0 < mine; ++i0, ++filled) {
-        const int slot = filled % STAGES;
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
-        if (RUN && !broken && !tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1)) broken = true;
-        __syncwarp();  // copies by other lanes have arrived; and everyone has read the stage that is filled next
-        if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
-        const int j0 = (tile_lo + warp + i0 * WARPS) * TILE;
-        const unsigned char* stage = ring + slot * S::BYTES;
-
-        // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
-        // (four sums of products each, so that none waits for another for long)
-        float s[NT][4];
-        {
-            float c[NT][4][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c[nt][k][e] = 0.f;
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) {
-                const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
-                const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
-                const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_e4m3(c[nt][0], a0, qb[nt][2 * x][0][0], qb[nt][2 * x][0][1]);
-                    mma_e4m3(c[nt][1], a0, qb[nt][2 * x][1][0], qb[nt][2 * x][1][1]);
-                    mma_e4m3(c[nt][2], a1, qb[nt][2 * x + 1][0][0], qb[nt][2 * x + 1][0][1]);
-                    mma_e4m3(c[nt][3], a1, qb[nt][2 * x + 1][1][0], qb[nt][2 * x + 1][1][1]);
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = (c[nt][0][e] + c[nt][2][e]) + (c[nt][1][e] + c[nt][3][e]);
-        }
-        unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 2 * t + (e & 1) + 8 * (e >> 1);
-            if constexpr (D == 128) {
-                const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(row, g));
-                v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(stage + S::VALUES + S::key(row, g >> 1) + (g & 1) * 8);
-                v[e][0] = w.x, v[e][1] = w.y;
-            }
-        }
-        float ev[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const unsigned char* at = scales[warp][slot] + g + 8 * x;
-            const float ks = __uint_as_float((unsigned)at[0] << 23);
-            ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) s[nt][2 * x + e] *= ks * factor[nt][e];
-        }
-        if (j0 < whole_from || j0 > whole_to) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int j = j0 + g + 8 * x;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (j > pos[nt][e] || j >= key_end || (p.window > 0 && j <= pos[nt][e] - p.window)) s[nt][2 * x + e] = -INFINITY;
-            }
-            // a value that no row of the tile sees is nobody's
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
-                if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
-#pragma unroll
-                    for (int w = 0; w < D / 32; ++w) v[e][w] = 0u;
-                }
-            }
-            if (pos_min != pos_max) {
-                // Some row may see a key that another does not, and NaN times a weight of zero is NaN: NaN among the values is taken out and
-                // counted by a product of its own, of ones where a value is NaN and where a row sees a key.
-                unsigned any = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int w = 0; w < D / 32; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                if (__any_sync(0xffffffffu, any != 0)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        unsigned seen[2];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            seen[x] = transpose((s[nt][2 * x] == -INFINITY ? 0u : 0x3c00u) | (s[nt][2 * x + 1] == -INFINITY ? 0u : 0x3c000000u));
-#pragma unroll
-                        for (int x = 0; x < MTILES; ++x) {
-                            unsigned bad[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {  // lane byte 2 x + (q & 1), keys 2 t + 8 (q >> 1) and the next
-                                const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
-                                bad[q] = (((v[e][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c00u : 0u) |
-                                         (((v[e + 1][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c000000u : 0u);
-                            }
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(c, bad, seen[0], seen[1]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c[e] > 0.f) o[nt][x][e] = NAN;
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int w = 0; w < D / 32; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                }
-            }
-        }
-        // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
-        // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
-        unsigned pb[NT][2];
-        float u[NT][4];
-        bool behind = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                u[nt][e] = s[nt][e] + ev[e >> 1];
-                behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
-            }
-        if (__any_sync(0xffffffffu, behind)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int j = 0; j < KSTEPS; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
-                    const float keep = exp2_fast(m2[nt][e] - b);
-                    sum[nt][e] *= exp2_fast(m1[nt][e] - a);
-                    m1[nt][e] = a;
-                    m2[nt][e] = b;
-#pragma unroll
-                    for (int x = 0; x < MTILES; ++x) {
-                        o[nt][x][e] *= keep;
-                        o[nt][x][2 + e] *= keep;
-                    }
+                    const uint2 w = live ? *reinterpret_cast<const uint2*>(src + 8 * j + 4 * e) : make_uint2(0u, 0u);
+                    raw[nt][j][2 * e] = w.x;
+                    raw[nt][j][2 * e + 1] = w.y;
                 }
         }
+
+        // ---- the ring ----
+        const int* table = p.page_table + (long long)r * p.table_width;
+        // key `j` of the request as an index over [pages, 2, KV, page_size]
+        auto place = [&](int j) -> long long {
+            const int at = j / p.page_size;
+            const int page = min(max(table[at], 0), p.pages - 1);
+            return ((long long)page * 2 * p.KV + h) * p.page_size + (j - at * p.page_size);
+        };
+        const long long to_values = (long long)p.KV * p.page_size;
+        int run[2] = {0, 0};  // this lane's tile of the next 32: the places of its runs
+        // a place behind the request's end is some place of the pool: what lies there is masked
+        auto issue = [&](int i, int slot) {
+            const int j0 = (tile_lo + warp + i * WARPS) * TILE;
+            unsigned char* dst = ring + slot * S::BYTES;
+            const unsigned scale_dst = tma::smem_addr(scales[warp][slot]);
+            if constexpr (RUN != 0) {
+                if ((i & 31) == 0) {
+                    const int j = j0 + lane * (WARPS * TILE);
+#pragma unroll
+                    for (int x = 0; x < TILE / RUN; ++x) run[x] = j + 8 * x < key_end ? (int)place(j + 8 * x) : 0;
+                }
+                // lanes 0 to 3 ask for the exponents of the keys' and the values' eights, lane 0 for the boxes
+                const int at0 = __shfl_sync(0xffffffffu, run[0], i & 31), at1 = RUN == 8 ? __shfl_sync(0xffffffffu, run[1], i & 31) : at0 + 8;
+                if (lane < 4) copy_async<8>(scale_dst + 8 * lane, p.exponents + ((lane & 1) ? at1 : at0) + (lane >> 1) * to_values);
+                if (lane == 0) {
+                    tma::mbar_expect_tx(&full[warp][slot], S::BYTES);
+                    tma::load_3d(dst, &map, 0, at0, 0, &full[warp][slot]);
+                    if (RUN == 8) tma::load_3d(dst + S::SECOND, &map, 0, at1, 0, &full[warp][slot]);
+                }
+            } else {
+                // lane l finds key l's place
+                const bool is_there = j0 + (lane & 15) < key_end;
+                const long long own = is_there ? place(j0 + (lane & 15)) : 0;
+                const unsigned char exponent = is_there ? __ldg(p.exponents + own + (lane >> 4) * to_values) : 127;
+                asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(scale_dst + lane), "r"((unsigned)exponent) : "memory");
+                constexpr int CHUNKS = D / 16, AT_ONCE = 32 / CHUNKS;  // of a row; rows a copy
+#pragma unroll
+                for (int k = 0; k < TILE / AT_ONCE; ++k) {
+                    const int row = k * AT_ONCE + lane / CHUNKS, c = lane % CHUNKS;
+                    const long long key = (long long)__shfl_sync(0xffffffffu, (unsigned long long)own, row);
+                    const unsigned to = tma::smem_addr(dst) + S::key(row, c);
+                    copy_async<16>(to, p.pool + key * D + 16 * c);
+                    copy_async<16>(to + S::VALUES, p.pool + (key + to_values) * D + 16 * c);
+                }
+            }
+        };
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (i < mine) issue(i, (filled + i) % STAGES);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+
+        // ---- q: product j of a key takes lanes (D / 4) t + 8 j + 0 .. 7 of a row, as the keys' bytes lie ----
+        unsigned qb[NT][KSTEPS][2][2];  // [upper, lower bits][first, second four lanes]
+        float factor[NT][2];  // of this thread's rows, which are 2 t and 2 t + 1 of every tile in the products' results
+        int pos[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            unsigned top = 0;
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned a = raw[nt][j][e] & 0x7fffu, b = (raw[nt][j][e] >> 16) & 0x7fffu;
+                    top = max(top, max(a < 0x7f80u ? a : 0u, b < 0x7f80u ? b : 0u));
+                }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the row's largest value to [2^7, 2^8): 2^shift, in two factors because either end may leave 32 bits' exponents
+            const int shift = top ? 134 - max((int)(top >> 7), 1) : 0;
+            const float f0 = __uint_as_float((unsigned)(127 + shift / 2) << 23), f1 = __uint_as_float((unsigned)(127 + shift - shift / 2) << 23);
+            const float own = p.scale / f0 / f1;
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        v[2 * i] = __uint_as_float(raw[nt][j][2 * e + i] << 16) * f0 * f1;
+                        v[2 * i + 1] = __uint_as_float(raw[nt][j][2 * e + i] & 0xffff0000u) * f0 * f1;
+                    }
+                    const unsigned upper = fp8::pack4(v[0], v[1], v[2], v[3], 1.f);
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const unsigned h2 = half2_of((unsigned short)(upper >> (16 * i)));
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+                        w[2 * i] = v[2 * i] - back.x;
+                        w[2 * i + 1] = v[2 * i + 1] - back.y;
+                    }
+                    qb[nt][j][0][e] = upper;
+                    qb[nt][j][1][e] = fp8::pack4(w[0], w[1], w[2], w[3], 1.f);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                factor[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
+                pos[nt][e] = __shfl_sync(0xffffffffu, own_pos[nt], (2 * t + e) * 4);
+            }
+        }
+
+        // o[nt][x]: lanes (D / 8) g + 2 x (+ 1) of the head, rows 2 t, 2 t + 1 of tile nt: [lane][row]
+        float o[NT][MTILES][4], m1[NT][2], m2[NT][2], sum[NT][2];  // sum: this thread's keys alone
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sum[nt][e] += exp2_fast(s[nt][e] - m1[nt][e]) + exp2_fast(s[nt][2 + e] - m1[nt][e]);
-                u[nt][e] = exp2_fast(u[nt][e] - m2[nt][e]);
-                u[nt][2 + e] = exp2_fast(u[nt][2 + e] - m2[nt][e]);
-            }
-            pb[nt][0] = transpose(pack_half(u[nt][0], u[nt][1]));
-            pb[nt][1] = transpose(pack_half(u[nt][2], u[nt][3]));
+            for (int x = 0; x < MTILES; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][x][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) m1[nt][e] = m2[nt][e] = NOTHING, sum[nt][e] = 0.f;
         }
-        // ---- values: tile x takes bytes 2 x and 2 x + 1 of the thread's of every key ----
-#pragma unroll
-        for (int x = 0; x < MTILES; ++x) {
-            unsigned a[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
-                a[q] = half2_of((unsigned short)__byte_perm(v[e][b / 4], v[e + 1][b / 4], 0x0040u + 0x0011u * (b & 3)));
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][x], a, pb[nt][0], pb[nt][1]);
-        }
-    }
 
-    // ---- the warps meet, where the rings were ----
-    asm volatile("cp.async.wait_all;\n" ::: "memory");
-    if (broken) {  // a wait gave up: the result is void; what is still on its way must land before the memory serves another end
-        if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
-        for (int i = max(0, filled - STAGES); i < filled; ++i) (void)tma::mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
-    }
-    // the rings were written by the other proxy too, and will be: order what threads do to the same places
-    if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    __syncthreads();
-    float* merge = reinterpret_cast<float*>(smem);
+        // tiles that begin in here are seen whole by every row
+        const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
+        for (int i0 = 0; i0 < mine; ++i0, ++filled) {
+            const int slot = filled % STAGES;
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
+            if (RUN && !broken && !tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1)) broken = true;
+            __syncwarp();  // copies by other lanes have arrived; and everyone has read the stage that is filled next
+            if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            const int j0 = (tile_lo + warp + i0 * WARPS) * TILE;
+            const unsigned char* stage = ring + slot * S::BYTES;
+
+            // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
+            // (four sums of products each, so that none waits for another for long)
+            float s[NT][4];
+            {
+                float c[NT][4][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+                    for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], x);
-            const int row = 8 * nt + 2 * t + e;
-            if (row0 + row >= rows) continue;
-            if (g == 0) {
-                stats[warp][row][0] = m1[nt][e];
-                stats[warp][row][1] = m2[nt][e];
-                stats[warp][row][2] = sum[nt][e];
+                        for (int e = 0; e < 4; ++e) c[nt][k][e] = 0.f;
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) {
+                    const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
+                    const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
+                    const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_e4m3(c[nt][0], a0, qb[nt][2 * x][0][0], qb[nt][2 * x][0][1]);
+                        mma_e4m3(c[nt][1], a0, qb[nt][2 * x][1][0], qb[nt][2 * x][1][1]);
+                        mma_e4m3(c[nt][2], a1, qb[nt][2 * x + 1][0][0], qb[nt][2 * x + 1][0][1]);
+                        mma_e4m3(c[nt][3], a1, qb[nt][2 * x + 1][1][0], qb[nt][2 * x + 1][1][1]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] = (c[nt][0][e] + c[nt][2][e]) + (c[nt][1][e] + c[nt][3][e]);
             }
-            // lanes (D / 8) g + 2 x, + 1 at columns 16 x + 2 g, + 1: the warp's stores meet in no bank
-            float* at = merge + ((size_t)warp * ROWS + row) * PITCH + 2 * g;
+            unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-            for (int x = 0; x < MTILES; ++x) *reinterpret_cast<float2*>(at + 16 * x) = make_float2(o[nt][x][e], o[nt][x][2 + e]);
-        }
-    __syncthreads();
-    const int live_rows = min(ROWS, rows - row0);
-    for (int i = threadIdx.x; i < live_rows * (D / 2); i += THREADS) {
-        const int row = i / (D / 2), c = (i - row * (D / 2)) * 2;
-        float a = NOTHING, b = NOTHING;
+            for (int e = 0; e < 4; ++e) {
+                const int row = 2 * t + (e & 1) + 8 * (e >> 1);
+                if constexpr (D == 128) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(row, g));
+                    v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(stage + S::VALUES + S::key(row, g >> 1) + (g & 1) * 8);
+                    v[e][0] = w.x, v[e][1] = w.y;
+                }
+            }
+            float ev[2];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            a = fmaxf(a, stats[w][row][0]);
-            b = fmaxf(b, stats[w][row][1]);
-        }
-        float total = 0.f, y0 = 0.f, y1 = 0.f;
+            for (int x = 0; x < 2; ++x) {
+                const unsigned char* at = scales[warp][slot] + g + 8 * x;
+                const float ks = __uint_as_float((unsigned)at[0] << 23);
+                ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            total += stats[w][row][2] * exp2_fast(stats[w][row][0] - a);
-            const float f = exp2_fast(stats[w][row][1] - b);
-            const float2 x = *reinterpret_cast<const float2*>(merge + ((size_t)w * ROWS + row) * PITCH + c);
-            y0 = fmaf(x.x, f, y0);
-            y1 = fmaf(x.y, f, y1);
-        }
-        if (part < 0) {
-            finish<D>(p, first, h, row0 + row, c, a, b, total, y0, y1);
-        } else {
-            *reinterpret_cast<float2*>(p.part_sums + ((size_t)part * ROWS + row) * PITCH + c) = make_float2(y0, y1);
-            if (c == 0) {
-                float* st = p.part_stats + ((size_t)part * ROWS + row) * 3;
-                st[0] = a;
-                st[1] = b;
-                st[2] = total;
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) s[nt][2 * x + e] *= ks * factor[nt][e];
+            }
+            if (j0 < whole_from || j0 > whole_to) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int j = j0 + g + 8 * x;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (j > pos[nt][e] || j >= key_end || (p.window > 0 && j <= pos[nt][e] - p.window)) s[nt][2 * x + e] = -INFINITY;
+                }
+                // a value that no row of the tile sees is nobody's
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
+                    if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
+#pragma unroll
+                        for (int w = 0; w < D / 32; ++w) v[e][w] = 0u;
+                    }
+                }
+                if (pos_min != pos_max) {
+                    // Some row may see a key that another does not, and NaN times a weight of zero is NaN: NaN among the values is taken out and
+                    // counted by a product of its own, of ones where a value is NaN and where a row sees a key.
+                    unsigned any = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int w = 0; w < D / 32; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            unsigned seen[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                seen[x] = transpose((s[nt][2 * x] == -INFINITY ? 0u : 0x3c00u) | (s[nt][2 * x + 1] == -INFINITY ? 0u : 0x3c000000u));
+#pragma unroll
+                            for (int x = 0; x < MTILES; ++x) {
+                                unsigned bad[4];
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {  // lane byte 2 x + (q & 1), keys 2 t + 8 (q >> 1) and the next
+                                    const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
+                                    bad[q] = (((v[e][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c00u : 0u) |
+                                             (((v[e + 1][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c000000u : 0u);
+                                }
+                                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_f16(c, bad, seen[0], seen[1]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (c[e] > 0.f) o[nt][x][e] = NAN;
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int w = 0; w < D / 32; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    }
+                }
+            }
+            // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
+            // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
+            unsigned pb[NT][2];
+            float u[NT][4];
+            bool behind = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    u[nt][e] = s[nt][e] + ev[e >> 1];
+                    behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
+                }
+            if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
+                        const float keep = exp2_fast(m2[nt][e] - b);
+                        sum[nt][e] *= exp2_fast(m1[nt][e] - a);
+                        m1[nt][e] = a;
+                        m2[nt][e] = b;
+#pragma unroll
+                        for (int x = 0; x < MTILES; ++x) {
+                            o[nt][x][e] *= keep;
+                            o[nt][x][2 + e] *= keep;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sum[nt][e] += exp2_fast(s[nt][e] - m1[nt][e]) + exp2_fast(s[nt][2 + e] - m1[nt][e]);
+                    u[nt][e] = exp2_fast(u[nt][e] - m2[nt][e]);
+                    u[nt][2 + e] = exp2_fast(u[nt][2 + e] - m2[nt][e]);
+                }
+                pb[nt][0] = transpose(pack_half(u[nt][0], u[nt][1]));
+                pb[nt][1] = transpose(pack_half(u[nt][2], u[nt][3]));
+            }
+            // ---- values: tile x takes bytes 2 x and 2 x + 1 of the thread's of every key ----
+#pragma unroll
+            for (int x = 0; x < MTILES; ++x) {
+                unsigned a[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
+                    a[q] = half2_of((unsigned short)__byte_perm(v[e][b / 4], v[e + 1][b / 4], 0x0040u + 0x0011u * (b & 3)));
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][x], a, pb[nt][0], pb[nt][1]);
             }
         }
-    }
-    if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    __syncthreads();  // the rings are filled again
+
+        // ---- the warps meet, where the rings were ----
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (broken) {  // a wait gave up: the result is void; what is still on its way must land before the memory serves another end
+            if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
+            for (int i = max(0, filled - STAGES); i < filled; ++i) (void)tma::mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
+        }
+        // the rings were written by the other proxy too, and will be: order what threads do to the same places
+        if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncthreads();
+        float* merge = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], x);
+                const int row = 8 * nt + 2 * t + e;
+                if (row0 + row >= rows) continue;
+                if (g == 0) {
+                    stats[warp][row][0] = m1[nt][e];
+                    stats[warp][row][1] = m2[nt][e];
+                    stats[warp][row][2] = sum[nt][e];
+                }
+                // lanes (D / 8) g + 2 x, + 1 at columns 16 x + 2 g, + 1: the warp's stores meet in no bank
+                float* at = merge + ((size_t)warp * ROWS + row) * PITCH + 2 * g;
+#pragma unroll
+                for (int x = 0; x < MTILES; ++x) *reinterpret_cast<float2*>(at + 16 * x) = make_float2(o[nt][x][e], o[nt][x][2 + e]);
+            }
+        __syncthreads();
+        const int live_rows = min(ROWS, rows - row0);
+        for (int i = threadIdx.x; i < live_rows * (D / 2); i += THREADS) {
+            const int row = i / (D / 2), c = (i - row * (D / 2)) * 2;
+            float a = NOTHING, b = NOTHING;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                a = fmaxf(a, stats[w][row][0]);
+                b = fmaxf(b, stats[w][row][1]);
+            }
+            float total = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                total += stats[w][row][2] * exp2_fast(stats[w][row][0] - a);
+                const float f = exp2_fast(stats[w][row][1] - b);
+                const float2 x = *reinterpret_cast<const float2*>(merge + ((size_t)w * ROWS + row) * PITCH + c);
+                y0 = fmaf(x.x, f, y0);
+                y1 = fmaf(x.y, f, y1);
+            }
+            if (part < 0) {
+                finish<D>(p, first, h, row0 + row, c, a, b, total, y0, y1);
+            } else {
+                *reinterpret_cast<float2*>(p.part_sums + ((size_t)part * ROWS + row) * PITCH + c) = make_float2(y0, y1);
+                if (c == 0) {
+                    float* st = p.part_stats + ((size_t)part * ROWS + row) * 3;
+                    st[0] = a;
+                    st[1] = b;
+                    st[2] = total;
+                }
+            }
+        }
+        if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncthreads();  // the rings are filled again
     }
 }
 
@@ -690,21 +706,28 @@ attention8_join_kernel(const Attn8Params p) {
     }
 }
 
-template <int D, int NT, int RUN>
-int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
+template <int D, int NT, int RUN, int WARPS>
+int launch_warps(const Attn8Params& p, int longest, cudaStream_t stream) {
     constexpr size_t ring = (size_t)WARPS * STAGES * 2 * TILE * D, merge = (size_t)WARPS * 8 * NT * (D + 4) * sizeof(float);
     constexpr size_t smem = (ring > merge ? ring : merge) + 1024;
     const long long row_tiles = ((long long)longest * p.G + 8 * NT - 1) / (8 * NT), pairs = (long long)p.requests * p.KV;
     if (row_tiles > 65535 || pairs > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
-    const cudaError_t e = cudaFuncSetAttribute(attention8_kernel<D, NT, RUN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
+    auto kernel = attention8_kernel<D, NT, RUN, WARPS>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
     CUtensorMap map = {};
     const uint64_t values = (uint64_t)p.KV * p.page_size, keys = p.pages * 2 * values;  // a key's value lies so many places behind it
-    if (RUN && !tma::make_map_2d_u8_twice(&map, p.pool, keys - values, D, D, values * D, RUN, D, Stage<D, RUN ? RUN : TILE>::SWIZZLE)) return LLM_ERR_UNSUPPORTED;
+    if (RUN && !tma::make_map_2d_u8_twice(&map, p.pool, keys - values, D, D, values * D, RUN, D, Stage<D, RUN ? RUN : TILE>::SWIZZLE))
+        return LLM_ERR_UNSUPPORTED;
     const dim3 units((unsigned)pairs, (unsigned)row_tiles);
-    const int code = launch_pdl(attention8_kernel<D, NT, RUN>, p.ranges ? dim3(p.ranges) : units, dim3(THREADS), smem, stream, p, map);
+    const int code = launch_pdl(kernel, p.ranges ? dim3(p.ranges) : units, dim3(WARPS * 32), smem, stream, p, map);
     if (code || !p.ranges) return code;
     return launch_pdl(attention8_join_kernel<D, NT>, units, dim3(JOIN_THREADS), 0, stream, p);
+}
+
+template <int D, int NT, int RUN>
+int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
+    return p.warps == 2 ? launch_warps<D, NT, RUN, 2>(p, longest, stream) : launch_warps<D, NT, RUN, 8>(p, longest, stream);
 }
 
 }  // namespace
@@ -714,25 +737,28 @@ LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longe
 
 // q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, on 16
 // bytes; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
-// most tokens a request brings; with `below` requests that bring so many or more are left out, and their rows of out as they are.  out [n, H D].  window 0: none.  ranges: CTAs that share the step's keys evenly, with scratch memory of
-// ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and tile of rows.  D 64 or 128.
+// most tokens a request brings; with `below` requests that bring so many or more are left out, and their
+// rows of out as they are.  out [n, H D].  window 0: none.  warps of a CTA: 2 or 8.  ranges: CTAs that share the step's keys evenly, with
+// scratch memory of ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and
+// tile of rows.  D 64 or 128.
 LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long long out_stride, const void* pool, const void* exponents,
                               const int* page_table, int table_width, const int* cu_tokens, const int* context_lens, int requests, int n,
-                              int longest, int below, int H, int KV, int D, int page_size, int pages, int window, float scale, int ranges,
+                              int longest, int below, int H, int KV, int D, int page_size, int pages, int window, float scale, int warps, int ranges,
                               float* scratch, int* error_flag, cudaStream_t stream) {
     if (n <= 0 || requests <= 0) return 0;
-    if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || ranges < 0 || window < 0 ||
+    if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || (warps != 2 && warps != 8) || ranges < 0 || window < 0 ||
         (ranges && (!scratch || requests > MAX_REQUESTS || ((uintptr_t)scratch & 15))) || (q_stride & 3) || ((uintptr_t)q & 7) ||
         (out_stride & 3) || ((uintptr_t)out & 7) || ((uintptr_t)pool & 15) || ((uintptr_t)exponents & 15) ||
         (long long)table_width * page_size > 0x7fff0000)
         return LLM_ERR_BAD_ARGUMENT;
     const int rows = llm_attention8_rows(longest, H / KV);
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
-                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, below, error_flag, ranges,
+                     page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, below, error_flag, warps, ranges,
                      scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};
     // a tensor map's rows are counted in 32 bits
     const int run = (long long)pages * 2 * KV * page_size > 0x7fffffffLL ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 0;
-#define ATTENTION8(D_, NT_) (run == 16 ? launch<D_, NT_, 16>(p, longest, stream) : run == 8 ? launch<D_, NT_, 8>(p, longest, stream) : launch<D_, NT_, 0>(p, longest, stream))
+#define ATTENTION8(D_, NT_) \
+    (run == 16 ? launch<D_, NT_, 16>(p, longest, stream) : run == 8 ? launch<D_, NT_, 8>(p, longest, stream) : launch<D_, NT_, 0>(p, longest, stream))
     if (D == 64) return rows == 8 ? ATTENTION8(64, 1) : ATTENTION8(64, 2);
     if (D == 128) return rows == 8 ? ATTENTION8(128, 1) : ATTENTION8(128, 2);
 #undef ATTENTION8

@@ -96,7 +96,7 @@ _SIGNATURES = {
     "llm_linear8": [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "llm_expand_pages8": [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp],
-    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
+    "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
 }
 
@@ -2468,8 +2468,10 @@ def rope_kv_write8(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tens
 def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tensor, page_table: torch.Tensor, ctx, *, num_heads: int,
                      num_kv_heads: int, head_dim: int, scale: float, window: int | None = None) -> torch.Tensor:
     """:func:`paged_attention` over 8-bit pages as :func:`rope_kv_write8` leaves them.  ``q`` rows (bfloat16) start with the rotated query
-    heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  Where requests may be
-    long their keys are spread evenly over the CTAs, wherever requests begin and end, and joined by a second kernel.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
+    heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  Where it pays the keys
+    are spread evenly over the CTAs, wherever requests begin and end, and joined by a second kernel.  Requests that bring so many new tokens
+    that :func:`paged_attention` would take them to tcgen05 have their pages unpacked to bfloat16 first, in scratch memory of at most 2 GiB,
+    and go the same way from there.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
     width = num_heads * head_dim
     if not (q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= width and q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0
             and num_kv_heads > 0 and num_heads % num_kv_heads == 0 and (window is None or window >= 1)):
@@ -2498,14 +2500,14 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
                 return out
     keys = getattr(ctx, "max_context_len", None) or int(context_lens.max())
     group = num_heads // num_kv_heads
-    ranges = _attention8_ranges(requests, num_kv_heads, longest * group, keys if window is None else min(keys, window + longest))
+    warps, ranges = _attention8_split(requests, num_kv_heads, longest * group, keys if window is None else min(keys, window + longest), head_dim)
     scratch = None
     if ranges:
         scratch = q.new_empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32)
         add_launches(1)
     _check8(_launch("llm_attention8", q.data_ptr(), q.stride(0), out.data_ptr(), width, pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), page_table.shape[1],
                     cu_tokens.data_ptr(), context_lens.data_ptr(), requests, n, longest, below, num_heads, num_kv_heads, head_dim, pool.shape[3],
-                    pool.shape[0], int(window or 0), float(scale), ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
+                    pool.shape[0], int(window or 0), float(scale), warps, ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
             "paged_attention8")
     return out
 
@@ -2539,14 +2541,29 @@ def _attention8_portions(q, pool, exponents, page_table, ctx, out, heads: int, k
     return least
 
 
-_ATTENTION8_RANGES: int | None = None  # for measurements: so many whatever the rule says
+_ATTENTION8_SPLIT: tuple | None = None  # for tests and measurements: (warps, stretches) whatever the rule says
 
 
-def _attention8_ranges(requests: int, kv_heads: int, rows: int, keys: int) -> int:
-    """Over how many CTAs a step's keys are spread evenly (0: a CTA takes a tile of rows with all its keys): as many as there is room for at
-    once, where requests may be long."""
-    if _ATTENTION8_RANGES is not None:
-        return _ATTENTION8_RANGES
-    if keys <= 256 or requests > 1024:
-        return 0
-    return _sm_count() * (2 if rows <= 8 else 1)
+def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_dim: int) -> tuple:
+    """How :func:`paged_attention8` shares its work out: ``(warps of a CTA, stretches)``.
+
+    A unit is a tile of 8 or 16 rows of a request and a key head, with at most ``keys`` keys.  Without stretches (0) a CTA takes a unit; with
+    them the keys of all units are dealt out evenly and a second kernel joins what was cut.  Measured on 148 SMs with heads of 128 lanes
+    (64 lanes: two thirds of what goes by keys), CTAs of 8 warps, requests of random lengths up to k thousands of keys, u units an SM: a CTA by itself takes 4 + 8 k us
+    and an SM 2 + 6 k us a unit, against 12 + u (6 + 5 k) us for stretches.  64 units of 4,000 keys: 36.5 us, in stretches 23.2; 256 of 8,191:
+    106 and 83; 256 of 1,000: 18.3 and 27.9; 1,024 of 2,000: 84 and 109.  Stretches are as many as CTAs find room at once, or half of them
+    where there is little for each, which leaves less to join: 8 units of 8,000 keys 17.4 us instead of 22.8, 64 of 4,000 28.3
+    instead of 23.2.  Many short units are better off with CTAs of 2 warps, of which there is room for four times as many: 1,824 units of
+    20 keys take 13.3 us instead of 32.7, of 250 keys 29 instead of 44; 256 units of 1,000 30 instead of 18."""
+    if _ATTENTION8_SPLIT is not None:
+        return _ATTENTION8_SPLIT
+    height = 8 if rows <= 8 else 16
+    units, sms = requests * kv_heads * -(-rows // height), _sm_count()
+    if keys <= 512 and units > 2 * sms:
+        return 2, 0
+    if keys <= 256 or requests > 1024:  # (the list of requests' shares is held in shared memory)
+        return 8, 0
+    k = keys * (head_dim + 64) / 192e3
+    if max(4 + 8 * k, -(-units // sms) * (2 + 6 * k)) <= 12 + units / sms * (6 + 5 * k):
+        return 8, 0
+    return 8, sms * (2 if height == 8 and units * keys >= 1700 * sms else 1)

@@ -322,6 +322,32 @@ def test_attention_of_prompt_portions(H, KV, D, page_size, counts, held, window)
         assert (off <= (2.0**-8 + 2.0**-14) * size + 2.0**-8 * want.abs()).all(), r
 
 
+@pytest.mark.parametrize("split", [(2, 0), (8, 0), (8, 1), (8, 5), (8, 148), (2, 9)], ids=str)
+@pytest.mark.parametrize("H,KV,D,page_size", [(8, 2, 64, 16), (40, 4, 64, 8), (16, 2, 128, 24), (20, 1, 128, 16), (4, 4, 128, 5)])
+def test_attention_however_it_is_shared_out(monkeypatch, H, KV, D, page_size, split):
+    counts, held = [1, 1, 7, 0, 1, 30], [1, 900, 130, 40, 0, 600]
+    monkeypatch.setattr(ops(), "_ATTENTION8_SPLIT", split)
+    ctx, table, _, pages = a_step(counts, held, page_size, 5)
+    pool, exps = pages8(pages, KV, page_size, D, 12)
+    q = torch.randn(ctx.num_tokens, H * D, generator=gen(4), device=DEV).to(BF16)
+    for window in (None, 50):
+        got = ops().paged_attention8(q, pool, exps, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1, window=window)
+        check_attention(got, q, pool, exps, table, ctx, H, D, 0.1, window, f"{split} {window}")
+
+
+def test_attention_of_many_short_requests():
+    """More tiles of rows than there is room for at once: CTAs of two warps."""
+    H, KV, D, page_size = 16, 16, 64, 16
+    g = torch.Generator().manual_seed(8)
+    held = torch.randint(1, 60, (50,), generator=g).tolist()
+    ctx, table, _, pages = a_step([1] * 50, held, page_size, 9)
+    pool, exps = pages8(pages, KV, page_size, D, 13)
+    q = torch.randn(50, H * D, generator=gen(5), device=DEV).to(BF16)
+    assert ops()._attention8_split(50, KV, 1, max(held), D) == (2, 0)
+    got = ops().paged_attention8(q, pool, exps, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.125)
+    check_attention(got, q, pool, exps, table, ctx, H, D, 0.125, None)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_reaches_the_rows_that_see(D):
     """NaN in a value or a key spoils the rows that see it and no other, also inside a tile of 16 keys that others see in part."""

@@ -112,7 +112,7 @@ def test_captured_steps_are_the_eager_ones(monkeypatch):
     from llmserve_triton_kernels_b200 import ops
     from llmserve_triton_kernels_b200.engine.batch import StepEntry
 
-    monkeypatch.setattr(ops, "_ATTENTION8_RANGES", 37)
+    monkeypatch.setattr(ops, "_ATTENTION8_SPLIT", (8, 37))
     g = torch.Generator().manual_seed(1)
     seqs = [torch.randint(0, 300, (n,), generator=g).tolist() for n in (200, 37, 90)]
     results = []
