@@ -5,8 +5,8 @@
 // k-block of both operands.  Its four products (K = 32 each) start from zero in tensor memory and leave it at once: the epilogue
 // warps add them to 32-bit sums in registers, times sx of their row and sw of their columns.  Scales of any value are allowed
 // that way, and no sum is longer than 128 terms before it is rounded to 32 bits.  Roles, by warp:
-//   warp 0     : TMA producer, a ring of STAGES slots;
-//   warp 1     : issues the products into one of NBUF accumulators of tensor memory, in turn;
+//   warps 0, 1 : TMA producers, every other slot of a ring of STAGES each;
+//   warps 2, 3 : issue the products, every other k-block each, into one of NBUF accumulators of tensor memory, in turn;
 //   warps 4-19 : the sums.  A warp owns its 32 rows (lanes) and a quarter of the tile's columns, two columns to an instruction
 //                (fma.rn.f32x2).  The sums and 32 columns on their way need more registers than 640 threads are launched with: the
 //                first four warps give theirs up.
@@ -29,21 +29,15 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int BM = 128, BK = 128, UMMA_K = 32, EPI_WARPS = 16, FIRST_EPI = 4;
+constexpr int BM = 128, BK = 128, UMMA_K = 32, EPI_WARPS = 16, FIRST_EPI = 4, FIRST_ISSUER = 2;
 constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
 // 640 threads are launched with 96 registers each: 5 x 96 = 32 + 4 x 112
 constexpr int FEW_REGISTERS = 32, MANY_REGISTERS = 112;
 
-__device__ __forceinline__ unsigned long long pair_of(unsigned lo, unsigned hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-
 // sums += columns * scale, 32 columns as 16 pairs.
 __device__ __forceinline__ void add_columns(unsigned long long* sums, const unsigned (&v)[32], unsigned long long scale) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sums[j]) : "l"(pair_of(v[2 * j], v[2 * j + 1])), "l"(scale));
+    for (int j = 0; j < 16; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sums[j]) : "l"(umma::pair_of(v[2 * j], v[2 * j + 1])), "l"(scale));
 }
 
 // 32 rows (the warp's lanes) x 32 columns of sums, turned round in shared memory so that lanes side by side write 16 bytes each of one row:
@@ -90,10 +84,10 @@ __device__ __forceinline__ void store_piece(const linear8::Operands& p, unsigned
     __syncwarp();  // the piece is written again
 }
 
-template <int BN, int STAGES, typename TO>
+template <int STAGES, typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
-    constexpr int A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN * BK;
+gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    constexpr int BN = 128, A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN * BK;
     constexpr int NBUF = 4, TMEM_COLS = NBUF * BN;
     static_assert(TMEM_COLS == 512, "all columns of tensor memory");
     constexpr int COLS = BN / (EPI_WARPS / 4);  // of an epilogue warp
@@ -101,7 +95,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
 
@@ -120,21 +114,24 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
             tma::mbar_init(&acc_full[b], 1);
             tma::mbar_init(&acc_empty[b], EPI_WARPS);
         }
-        tma::mbar_init(&drained, 1);
+        tma::mbar_init(&drained[0], 1);
+        tma::mbar_init(&drained[1], 1);
         gave_up = 0;
         tma::mbar_fence_init();
         tma::prefetch_map(&xmap);
         tma::prefetch_map(&wmap);
     }
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tma::smem_addr(&tmem_base)), "n"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    pdl_wait();  // x comes from the kernel before
-    pdl_trigger();
+    if (warp >= FIRST_ISSUER) {  // x and its scales come from the kernel before; the producers ask for weights first
+        pdl_wait();
+        pdl_trigger();
+    }
 
     auto fail = [&]() {
         *(volatile int*)&gave_up = 1;
@@ -183,7 +180,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
-                    const unsigned long long both = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+                    const unsigned long long both = umma::pair_of(__float_as_uint(scale), __float_as_uint(scale));
 #pragma unroll
                     for (int c = 0; c < COLS; c += 32) {
                         unsigned v[32];
@@ -209,60 +206,78 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
             fail();
             return false;
         };
-        if (warp == 0) {
-            // ---- producer ----
+        const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
+        if (warp < FIRST_ISSUER) {
+            // ---- producers ----
             int it = 0, s = 0, turn = 0;
             bool ok = true;
+            const int ahead = early ? min(STAGES, kblocks) : 0;  // slots whose weights are asked for while x is still made
+            if (umma::elect_one()) {
+                for (int i = which; i < ahead; i += 2) {
+                    tma::mbar_expect_tx(&full[i], SLOT_BYTES);
+                    tma::load_2d(ring + (size_t)i * SLOT_BYTES + A_BYTES, &wmap, i * BK, ((int)blockIdx.x / row_tiles) * BN, &full[i]);
+                }
+            }
+            __syncwarp();
+            pdl_wait();
+            pdl_trigger();
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
                 const int m0 = (tile % row_tiles) * BM, n0 = (tile / row_tiles) * BN;
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
-                    if (!ok) break;
-                    unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                    if (umma::elect_one()) {
-                        tma::mbar_expect_tx(&full[s], SLOT_BYTES);
-                        tma::load_2d(slot, &xmap, kb * BK, m0, &full[s]);
-                        tma::load_2d(slot + A_BYTES, &wmap, kb * BK, n0, &full[s]);
+                    if ((it & 1) == which) {
+                        if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                        if (!ok) break;
+                        unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                        if (umma::elect_one()) {
+                            if (it >= ahead) {
+                                tma::mbar_expect_tx(&full[s], SLOT_BYTES);
+                                tma::load_2d(slot + A_BYTES, &wmap, kb * BK, n0, &full[s]);
+                            }
+                            tma::load_2d(slot, &xmap, kb * BK, m0, &full[s]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
             if (!ok)  // nobody waits for the copies on their way any more
-                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
-        } else if (warp == 1) {
-            // ---- tensor-core issuer ----
+                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
+                    if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        } else {
+            // ---- tensor-core issuers ----
             int it = 0, s = 0, turn = 0;
             bool ok = true;
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const int buf = it % NBUF;
-                    ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                    const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
-                    const unsigned d = tmem_base + buf * BN;
-                    if (umma::elect_one()) {
+                    if ((it & 1) == which) {
+                        const int buf = it % NBUF;
+                        ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                        const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
+                        const unsigned d = tmem_base + buf * BN;
+                        if (umma::elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
-                            umma::mma_e4m3(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
-                        umma::commit(&empty[s]);
-                        umma::commit(&acc_full[buf]);
+                            for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
+                                umma::mma_e4m3(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
+                            umma::commit(&empty[s]);
+                            umma::commit(&acc_full[buf]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
             if (!ok) {  // nor for the products
-                if (umma::elect_one()) umma::commit(&drained);
-                (void)tma::mbar_wait(&drained, 0);
+                if (umma::elect_one()) umma::commit(&drained[which]);
+                (void)tma::mbar_wait(&drained[which], 0);
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
@@ -273,7 +288,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int* error_flag, const __grid_co
 // the way from L2 to an SM does not bring in the products' time; a pair's needs 32 KB an SM.
 template <int STAGES, typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
     constexpr int BN = 256, A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN / 2 * BK;  // of one CTA
     constexpr int NBUF = 2, TMEM_COLS = NBUF * BN;
     constexpr int COLS = BN / (EPI_WARPS / 4);  // of an epilogue warp
@@ -281,7 +296,7 @@ gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_const
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
 
@@ -301,21 +316,24 @@ gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_const
             tma::mbar_init(&acc_full[b], 1);
             tma::mbar_init(&acc_empty[b], 2 * EPI_WARPS);  // the first CTA's is waited for, by both CTAs' warps
         }
-        tma::mbar_init(&drained, 1);
+        tma::mbar_init(&drained[0], 1);
+        tma::mbar_init(&drained[1], 1);
         gave_up = 0;
         tma::mbar_fence_init();
         tma::prefetch_map(&xmap);
         tma::prefetch_map(&wmap);
     }
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tma::smem_addr(&tmem_base)), "n"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // both CTAs' barriers and tensor memory are there
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    pdl_wait();  // x comes from the kernel before
-    pdl_trigger();
+    if (warp >= FIRST_ISSUER) {  // x and its scales come from the kernel before; the producers ask for weights first
+        pdl_wait();
+        pdl_trigger();
+    }
 
     auto fail = [&]() {
         *(volatile int*)&gave_up = 1;
@@ -364,7 +382,7 @@ gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_const
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
-                    const unsigned long long both = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+                    const unsigned long long both = umma::pair_of(__float_as_uint(scale), __float_as_uint(scale));
 #pragma unroll
                     for (int c = 0; c < COLS; c += 32) {
                         unsigned v[32];
@@ -390,70 +408,89 @@ gemm8_pair_kernel(const linear8::Operands p, int* error_flag, const __grid_const
             fail();
             return false;
         };
-        if (warp == 0) {
-            // ---- producer ----
+        const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
+        if (warp < FIRST_ISSUER) {
+            // ---- producers ----
             int it = 0, s = 0, turn = 0;
             bool ok = true;
+            const int ahead = early ? min(STAGES, kblocks) : 0;  // slots whose weights are asked for while x is still made
+            if (umma::elect_one()) {
+                for (int i = which; i < ahead; i += 2) {
+                    if (place == 0) tma::mbar_expect_tx(&full[i], 2 * SLOT_BYTES);  // both CTAs' bytes
+                    tma::load_2d_pair(ring + (size_t)i * SLOT_BYTES + A_BYTES, &wmap, i * BK, (pair / row_tiles) * BN + place * (BN / 2), &full[i]);
+                }
+            }
+            __syncwarp();
+            pdl_wait();
+            pdl_trigger();
             for (int tile = pair; tile < tiles && ok; tile += pairs) {
                 const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + place * (BN / 2);
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
-                    if (!ok) break;
-                    unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                    if (umma::elect_one()) {
-                        if (place == 0) tma::mbar_expect_tx(&full[s], 2 * SLOT_BYTES);  // both CTAs' bytes
-                        tma::load_2d_pair(slot, &xmap, kb * BK, m0, &full[s]);
-                        tma::load_2d_pair(slot + A_BYTES, &wmap, kb * BK, n0, &full[s]);
+                    if ((it & 1) == which) {
+                        if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                        if (!ok) break;
+                        unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                        if (umma::elect_one()) {
+                            if (it >= ahead) {
+                                if (place == 0) tma::mbar_expect_tx(&full[s], 2 * SLOT_BYTES);
+                                tma::load_2d_pair(slot + A_BYTES, &wmap, kb * BK, n0, &full[s]);
+                            }
+                            tma::load_2d_pair(slot, &xmap, kb * BK, m0, &full[s]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
             // nobody waits for the copies on their way any more (they are counted at the first CTA, which outlives them: the CTAs leave together)
             if (!ok && place == 0)
-                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
-        } else if (warp == 1 && place == 0) {
-            // ---- tensor-core issuer, for both CTAs ----
+                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
+                    if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        } else if (place == 0) {
+            // ---- tensor-core issuers, for both CTAs ----
             int it = 0, s = 0, turn = 0;
             bool ok = true;
             for (int tile = pair; tile < tiles && ok; tile += pairs) {
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const int buf = it % NBUF;
-                    ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                    const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
-                    const unsigned d = tmem_base + buf * BN;
-                    if (umma::elect_one()) {
+                    if ((it & 1) == which) {
+                        const int buf = it % NBUF;
+                        ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                        const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
+                        const unsigned d = tmem_base + buf * BN;
+                        if (umma::elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
-                            umma::mma_e4m3_pair(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
-                        umma::commit_pair(&empty[s]);
-                        umma::commit_pair(&acc_full[buf]);
+                            for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
+                                umma::mma_e4m3_pair(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
+                            umma::commit_pair(&empty[s]);
+                            umma::commit_pair(&acc_full[buf]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
             if (!ok) {  // nor for the products
-                if (umma::elect_one()) umma::commit_pair(&drained);
-                (void)tma::mbar_wait(&drained, 0);
+                if (umma::elect_one()) umma::commit_pair(&drained[which]);
+                (void)tma::mbar_wait(&drained[which], 0);
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
 }
 
-template <int BN, int STAGES, typename TO>
-int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
+template <typename TO>
+int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
+    constexpr int BN = 128, STAGES = 4;
     constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
-    auto kernel = gemm8_tcgen05_kernel<BN, STAGES, TO>;
+    auto kernel = gemm8_tcgen05_kernel<STAGES, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
     CUtensorMap xmap, wmap;
@@ -463,11 +500,11 @@ int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
     const long long tiles = (long long)((p.N + BN - 1) / BN) * ((p.M + BM - 1) / BM);
     if (tiles > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
     const int sms = device_sms();
-    return launch_pdl(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(THREADS), smem, stream, p, error_flag, xmap, wmap);
+    return launch_pdl(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(THREADS), smem, stream, p, early, error_flag, xmap, wmap);
 }
 
 template <typename TO>
-int launch_pair(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
+int launch_pair(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     constexpr int STAGES = 4;
     constexpr size_t smem = (size_t)STAGES * 2 * BM * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
     auto kernel = gemm8_pair_kernel<STAGES, TO>;
@@ -494,21 +531,21 @@ int launch_pair(const linear8::Operands& p, int* error_flag, cudaStream_t stream
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p, error_flag, xmap, wmap);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, early, error_flag, xmap, wmap);
 }
 
 // A pair's tile of 256 x 256 takes 0.66 us a k-block, a CTA's of 128 x 128 0.45: pairs are faster (4,096 x 28,672 x 4,096: 533 us against
 // 714) but where their tiles leave most of them without work (512 x 4,096 x 4,096, 32 tiles for 74 pairs: 25.3 us against 20.2).
 template <typename TO>
-int by_shape(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
+int by_shape(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     const long long sms = device_sms(), pairs = sms / 2;
     auto rounds = [&](long long side, long long at_once) { return (((p.M + side - 1) / side) * ((p.N + side - 1) / side) + at_once - 1) / at_once; };
-    if (rounds(256, pairs) * 66 <= rounds(128, sms) * 45) return launch_pair<TO>(p, error_flag, stream);
-    return launch<128, 4, TO>(p, error_flag, stream);
+    if (rounds(256, pairs) * 66 <= rounds(128, sms) * 45) return launch_pair<TO>(p, early, error_flag, stream);
+    return launch<TO>(p, early, error_flag, stream);
 }
 
 }  // namespace
 
-int linear8::many(const Operands& p, int* error_flag, cudaStream_t stream) {
-    return p.out_dtype == LLM_F32 ? by_shape<float>(p, error_flag, stream) : by_shape<__nv_bfloat16>(p, error_flag, stream);
+int linear8::many(const Operands& p, bool early, int* error_flag, cudaStream_t stream) {
+    return p.out_dtype == LLM_F32 ? by_shape<float>(p, early, error_flag, stream) : by_shape<__nv_bfloat16>(p, early, error_flag, stream);
 }

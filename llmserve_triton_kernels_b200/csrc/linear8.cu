@@ -28,5 +28,5 @@ LLM_EXPORT int llm_linear8(const void* x, int x_dtype, long long ldx, const floa
     // The weights as the tall operand where x fills no tile of 128 rows by half, and where there are so few tiles that several CTAs may
     // share one's k-blocks (which that kernel does).
     const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
-    return M <= 64 || tiles * 2 <= device_sms() ? linear8::some(p, error_flag, stream) : linear8::many(p, error_flag, stream);
+    return M <= 64 || tiles * 2 <= device_sms() ? linear8::some(p, !given, error_flag, stream) : linear8::many(p, !given, error_flag, stream);
 }

@@ -23,7 +23,7 @@ struct Operands {
 int quantize_rows(const void* x, int dtype, long long ldx, unsigned char* values, float* scales, int M, int K, cudaStream_t stream);
 // `early`: w and sw may be read while the kernel in front still runs.
 int few(const Operands& p, bool early, cudaStream_t stream);
-int some(const Operands& p, int* error_flag, cudaStream_t stream);
-int many(const Operands& p, int* error_flag, cudaStream_t stream);
+int some(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
+int many(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
 
 }  // namespace linear8

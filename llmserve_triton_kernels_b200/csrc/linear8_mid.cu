@@ -3,7 +3,7 @@
 //
 // The reading of the weights bounds it: 16 KB a k-block and SM.  Roles, rings and accumulators are those of gemm8_tcgen05.cu (a
 // slot is one 128-byte k-block of both operands, its four products start from zero, the sums live in registers).  What differs: a
-// thread of the sums holds one row of w and half of x's rows, whose scales differ from column to column; they come through a few
+// thread of the sums holds one row of w and 32 of x's rows, whose scales differ from column to column; they come through a few
 // bytes of shared memory of the warp's own, 16 bytes a read for everyone.  Where there are fewer tiles than SMs, `SPLIT` CTAs (a
 // cluster) share a tile's k-blocks and add up in one another's shared memory.
 #include "common.cuh"
@@ -17,26 +17,19 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int BM = 128, BK = 128, UMMA_K = 32, EPI_WARPS = 8, FIRST_EPI = 4, NBUF = 4;
-constexpr int THREADS = (FIRST_EPI + EPI_WARPS) * 32;
+constexpr int BM = 128, BK = 128, UMMA_K = 32, FIRST_EPI = 4, FIRST_ISSUER = 2, NBUF = 4, MAX_SPLIT = 4;
 
-__device__ __forceinline__ unsigned long long pair_of(unsigned lo, unsigned hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-
-template <int BN, int STAGES, typename TO>
-__global__ void __launch_bounds__(THREADS, 1)
-linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
-    constexpr int A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN * BK, COLS = BN / 2, PITCH = BM + 4;
-    constexpr int TMEM_COLS = NBUF * BN;
+template <int BN, int STAGES, int EPI_WARPS, typename TO>
+__global__ void __launch_bounds__((FIRST_EPI + EPI_WARPS) * 32, 1)
+linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    constexpr int A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN * BK, COLS = BN / (EPI_WARPS / 4), PITCH = BM + 4;
+    constexpr int TMEM_COLS = NBUF * BN, THREADS = (FIRST_EPI + EPI_WARPS) * 32;
     static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "columns of tensor memory come in powers of two");
     static_assert((size_t)BN * PITCH * 4 <= (size_t)STAGES * SLOT_BYTES, "the sums of a split tile lie where the ring was");
     constexpr unsigned IDESC = umma::idesc_e4m3(BM, BN);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ __align__(16) float scales[EPI_WARPS][2][COLS];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up;
@@ -57,21 +50,24 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
             tma::mbar_init(&acc_full[b], 1);
             tma::mbar_init(&acc_empty[b], EPI_WARPS);
         }
-        tma::mbar_init(&drained, 1);
+        tma::mbar_init(&drained[0], 1);
+        tma::mbar_init(&drained[1], 1);
         gave_up = 0;
         tma::mbar_fence_init();
         tma::prefetch_map(&xmap);
         tma::prefetch_map(&wmap);
     }
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tma::smem_addr(&tmem_base)), "n"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    pdl_wait();  // x comes from the kernel before
-    pdl_trigger();
+    if (warp >= FIRST_ISSUER) {  // x and its scales come from the kernel before; the producers ask for weights first
+        pdl_wait();
+        pdl_trigger();
+    }
 
     auto fail = [&]() {
         *(volatile int*)&gave_up = 1;
@@ -84,61 +80,79 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
         return false;
     };
 
-    if (warp == 0) {
-        // ---- producer ----
+    const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
+    if (warp < FIRST_ISSUER) {
+        // ---- producers ----
         int it = 0, s = 0, turn = 0;
         bool ok = true;
+        const int ahead = early ? min(STAGES, k_hi - k_lo) : 0;  // slots whose weights are asked for while x is still made
+        if (umma::elect_one()) {
+            for (int i = which; i < ahead; i += 2) {
+                tma::mbar_expect_tx(&full[i], SLOT_BYTES);
+                tma::load_2d(ring + (size_t)i * SLOT_BYTES, &wmap, (k_lo + i) * BK, (first_tile % col_tiles) * BM, &full[i]);
+            }
+        }
+        __syncwarp();
+        pdl_wait();
+        pdl_trigger();
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
-                if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
-                if (!ok) break;
-                unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                if (umma::elect_one()) {
-                    tma::mbar_expect_tx(&full[s], SLOT_BYTES);
-                    tma::load_2d(slot, &wmap, kb * BK, (tile % col_tiles) * BM, &full[s]);
-                    tma::load_2d(slot + A_BYTES, &xmap, kb * BK, (tile / col_tiles) * BN, &full[s]);
+                if ((it & 1) == which) {
+                    if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                    if (!ok) break;
+                    unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                    if (umma::elect_one()) {
+                        if (it >= ahead) {
+                            tma::mbar_expect_tx(&full[s], SLOT_BYTES);
+                            tma::load_2d(slot, &wmap, kb * BK, (tile % col_tiles) * BM, &full[s]);
+                        }
+                        tma::load_2d(slot + A_BYTES, &xmap, kb * BK, (tile / col_tiles) * BN, &full[s]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 if (++s == STAGES) s = 0, ++turn;
             }
         }
         if (!ok)  // nobody waits for the copies on their way any more
-            for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
-    } else if (warp == 1) {
-        // ---- tensor-core issuer ----
+            for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
+                if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    } else if (warp < FIRST_EPI) {
+        // ---- tensor-core issuers ----
         int it = 0, s = 0, turn = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
-                const int buf = it % NBUF;
-                ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1)) && !failed();
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
-                const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
-                const unsigned d = tmem_base + buf * BN;
-                if (umma::elect_one()) {
+                if ((it & 1) == which) {
+                    const int buf = it % NBUF;
+                    ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1)) && !failed();
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
+                    const unsigned long long a = umma::desc_sw128(slot), b = umma::desc_sw128(slot + A_BYTES);
+                    const unsigned d = tmem_base + buf * BN;
+                    if (umma::elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k) umma::mma_e4m3(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
-                    umma::commit(&empty[s]);
-                    umma::commit(&acc_full[buf]);
+                        for (int k = 0; k < BK / UMMA_K; ++k) umma::mma_e4m3(d, a + 2 * k, b + 2 * k, IDESC, k != 0);
+                        umma::commit(&empty[s]);
+                        umma::commit(&acc_full[buf]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 if (++s == STAGES) s = 0, ++turn;
             }
         }
         if (!ok) {  // nor for the products
-            if (umma::elect_one()) umma::commit(&drained);
-            (void)tma::mbar_wait(&drained, 0);
+            if (umma::elect_one()) umma::commit(&drained[which]);
+            (void)tma::mbar_wait(&drained[which], 0);
         }
     } else if (warp >= FIRST_EPI) {
-        // ---- sums: rows (warp % 4) * 32 + lane of w, COLS rows of x from half * COLS on ----
-        const int quarter = warp & 3, half = (warp - FIRST_EPI) >> 2;
+        // ---- sums: rows (warp % 4) * 32 + lane of w, COLS rows of x from part * COLS on ----
+        const int quarter = warp & 3, part = (warp - FIRST_EPI) >> 2;
         float(&mine)[2][COLS] = scales[warp - FIRST_EPI];
         int it = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
-            const int n = (tile % col_tiles) * BM + quarter * 32 + lane, m_first = (tile / col_tiles) * BN + half * COLS;
+            const int n = (tile % col_tiles) * BM + quarter * 32 + lane, m_first = (tile / col_tiles) * BN + part * COLS;
             const float* sw = p.sw + (size_t)(tile % col_tiles) * p.kblocks;
             unsigned long long acc[COLS / 2];
 #pragma unroll
@@ -178,7 +192,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    const unsigned base = tmem_base + buf * BN + half * COLS + ((unsigned)(quarter * 32) << 16);
+                    const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
 #pragma unroll
                     for (int c = 0; c < COLS; c += 32) {
                         unsigned v[32];
@@ -192,8 +206,8 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&mine[i & 1][c + j]);
-                            asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc[(c + j) / 2]) : "l"(pair_of(v[j], v[j + 1])), "l"(s.x));
-                            asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc[(c + j) / 2 + 1]) : "l"(pair_of(v[j + 2], v[j + 3])), "l"(s.y));
+                            asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc[(c + j) / 2]) : "l"(umma::pair_of(v[j], v[j + 1])), "l"(s.x));
+                            asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(acc[(c + j) / 2 + 1]) : "l"(umma::pair_of(v[j + 2], v[j + 3])), "l"(s.y));
                         }
                     }
                     ++it;
@@ -212,13 +226,13 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
                 // The ring's slots have all been read by the products (they were waited for); their memory takes the sums.
                 float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) sums[(half * COLS + j) * PITCH + quarter * 32 + lane] = __uint_as_float((unsigned)(acc[j / 2] >> (32 * (j & 1))));
+                for (int j = 0; j < COLS; ++j) sums[(part * COLS + j) * PITCH + quarter * 32 + lane] = __uint_as_float((unsigned)(acc[j / 2] >> (32 * (j & 1))));
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    if (warp == 1) {
+    if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
@@ -231,14 +245,19 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
     for (int i = threadIdx.x; i < ((rows + split - 1) / split) * (BM / 4); i += THREADS) {
         const int m = (i / (BM / 4)) * split + rank, c = (i % (BM / 4)) * 4, n = n0 + c;
         if (m >= rows || n >= p.N) continue;
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < split; ++r) {
-            const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + m * PITCH + c, r));
-            y[0] += v.x;
-            y[1] += v.y;
-            y[2] += v.z;
-            y[3] += v.w;
-        }
+        float4 v[MAX_SPLIT];  // asked for together: each takes some 700 cycles
+#pragma unroll
+        for (int r = 0; r < MAX_SPLIT; ++r)
+            if (r < split) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + m * PITCH + c, r));
+        float y[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+        for (int r = 1; r < MAX_SPLIT; ++r)
+            if (r < split) {
+                y[0] += v[r].x;
+                y[1] += v[r].y;
+                y[2] += v[r].z;
+                y[3] += v[r].w;
+            }
         TO* out = reinterpret_cast<TO*>(p.out) + (size_t)(m0 + m) * p.ldo + n;
         if (n + 4 <= p.N && ((uintptr_t)out & (4 * sizeof(TO) - 1)) == 0) {
             store4(out, y);
@@ -248,13 +267,14 @@ linear8_mid_kernel(const linear8::Operands p, int split, int* error_flag, const 
                 if (n + j < p.N) out[j] = from_float<TO>(y[j]);
         }
     }
-    cluster.sync();  // nobody leaves while its sums are read
+    // nobody leaves while its sums are read (which has been done: nothing has to be made visible)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
 
-template <int BN, int STAGES, typename TO>
-int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
+template <int BN, int STAGES, int EPI_WARPS, typename TO>
+int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024;
-    auto kernel = linear8_mid_kernel<BN, STAGES, TO>;
+    auto kernel = linear8_mid_kernel<BN, STAGES, EPI_WARPS, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
     CUtensorMap xmap, wmap;
@@ -265,10 +285,10 @@ int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
     if (tiles > 0x7fffffffLL) return LLM_ERR_UNSUPPORTED;
     const int sms = device_sms();
     int split = 1;  // doubled while all CTAs still run at once and none has fewer than four k-blocks
-    while (split < 4 && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
+    while (split < MAX_SPLIT && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3((FIRST_EPI + EPI_WARPS) * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -280,12 +300,12 @@ int launch(const linear8::Operands& p, int* error_flag, cudaStream_t stream) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p, split, error_flag, xmap, wmap);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, split, early, error_flag, xmap, wmap);
 }
 
 }  // namespace
 
-int linear8::some(const Operands& p, int* error_flag, cudaStream_t stream) {
-    if (p.out_dtype == LLM_F32) return p.M <= 64 ? launch<64, 7, float>(p, error_flag, stream) : launch<128, 6, float>(p, error_flag, stream);
-    return p.M <= 64 ? launch<64, 7, __nv_bfloat16>(p, error_flag, stream) : launch<128, 6, __nv_bfloat16>(p, error_flag, stream);
+int linear8::some(const Operands& p, bool early, int* error_flag, cudaStream_t stream) {
+    if (p.out_dtype == LLM_F32) return p.M <= 64 ? launch<64, 7, 8, float>(p, early, error_flag, stream) : launch<128, 6, 16, float>(p, early, error_flag, stream);
+    return p.M <= 64 ? launch<64, 7, 8, __nv_bfloat16>(p, early, error_flag, stream) : launch<128, 6, 16, __nv_bfloat16>(p, early, error_flag, stream);
 }

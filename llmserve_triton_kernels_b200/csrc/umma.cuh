@@ -97,6 +97,13 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Two 32-bit numbers as an operand of the instructions on pairs.
+__device__ __forceinline__ unsigned long long pair_of(unsigned lo, unsigned hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+
 // The same in two halves, so that work goes on between asking and having: what was asked for may be used after its wait.
 __device__ __forceinline__ void tmem_ask32(unsigned taddr, unsigned (&r)[32]) {
     asm volatile(
