@@ -10,16 +10,17 @@
 //   warps 4-19 : the sums.  A warp owns its 32 rows (lanes) and a quarter of the tile's columns, two columns to an instruction
 //                (fma.rn.f32x2).  The sums and 32 columns on their way need more registers than 640 threads are launched with: the
 //                first four warps give theirs up.
-// The sums are what bounds it: one multiplication and addition for every 128 of a product take an SM's arithmetic 280 cycles for a
-// 128 x 256 tile's k-block, the reading of tensor memory 200 and the products 512, and they overlap in part (without the sums'
-// additions 4,096 x 28,672 x 4,096 took 395 us, with them 525).  What it measured: 533 us there, 1,806 TFLOP/s; the framework's bfloat16
-// product of the vendor's library reaches 1,670 at most on this chip.  Scales are read where rows lie side by side (linear8.h): from
-// [rows, blocks] the same product took 640 us.
+// The sums are what bounds it: what a warp does for a k-block of 32 columns (wait, read tensor memory, 16 instructions of sums, give
+// the accumulator back) takes it some 500 cycles beside three others on its quarter of the SM, the products 512 for a 256 x 256 tile of
+// a pair.  The roles that issue were the bound before they were two warps each: a k-block's waits, products and commits take one
+// warp 600 cycles (533 us for 4,096 x 28,672 x 4,096 with one, 459 with two: 2,096 TFLOP/s with x quantised in front).  Scales are read
+// where rows lie side by side (linear8.h): from [rows, blocks] the same product took 100 us more.
 // One CTA per SM walks 128 x 128 tiles, or a pair of CTAs 256 x 256, column tiles outermost, so that CTAs that run at the same time share their weights.  What lies beyond
 // the matrices arrives as zeros and is masked at the store.  Every wait is bounded; one that gives up sets *error_flag and the
 // roles run to their ends.
 #include "common.cuh"
 #include "linear8.h"
+#include "linear8_store.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -38,50 +39,6 @@ constexpr int FEW_REGISTERS = 32, MANY_REGISTERS = 112;
 __device__ __forceinline__ void add_columns(unsigned long long* sums, const unsigned (&v)[32], unsigned long long scale) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sums[j]) : "l"(umma::pair_of(v[2 * j], v[2 * j + 1])), "l"(scale));
-}
-
-// 32 rows (the warp's lanes) x 32 columns of sums, turned round in shared memory so that lanes side by side write 16 bytes each of one row:
-// a thread's own row would be a sector of each of 32 rows a store, which the way to memory takes several times as long for.
-template <typename TO>
-constexpr int PIECE_PITCH = 32 * sizeof(TO) + 16;
-template <typename TO>
-constexpr int PIECE_BYTES = 32 * PIECE_PITCH<TO>;
-template <typename TO>
-__device__ __forceinline__ void store_piece(const linear8::Operands& p, unsigned char* piece, const unsigned long long* sums, int m0, int n0, int lane) {
-    constexpr int EACH = 16 / sizeof(TO), LANES = 32 / EACH;  // columns of 16 bytes; lanes of a row
-    unsigned char* mine = piece + lane * PIECE_PITCH<TO>;
-#pragma unroll
-    for (int j = 0; j < 32; j += EACH) {
-        if constexpr (sizeof(TO) == 4) {
-            *reinterpret_cast<ulonglong2*>(mine + j * 4) = make_ulonglong2(sums[j / 2], sums[j / 2 + 1]);
-        } else {
-            unsigned u[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 a = __floats2bfloat162_rn(__uint_as_float((unsigned)sums[j / 2 + i]), __uint_as_float((unsigned)(sums[j / 2 + i] >> 32)));
-                u[i] = *reinterpret_cast<const unsigned*>(&a);
-            }
-            *reinterpret_cast<uint4*>(mine + j * 2) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-    }
-    __syncwarp();
-    const int c = (lane % LANES) * EACH, valid = p.N - n0 - c;
-    TO* out = reinterpret_cast<TO*>(p.out) + n0 + c;
-    const bool wide = valid >= EACH && ((uintptr_t)out & 15) == 0 && (p.ldo * sizeof(TO)) % 16 == 0;
-#pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 32 / LANES) {
-        const int row = r0 + lane / LANES, m = m0 + row;
-        if (m >= p.M) continue;
-        const unsigned char* from = piece + row * PIECE_PITCH<TO> + c * sizeof(TO);
-        if (wide) {
-            *reinterpret_cast<uint4*>(out + (size_t)m * p.ldo) = *reinterpret_cast<const uint4*>(from);
-        } else {
-#pragma unroll
-            for (int i = 0; i < EACH; ++i)
-                if (i < valid) out[(size_t)m * p.ldo + i] = reinterpret_cast<const TO*>(from)[i];
-        }
-    }
-    __syncwarp();  // the piece is written again
 }
 
 template <int STAGES, typename TO>
@@ -195,7 +152,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < COLS; c += 32) {
-                    if (n0 + c < p.N) store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
+                    if (n0 + c < p.N) linear8::store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * linear8::PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
                 }
             }
         }
@@ -397,7 +354,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < COLS; c += 32) {
-                    if (n0 + c < p.N) store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
+                    if (n0 + c < p.N) linear8::store_piece<TO>(p, staging + (size_t)(warp - FIRST_EPI) * linear8::PIECE_BYTES<TO>, acc + c / 2, m0 + quarter * 32, n0 + c, lane);
                 }
             }
         }
@@ -489,7 +446,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
 template <typename TO>
 int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     constexpr int BN = 128, STAGES = 4;
-    constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
+    constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK + 1024 + EPI_WARPS * linear8::PIECE_BYTES<TO>;
     auto kernel = gemm8_tcgen05_kernel<STAGES, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
@@ -506,7 +463,7 @@ int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t 
 template <typename TO>
 int launch_pair(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     constexpr int STAGES = 4;
-    constexpr size_t smem = (size_t)STAGES * 2 * BM * BK + 1024 + EPI_WARPS * PIECE_BYTES<TO>;
+    constexpr size_t smem = (size_t)STAGES * 2 * BM * BK + 1024 + EPI_WARPS * linear8::PIECE_BYTES<TO>;
     auto kernel = gemm8_pair_kernel<STAGES, TO>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // of the current device
     if (e != cudaSuccess) return (int)e;
@@ -517,30 +474,16 @@ int launch_pair(const linear8::Operands& p, int early, int* error_flag, cudaStre
     const long long tiles = (long long)((p.N + 255) / 256) * ((p.M + 255) / 256);
     if (tiles > 0x3fffffffLL) return LLM_ERR_UNSUPPORTED;
     const int pairs = device_sms() / 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles < pairs ? tiles : pairs) * 2);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p, early, error_flag, xmap, wmap);
+    return linear8::launch_clusters(kernel, (unsigned)(tiles < pairs ? tiles : pairs) * 2, THREADS, smem, 2, stream, p, early, error_flag, xmap, wmap);
 }
 
-// A pair's tile of 256 x 256 takes 0.66 us a k-block, a CTA's of 128 x 128 0.45: pairs are faster (4,096 x 28,672 x 4,096: 533 us against
-// 714) but where their tiles leave most of them without work (512 x 4,096 x 4,096, 32 tiles for 74 pairs: 25.3 us against 20.2).
+// A pair's tile of 256 x 256 takes 0.57 us a k-block, a CTA's of 128 x 128 0.39: pairs are faster (4,096 x 28,672 x 4,096: 459 us) but
+// where their tiles leave most of them without work (512 x 4,096 x 4,096, 32 tiles for 74 pairs: 18.5 us by single CTAs).
 template <typename TO>
 int by_shape(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
     const long long sms = device_sms(), pairs = sms / 2;
     auto rounds = [&](long long side, long long at_once) { return (((p.M + side - 1) / side) * ((p.N + side - 1) / side) + at_once - 1) / at_once; };
-    if (rounds(256, pairs) * 66 <= rounds(128, sms) * 45) return launch_pair<TO>(p, early, error_flag, stream);
+    if (rounds(256, pairs) * 57 <= rounds(128, sms) * 39) return launch_pair<TO>(p, early, error_flag, stream);
     return launch<TO>(p, early, error_flag, stream);
 }
 

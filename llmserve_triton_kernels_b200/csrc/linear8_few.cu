@@ -1,4 +1,4 @@
-// y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in b} x[m, k] w[n, k] for few rows (M <= 64): x and w in e4m3, a scale for every 128 k.
+// y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in b} x[m, k] w[n, k] for up to 16 rows: x and w in e4m3, a scale for every 128 k.
 //
 // The weights are read from HBM once, 16 bytes a lane straight into tensor-core fragments; the rows of x ride along as the
 // narrow side (the 16 rows of an mma.sync m16n8k32 tile are 16 output features, its 8 columns are 8 rows of x).  A lane takes
@@ -8,12 +8,16 @@
 //
 // A block's four products start from zero and enter the 32-bit sums times both scales.  (The e4m3 product of mma.sync adds
 // its 32 terms without loss on this chip: 2,048 terms came out within 1.6e-7 of the 64-bit sum.)
+//
+// The weights' bytes bound it, and where they are few what comes before the first of them: 8 rows by 28,672 features of 4,096 take 25.2
+// us, 4.7 TB/s (26 with x quantised in front), 1 row by 2,560 of 2,048 some 5.  9 to 16 rows take it twice the products, which
+// tell for large weights: 16 rows by 28,672 are left to linear8_mid.cu, by 4,096 not (8.8 us against 10).
 #include "common.cuh"
 #include "linear8.h"
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, BLOCK = 128;
+constexpr int THREADS = 256, WARPS = THREADS / 32, BLOCK = 128, GROUP = 2;  // GROUP: k-blocks that a warp asks for at once
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
@@ -28,12 +32,11 @@ __device__ __forceinline__ uint4 load_weights(const unsigned char* p) {
 }
 
 // GROUP k-blocks of 16 weight rows: rows g and g + 8, 32 bytes of each.
-template <int GROUP>
 struct Weights {
     uint4 v[GROUP][4];
 };
 
-template <int NT, int GROUP, typename TO>
+template <int NT, typename TO>
 __global__ void __launch_bounds__(THREADS)
 linear8_few_kernel(const linear8::Operands p, const int early) {
     extern __shared__ __align__(16) float red[];  // [2][WARPS][NT * 4][32]
@@ -41,7 +44,7 @@ linear8_few_kernel(const linear8::Operands p, const int early) {
     const int tiles = (p.N + 15) / 16;
     const int groups = (p.kblocks + WARPS * GROUP - 1) / (WARPS * GROUP);  // of every warp and tile
 
-    auto fetch = [&](Weights<GROUP>& w, int tile, int group) {
+    auto fetch = [&](Weights& w, int tile, int group) {
         const unsigned char* r0 = p.w + (size_t)min(tile * 16 + g, p.N - 1) * p.K;
         const unsigned char* r1 = p.w + (size_t)min(tile * 16 + g + 8, p.N - 1) * p.K;
 #pragma unroll
@@ -55,7 +58,7 @@ linear8_few_kernel(const linear8::Operands p, const int early) {
         }
     };
 
-    Weights<GROUP> now, next;
+    Weights now, next;
     int tile = blockIdx.x, group = 0, turn = 0;
     if (early) fetch(now, tile, 0);
     pdl_wait();
@@ -127,28 +130,15 @@ linear8_few_kernel(const linear8::Operands p, const int early) {
     }
 }
 
-template <int NT, int GROUP, typename TO>
+template <int NT, typename TO>
 int launch(const linear8::Operands& p, int early, cudaStream_t stream) {
-    constexpr size_t smem = 2 * WARPS * NT * 128 * sizeof(float);
-    auto kernel = linear8_few_kernel<NT, GROUP, TO>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-    }
     const int tiles = (p.N + 15) / 16, most = device_sms() * 2;
-    return launch_pdl(kernel, dim3(tiles < most ? tiles : most), dim3(THREADS), smem, stream, p, early);
-}
-
-template <typename TO>
-int by_rows(const linear8::Operands& p, int early, cudaStream_t stream) {
-    if (p.M <= 8) return launch<1, 2, TO>(p, early, stream);
-    if (p.M <= 16) return launch<2, 2, TO>(p, early, stream);
-    if (p.M <= 32) return launch<4, 2, TO>(p, early, stream);
-    return launch<8, 1, TO>(p, early, stream);
+    return launch_pdl(linear8_few_kernel<NT, TO>, dim3(tiles < most ? tiles : most), dim3(THREADS), 2 * WARPS * NT * 128 * sizeof(float), stream, p, early);
 }
 
 }  // namespace
 
 int linear8::few(const Operands& p, bool early, cudaStream_t stream) {
-    return p.out_dtype == LLM_F32 ? by_rows<float>(p, early, stream) : by_rows<__nv_bfloat16>(p, early, stream);
+    if (p.out_dtype == LLM_F32) return p.M <= 8 ? launch<1, float>(p, early, stream) : launch<2, float>(p, early, stream);
+    return p.M <= 8 ? launch<1, __nv_bfloat16>(p, early, stream) : launch<2, __nv_bfloat16>(p, early, stream);
 }

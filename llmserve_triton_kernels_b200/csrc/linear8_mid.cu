@@ -1,19 +1,19 @@
 // y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in b} x[m, k] w[n, k] for some rows of x, on tcgen05 with the weights as the tall
 // operand: a tile is 128 rows of w by up to 64 or 128 rows of x, so that no tile is mostly padding.
 //
-// The reading of the weights bounds it: 16 KB a k-block and SM.  Roles, rings and accumulators are those of gemm8_tcgen05.cu (a
-// slot is one 128-byte k-block of both operands, its four products start from zero, the sums live in registers).  What differs: a
-// thread of the sums holds one row of w and 32 of x's rows, whose scales differ from column to column; they come through a few
-// bytes of shared memory of the warp's own, 16 bytes a read for everyone.  Where there are fewer tiles than SMs, `SPLIT` CTAs (a
-// cluster) share a tile's k-blocks and add up in one another's shared memory.
+// Roles, rings and accumulators are those of gemm8_tcgen05.cu (a slot is one 128-byte k-block of both operands, its four products
+// start from zero, the sums live in registers).  What differs: a thread of the sums holds one row of w and 32 of x's rows, whose
+// scales differ from column to column; they come through a few bytes of shared memory of the warp's own, 16 bytes a read for everyone.
+// Where there are fewer tiles than SMs, `split` CTAs (a cluster) share a tile's k-blocks and add up in one another's shared memory.
+//
+// What bounds it: a k-block of 64 rows takes the sums' warps some 600 cycles (16 KB of weights in 0.33 us, 7.5 TB/s over all SMs), of 128
+// 850; and around them some 6 us of a launch, of first copies, and of the cluster's meeting and adding.  33 rows by 32,000 features of
+// 2,048: 19 us, by 4,096 of 14,336 16.9, by 4,096 of 4,096 9.8, each with x quantised in front.
 #include "common.cuh"
 #include "linear8.h"
+#include "linear8_store.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
-
-#include <cooperative_groups.h>
-
-namespace cg = cooperative_groups;
 
 namespace {
 
@@ -236,39 +236,8 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
-    if (split == 1) return;
-    // ---- the cluster adds up: each CTA some rows of x, the partial sums in the order of the k-blocks ----
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const float* sums = reinterpret_cast<const float*>(ring);
-    const int m0 = (first_tile / col_tiles) * BN, n0 = (first_tile % col_tiles) * BM, rows = min(BN, p.M - m0);
-    for (int i = threadIdx.x; i < ((rows + split - 1) / split) * (BM / 4); i += THREADS) {
-        const int m = (i / (BM / 4)) * split + rank, c = (i % (BM / 4)) * 4, n = n0 + c;
-        if (m >= rows || n >= p.N) continue;
-        float4 v[MAX_SPLIT];  // asked for together: each takes some 700 cycles
-#pragma unroll
-        for (int r = 0; r < MAX_SPLIT; ++r)
-            if (r < split) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + m * PITCH + c, r));
-        float y[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-#pragma unroll
-        for (int r = 1; r < MAX_SPLIT; ++r)
-            if (r < split) {
-                y[0] += v[r].x;
-                y[1] += v[r].y;
-                y[2] += v[r].z;
-                y[3] += v[r].w;
-            }
-        TO* out = reinterpret_cast<TO*>(p.out) + (size_t)(m0 + m) * p.ldo + n;
-        if (n + 4 <= p.N && ((uintptr_t)out & (4 * sizeof(TO) - 1)) == 0) {
-            store4(out, y);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.N) out[j] = from_float<TO>(y[j]);
-        }
-    }
-    // nobody leaves while its sums are read (which has been done: nothing has to be made visible)
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+    if (split > 1)
+        linear8::join_cluster<BN, THREADS, MAX_SPLIT, TO>(p, reinterpret_cast<const float*>(ring), split, rank, (first_tile / col_tiles) * BN, (first_tile % col_tiles) * BM);
 }
 
 template <int BN, int STAGES, int EPI_WARPS, typename TO>
@@ -286,21 +255,8 @@ int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t 
     const int sms = device_sms();
     int split = 1;  // doubled while all CTAs still run at once and none has fewer than four k-blocks
     while (split < MAX_SPLIT && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms));
-    cfg.blockDim = dim3((FIRST_EPI + EPI_WARPS) * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = split;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p, split, early, error_flag, xmap, wmap);
+    return linear8::launch_clusters(kernel, (unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms), (FIRST_EPI + EPI_WARPS) * 32, smem, split, stream, p, split, early, error_flag,
+                                    xmap, wmap);
 }
 
 }  // namespace

@@ -52,6 +52,23 @@ __device__ __forceinline__ void mma_e4m3_pair(unsigned d_tmem, unsigned long lon
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)accumulate) : "memory");
 }
+// ... of operands in blocks of 32 k, each with a power of two (its biased exponent, a byte).  A scale's place in tensor memory: row r's is
+// lane r % 32 of column r / 32 behind the address, in each of the four quarters of the lanes; the lowest byte of the column's four.
+__host__ __device__ constexpr unsigned idesc_e4m3_scaled(int M, int N) {
+    return ((unsigned)(N >> 3) << 17) | (1u << 23) | ((unsigned)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3_scaled(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc, unsigned a_scales, unsigned b_scales, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((unsigned)accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_e4m3_scaled_pair(unsigned d_tmem, unsigned long long a, unsigned long long b, unsigned idesc, unsigned a_scales, unsigned b_scales, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((unsigned)accumulate) : "memory");
+}
 // Arrives at this barrier of both CTAs once the pair's products issued so far have ended.
 __device__ __forceinline__ void commit_pair(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"

@@ -93,7 +93,7 @@ _SIGNATURES = {
     "llm_expert_act_scale": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "llm_branch_sum_norm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _f, _vp],
     "llm_quantize_blocks": [_vp, _i, _ll, _vp, _vp, _i, _i, _i, _vp],
-    "llm_linear8": [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp],
+    "llm_linear8": [_vp, _i, _ll, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "llm_expand_pages8": [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp],
     "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp],
@@ -2331,10 +2331,11 @@ def _here(*tensors) -> None:
 
 class Quantized:
     """A matrix ``[M, K]`` in 8 bits: ``values`` (float8_e4m3fn, contiguous) times a float32 scale for every block of ``rows`` (1 or 128)
-    rows and 128 columns, ``scales [ceil(M / rows), ceil(K / 128)]``.  A weight (``rows`` 128) may carry any positive scales, such as
-    a checkpoint's; :func:`quantize_blocks` makes powers of two."""
+    rows and 128 columns, ``scales [ceil(M / rows), ceil(K / 128)]``.  Scales may be any positive numbers, such as a checkpoint's.
+    ``powers_of_two`` says that they are powers of two from 2^-126 on, as :func:`quantize_blocks` makes them, which the tensor cores
+    take as they are: a product of many rows is faster with them."""
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int = 1):
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int = 1, powers_of_two: bool = False):
         shape = values.shape
         # (one test of everything: a call's own time is of the order of the smallest kernels')
         if not (rows in (1, _BLOCK8) and values.dtype == _E4M3 and len(shape) == 2 and values.is_contiguous() and scales.dtype == torch.float32
@@ -2343,7 +2344,7 @@ class Quantized:
             _need(values.dtype == _E4M3 and len(shape) == 2 and values.is_contiguous(), "Quantized: values are a contiguous float8_e4m3fn matrix")
             _need(scales.device == values.device, "Quantized: values and scales lie on one device")
             raise KernelError(f"Quantized: scales are contiguous float32 {[-(-shape[0] // rows), -(-shape[1] // _BLOCK8)]}")
-        self.values, self.scales, self.rows, self.shape = values, scales, rows, shape
+        self.values, self.scales, self.rows, self.shape, self.powers_of_two = values, scales, rows, shape, powers_of_two
 
     @property
     def device(self) -> torch.device:
@@ -2373,7 +2374,7 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Quantized:
     scales = x.new_empty((-(-m // rows), -(-k // _BLOCK8)), dtype=torch.float32)
     if m and k:
         _check8(_launch("llm_quantize_blocks", x.data_ptr(), code, x.stride(0), values.data_ptr(), scales.data_ptr(), m, k, rows, _stream()), "quantize_blocks")
-    return Quantized(values, scales, rows)
+    return Quantized(values, scales, rows, powers_of_two=True)
 
 
 def _check8(code: int, what: str) -> None:
@@ -2390,8 +2391,9 @@ def quantize_weight(w: torch.Tensor) -> Quantized:
 def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x [M, K] @ w [N, K]^T -> [M, N]`` in 8 bits: ``x`` is quantised row by row in blocks of 128 (:func:`quantize_blocks`; it may
     come as a :class:`Quantized` already), ``w`` has a scale for every block of 128 x 128.  Every block's products are summed on
-    the tensor cores and enter 32-bit sums times both scales: up to 64 rows through a kernel that streams the weights,
-    more on tcgen05.  ``K`` is a multiple of 16.  ``out_dtype``: float32 or bfloat16 (default: that of ``x``, bfloat16 for a quantised one)."""
+    the tensor cores and enter 32-bit sums times both scales; scales that are powers of two on both sides (those of
+    :func:`quantize_weight` are) the tensor cores may apply themselves, and sum over all blocks.  Few rows go to a kernel that
+    streams the weights, more to tcgen05.  ``K`` is a multiple of 16.  ``out_dtype``: float32 or bfloat16 (default: that of ``x``, bfloat16 for a quantised one)."""
     _need(isinstance(w, Quantized) and w.rows == _BLOCK8, "linear8: w is a Quantized matrix with a scale for every 128 rows")
     if isinstance(x, NormedInput):
         x = x.materialize()
@@ -2419,7 +2421,7 @@ def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tens
         xq = xt.new_empty((m * k + 4 * m * blocks,), dtype=torch.uint8)
     _need(w.values.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
     _check8(_launch("llm_linear8", xt.data_ptr(), x_code, 0 if given else xt.stride(0), x.scales.data_ptr() if given else None, None if given else xq.data_ptr(),
-                    w.values.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, m, n, k, n, _error_flag_ptr(), _stream()), "linear8")
+                    w.values.data_ptr(), w.scales.data_ptr(), w.powers_of_two and (not given or x.powers_of_two), out.data_ptr(), code, m, n, k, n, _error_flag_ptr(), _stream()), "linear8")
     if not given:
         add_launches(1)
     return out

@@ -121,6 +121,73 @@ def test_linear_of_many_tiles():
         check_product(ops().linear8(x, w, out_dtype=F32), x, w, f"{m} x {n} x {k}, 32-bit")
 
 
+def spread(m, k, rows, seed, most=8):
+    """Normal numbers, every block of ``rows`` by 128 times a power of two of its own."""
+    g = gen(seed)
+    e = torch.randint(-most, most + 1, (-(-m // rows), -(-k // 128)), generator=g, device=DEV).float()
+    return torch.randn(m, k, generator=g, device=DEV) * torch.exp2(e).repeat_interleave(rows, 0)[:m].repeat_interleave(128, 1)[:, :k]
+
+
+def check_scaled(got, x, w, what=""):
+    """Sums of 32 terms and over K / 32 of them, with truncation, and at most four partial sums: (32 + 4 blocks + 4) steps of 2^-23 of the
+    terms' sizes; then half a step of the output's type."""
+    want, size = plain.linear(x, w.values, w.scales)
+    steps = 32 + 4 * w.scales.shape[1] + 4
+    out = torch.finfo(got.dtype).eps / 2
+    off = (got.to(F64) - want).abs()
+    assert (off <= steps * 2.0**-23 * size * (1 + out) + out * want.abs()).all(), f"{what}: {(off / size.clamp(min=1e-30)).max():.3g} of the terms' sizes"
+
+
+@pytest.mark.parametrize("k", [16, 128, 144, 528, 1040, 2064])
+@pytest.mark.parametrize("n", [1, 16, 130, 400])
+def test_linear_with_powers_of_two(n, k):
+    w = ops().quantize_weight(spread(n, k, 128, n + k))
+    assert w.powers_of_two
+    x = spread(300, k, 1, k)
+    for m in (9, 17, 32, 33, 64, 65, 127, 128, 129, 300):
+        for out in (BF16, F32):
+            got = ops().linear8(x[:m], w, out_dtype=out)
+            assert got.dtype == out and tuple(got.shape) == (m, n)
+            check_scaled(got, x[:m], w, f"{m} rows, {out}")
+
+
+@pytest.mark.parametrize("m,n,k", [(1100, 2000, 272), (513, 9000, 400), (65, 20000, 144), (2049, 1500, 528), (300, 19000, 1040), (40, 24000, 656)])
+def test_linear_of_many_tiles_with_powers_of_two(m, n, k):
+    w = ops().quantize_weight(spread(n, k, 128, m))
+    x = spread(m, k, 1, n).to(BF16)
+    check_scaled(ops().linear8(x, w), x, w)
+    check_scaled(ops().linear8(x, w, out_dtype=F32), x, w, "32-bit")
+    q = ops().quantize_blocks(x)  # a caller's: its scales lie the other way round
+    assert q.powers_of_two and torch.equal(ops().linear8(q, w), ops().linear8(x, w))
+    # the same numbers without the promise, by the kernels for scales of any value
+    plainer = ops().Quantized(w.values, w.scales, 128)
+    check_product(ops().linear8(x, plainer), x, plainer)
+    check_product(ops().linear8(ops().Quantized(q.values, q.scales), w), x, w)
+
+
+@pytest.mark.parametrize("m,n", [(40, 200), (200, 200), (400, 9000)])
+def test_linear_where_powers_of_two_end(m, n):
+    """Scales at both ends of 32 bits' exponents whose products lie inside; blocks of zeros; NaN that stays in its row."""
+    k = 640
+    x, w = torch.randn(m, k, generator=gen(1), device=DEV), torch.randn(n, k, generator=gen(2), device=DEV)
+    x[:, :128] *= 2.0**-118
+    w[:, :128] *= 2.0**115
+    x[:, 128:256] *= 2.0**110
+    w[:, 128:256] *= 2.0**-113
+    x[:, 256:384] = 0
+    w[:, 384:512] = 0
+    wq = ops().quantize_weight(w)
+    want = ops().linear8(x, wq)
+    check_scaled(want, x, wq)
+    bad = x.clone()
+    bad[m // 2, 300] = torch.nan
+    bad[m - 1, 5] = torch.inf
+    got = ops().linear8(bad, wq)
+    spoilt = torch.zeros(m, dtype=torch.bool, device=DEV)
+    spoilt[[m // 2, m - 1]] = True
+    assert got[spoilt].isnan().all() and torch.equal(got[~spoilt], want[~spoilt])
+
+
 @pytest.mark.parametrize("m", [5, 40, 100])
 def test_linear_of_rows_in_other_forms(m):
     k, n = 400, 200
