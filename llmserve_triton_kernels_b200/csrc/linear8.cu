@@ -26,10 +26,13 @@ LLM_EXPORT int llm_linear8(const void* x, int x_dtype, long long ldx, const floa
     // had ended, whoever wrote the weights among them.
     if (M <= linear8::FEW_ROWS || (M <= 2 * linear8::FEW_ROWS && (long long)N * K <= linear8::FEW_BYTES)) return linear8::few(p, !given, stream);
     // The weights as the tall operand where x fills no tile of 128 rows by half, and where there are so few tiles that several CTAs may
-    // share one's k-blocks (which those kernels do).  Powers of two go to the kernels that leave them to the tensor cores (measured
-    // with x quantised in front, 4,096 k: 256 rows by 4,096 features 15.0 us against 16.6, 4,096 by 28,672 357 against 459), but not where
-    // tiles of 128 x 128 go round once, which pairs of CTAs on larger ones leave idle (512 by 4,096: 18.5 us against 20.3).
-    const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128), sms = device_sms();
+    // share one's k-blocks (which those kernels do).
+    const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128), pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), sms = device_sms();
     if (M <= 64 || tiles * 2 <= sms) return powers ? linear8::some_scaled(p, !given, error_flag, stream) : linear8::some(p, !given, error_flag, stream);
-    return powers && tiles > sms ? linear8::many_scaled(p, !given, error_flag, stream) : linear8::many(p, !given, error_flag, stream);
+    // Powers of two go to the pairs of CTAs that leave them to the tensor cores where tiles of 128 x 128 go round more than once (measured with
+    // x quantised in front: 4,096 rows by 28,672 features of 4,096 357 us against 459; 512 by 4,096, once round, 20.3 against 18.5), two pairs to
+    // a tile where clusters of four find room for all tiles (some SMs are left over) and have k-blocks to share (512 by 4,096 of
+    // 14,336 36.5 us against 51.9, 1,024 by 2,048 of 5,632 22.5 against 24.8; 512 by 2,560 of 2,048 13.6 against 12.0).
+    if (powers && pair_tiles * 4 <= sms * 7 / 8 && p.kblocks >= 32) return linear8::many_scaled(p, 2, !given, error_flag, stream);
+    return powers && tiles > sms ? linear8::many_scaled(p, 1, !given, error_flag, stream) : linear8::many(p, !given, error_flag, stream);
 }

@@ -26,7 +26,7 @@ int few(const Operands& p, bool early, cudaStream_t stream);
 int some(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
 // The same for scales that are powers of two, x's and the weights'.
 int some_scaled(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
-int many_scaled(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
+int many_scaled(const Operands& p, int split, bool early, int* error_flag, cudaStream_t stream);
 int many(const Operands& p, bool early, int* error_flag, cudaStream_t stream);
 
 }  // namespace linear8

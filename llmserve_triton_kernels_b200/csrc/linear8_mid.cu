@@ -231,13 +231,14 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-    __syncthreads();
+    if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
     if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
     }
     if (split > 1)
-        linear8::join_cluster<BN, THREADS, MAX_SPLIT, TO>(p, reinterpret_cast<const float*>(ring), split, rank, (first_tile / col_tiles) * BN, (first_tile % col_tiles) * BM);
+        linear8::join_cluster<BN, BM, THREADS, MAX_SPLIT, 2, TO>(p, reinterpret_cast<const float*>(ring), split, rank, 0, 1, (first_tile / col_tiles) * BN,
+                                                                 (first_tile % col_tiles) * BM);
 }
 
 template <int BN, int STAGES, int EPI_WARPS, typename TO>

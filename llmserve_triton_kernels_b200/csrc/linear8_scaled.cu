@@ -250,13 +250,14 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-    __syncthreads();
+    if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
     if (warp == ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(512) : "memory");
     }
     if (split > 1)
-        linear8::join_cluster<BN, THREADS, MAX_SPLIT, TO>(p, reinterpret_cast<const float*>(ring), split, rank, (first_tile / col_tiles) * BN, (first_tile % col_tiles) * BM);
+        linear8::join_cluster<BN, BM, THREADS, MAX_SPLIT, 2, TO>(p, reinterpret_cast<const float*>(ring), split, rank, 0, 1, (first_tile / col_tiles) * BN,
+                                                                 (first_tile % col_tiles) * BM);
 }
 
 template <int BN, int STAGES, typename TO>
@@ -279,15 +280,18 @@ int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t 
 
 // Many rows: a pair of CTAs (a cluster of two) on tiles of 256 rows of x by 256 of the weights.  Each CTA loads and keeps its 128 rows of x,
 // half the tile's weights and its 128 rows of the result; the first CTA issues the products for both.  The sums take half of tensor
-// memory and the scales the rest, so the next tile waits until the sums are in registers (some 300 cycles of a tile's 16,000).
+// memory and the scales the rest, so the next tile waits until the sums are in registers (some 300 cycles of a tile's 16,000).  Two pairs may
+// share a tile's k-blocks; four did not pay (clusters of eight CTAs do not find room at once).
 constexpr int PAIR_EPI_WARPS = 16, PAIR_THREADS = (FIRST_EPI + PAIR_EPI_WARPS) * 32;
 
 template <int STAGES, typename TO>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
-linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int* error_flag, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
     constexpr int BN = 256, A_BYTES = BM * BK, SLOT_BYTES = A_BYTES + BN / 2 * BK;  // of one CTA
     constexpr int COLS = BN / (PAIR_EPI_WARPS / 4);  // of an epilogue warp
     constexpr int KB_COLS = 16;                      // of a k-block's scales: 4 of the CTA's rows of x, 8 of the weights' rows, 4 unused
+    constexpr int PITCH = BN + 4;
+    static_assert((size_t)BM * PITCH * 4 <= (size_t)STAGES * SLOT_BYTES + PAIR_EPI_WARPS * linear8::PIECE_BYTES<TO>, "a split tile's sums lie where ring and staging were");
     static_assert(BN <= SCALES_AT && SCALES_AT + GROUPS * GROUP * KB_COLS <= 512, "tensor memory");
     constexpr unsigned IDESC = umma::idesc_e4m3_scaled(2 * BM, BN);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -298,8 +302,10 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
     __shared__ int gave_up;
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int kblocks = p.kblocks;
-    const int place = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    // `split` pairs (1 or 2, a cluster) share a tile's k-blocks; the pair's first CTA has rank `leader` in the cluster
+    const int place = blockIdx.x & 1, index = (blockIdx.x >> 1) % split, pair = (blockIdx.x >> 1) / split, pairs = (gridDim.x >> 1) / split;
+    const unsigned leader = 2 * index;
+    const int per = (p.kblocks + split - 1) / split, k_lo = min(p.kblocks, index * per), k_hi = min(p.kblocks, k_lo + per);
     const int row_tiles = (p.M + 2 * BM - 1) / (2 * BM), tiles = row_tiles * ((p.N + BN - 1) / BN);
 
     if (threadIdx.x == 0) {
@@ -338,11 +344,11 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
         // ---- producers ----
         int it = 0, s = 0, turn = 0;
         bool ok = true;
-        const int ahead = early ? min(STAGES, kblocks) : 0;  // slots whose weights are asked for while x is still made
+        const int ahead = early ? min(STAGES, k_hi - k_lo) : 0;  // slots whose weights are asked for while x is still made
         if (umma::elect_one()) {
             for (int i = warp; i < ahead; i += 2) {
                 if (place == 0) tma::mbar_expect_tx(&full[i], 2 * SLOT_BYTES);  // both CTAs' bytes
-                tma::load_2d_pair(ring + (size_t)i * SLOT_BYTES + A_BYTES, &wmap, i * BK, (pair / row_tiles) * BN + place * (BN / 2), &full[i]);
+                tma::load_2d_pair(ring + (size_t)i * SLOT_BYTES + A_BYTES, &wmap, (k_lo + i) * BK, (pair / row_tiles) * BN + place * (BN / 2), &full[i]);
             }
         }
         __syncwarp();
@@ -350,7 +356,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
         pdl_trigger();
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + place * (BN / 2);
-            for (int kb = 0; kb < kblocks; ++kb, ++it) {
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 if ((it & 1) == warp) {
                     if (it >= STAGES) ok = f.there(&empty[s], (turn - 1) & 1) && !f.failed();
                     if (!ok) break;
@@ -378,9 +384,9 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
             bool ok = true;
             for (int tile = pair; tile < tiles && ok; tile += pairs, ++round) {
                 if (round > 0) ok = f.there(&acc_empty, (round - 1) & 1);
-                for (int kb = 0; kb < kblocks && ok; ++kb) {
-                    const int j = kb % GROUP, g = group % GROUPS;
-                    const bool last = kb == kblocks - 1;
+                for (int kb = k_lo; kb < k_hi && ok; ++kb) {
+                    const int j = (kb - k_lo) % GROUP, g = group % GROUPS;
+                    const bool last = kb == k_hi - 1;
                     ok = (j != 0 || f.there(&scales_full[g], (group / GROUPS) & 1)) && f.there(&full[s], turn & 1) && !f.failed();
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -390,10 +396,10 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
                     if (umma::elect_one()) {
 #pragma unroll
                         for (int k = 0; k < BK / UMMA_K; ++k)  // 32 k = 32 bytes further along the rows: two 16-byte units
-                            umma::mma_e4m3_scaled_pair(tmem_base, a + 2 * k, b + 2 * k, IDESC, scales, scales + 4, kb != 0 || k != 0);
-                        umma::commit_pair(&empty[s]);
-                        if (j == GROUP - 1 || last) umma::commit_pair(&scales_empty[g]);
-                        if (last) umma::commit_pair(&acc_full);
+                            umma::mma_e4m3_scaled_pair(tmem_base, a + 2 * k, b + 2 * k, IDESC, scales, scales + 4, kb != k_lo || k != 0);
+                        umma::commit_pair(&empty[s], leader);
+                        if (j == GROUP - 1 || last) umma::commit_pair(&scales_empty[g], leader);
+                        if (last) umma::commit_pair(&acc_full, leader);
                     }
                     __syncwarp();
                     if (j == GROUP - 1 || last) ++group;
@@ -401,7 +407,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
                 }
             }
             if (!ok) {  // nor for the products
-                if (umma::elect_one()) umma::commit_pair(&drained);
+                if (umma::elect_one()) umma::commit_pair(&drained, leader);
                 (void)tma::mbar_wait(&drained, 0);
             }
         }
@@ -413,7 +419,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int block = (tile / row_tiles) * (BN / 128);
-            const float *sw0 = p.sw + (size_t)block * kblocks, *sw1 = p.sw + (size_t)min(block + 1, last_block) * kblocks;
+            const float *sw0 = p.sw + (size_t)block * p.kblocks, *sw1 = p.sw + (size_t)min(block + 1, last_block) * p.kblocks;
             const float* sx[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) sx[c] = p.sx + (size_t)min((tile % row_tiles) * 2 * BM + place * BM + 32 * c + lane, p.M - 1) * p.sx_row;
@@ -421,14 +427,14 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
             auto ask = [&](int k0) {
 #pragma unroll
                 for (int i = 0; i < GROUP; ++i) {
-                    const int k = min(k0 + i, kblocks - 1);
+                    const int k = min(k0 + i, p.kblocks - 1);
                     w[i][0] = sw0[k], w[i][1] = sw1[k];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) x[i][c] = sx[c][(size_t)k * p.sx_block];
                 }
             };
-            ask(0);
-            for (int k0 = 0; k0 < kblocks; k0 += GROUP, ++group) {
+            ask(k_lo);
+            for (int k0 = k_lo; k0 < k_hi; k0 += GROUP, ++group) {
                 const int g = group % GROUPS;
                 ok = !f.failed() && (group < GROUPS || f.there(&scales_empty[g], (group / GROUPS - 1) & 1));
                 ok = __all_sync(0xffffffffu, ok);
@@ -450,8 +456,8 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tma::mbar_arrive_at(&scales_full[g], 0);
-                if (k0 + GROUP < kblocks) ask(k0 + GROUP);
+                if (lane == 0) tma::mbar_arrive_at(&scales_full[g], leader);
+                if (k0 + GROUP < k_hi) ask(k0 + GROUP);
             }
         }
     } else if (warp >= FIRST_EPI) {
@@ -469,7 +475,15 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
             for (int c = 0; c < COLS / 32; ++c) umma::tmem_have32(v[c]);
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) tma::mbar_arrive_at(&acc_empty, 0);
+            if (lane == 0) tma::mbar_arrive_at(&acc_empty, leader);
+            if (split > 1) {
+                // The ring's slots have all been read by the products (they were waited for); its memory takes the sums.
+                float* sums = reinterpret_cast<float*>(ring) + (quarter * 32 + lane) * PITCH + part * COLS;
+#pragma unroll
+                for (int j = 0; j < COLS; j += 4)
+                    *reinterpret_cast<uint4*>(sums + j) = make_uint4(v[j / 32][j % 32], v[j / 32][j % 32 + 1], v[j / 32][j % 32 + 2], v[j / 32][j % 32 + 3]);
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < COLS / 32; ++c) {
                 unsigned long long sums[16];
@@ -485,10 +499,13 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int early, int* error_flag
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(512) : "memory");
     }
+    if (split > 1)
+        linear8::join_cluster<BM, BN, PAIR_THREADS, 2, 3, TO>(p, reinterpret_cast<const float*>(ring), split, index, place, 2, (pair % row_tiles) * 2 * BM + place * BM,
+                                                                      (pair / row_tiles) * BN);
 }
 
 template <typename TO>
-int launch_pair(const linear8::Operands& p, int early, int* error_flag, cudaStream_t stream) {
+int launch_pair(const linear8::Operands& p, int split, int early, int* error_flag, cudaStream_t stream) {
     constexpr int STAGES = sizeof(TO) == 4 ? 4 : 5;
     constexpr size_t smem = (size_t)STAGES * 2 * BM * BK + 1024 + PAIR_EPI_WARPS * linear8::PIECE_BYTES<TO>;
     auto kernel = linear8_scaled_pair_kernel<STAGES, TO>;
@@ -501,7 +518,8 @@ int launch_pair(const linear8::Operands& p, int early, int* error_flag, cudaStre
     const long long tiles = (long long)((p.N + 255) / 256) * ((p.M + 255) / 256);
     if (tiles > 0x3fffffffLL) return LLM_ERR_UNSUPPORTED;
     const int pairs = device_sms() / 2;
-    return linear8::launch_clusters(kernel, (unsigned)(tiles < pairs ? tiles : pairs) * 2, PAIR_THREADS, smem, 2, stream, p, early, error_flag, xmap, wmap);
+    return linear8::launch_clusters(kernel, (unsigned)(split > 1 ? tiles * split : tiles < pairs ? tiles : pairs) * 2, PAIR_THREADS, smem, 2 * split, stream, p, split, early,
+                                    error_flag, xmap, wmap);
 }
 
 }  // namespace
@@ -511,6 +529,6 @@ int linear8::some_scaled(const Operands& p, bool early, int* error_flag, cudaStr
     return p.M <= 64 ? launch<64, 7, __nv_bfloat16>(p, early, error_flag, stream) : launch<128, 6, __nv_bfloat16>(p, early, error_flag, stream);
 }
 
-int linear8::many_scaled(const Operands& p, bool early, int* error_flag, cudaStream_t stream) {
-    return p.out_dtype == LLM_F32 ? launch_pair<float>(p, early, error_flag, stream) : launch_pair<__nv_bfloat16>(p, early, error_flag, stream);
+int linear8::many_scaled(const Operands& p, int split, bool early, int* error_flag, cudaStream_t stream) {
+    return p.out_dtype == LLM_F32 ? launch_pair<float>(p, split, early, error_flag, stream) : launch_pair<__nv_bfloat16>(p, split, early, error_flag, stream);
 }

@@ -52,37 +52,44 @@ __device__ __forceinline__ void store_piece(const Operands& p, unsigned char* pi
     __syncwarp();  // the piece is written again
 }
 
-// The CTAs of a cluster have summed some of a tile's k-blocks each, [BN rows of x][128 rows of w + 4] floats in shared memory: each adds up
-// some rows of x, the partial sums in the order of the k-blocks.
-template <int BN, int THREADS, int MAX_SPLIT, typename TO>
-__device__ __forceinline__ void join_cluster(const Operands& p, const float* sums, int split, int rank, int m0, int n0) {
-    constexpr int BM = 128, PITCH = BM + 4;
+// Some CTAs of a cluster have summed some of a tile's k-blocks each, [ROWS rows of x][WIDTH rows of w + 4] floats in shared memory: `split`
+// of them, from rank `first` on every `step`-th, of which this is number `index`.  Each adds up some rows of x, the partial sums in
+// the order of the k-blocks (the cluster has met since they were written); a thread asks for BATCH times four sums of every CTA at once, which take some 700 cycles.
+template <int ROWS, int WIDTH, int THREADS, int MAX_SPLIT, int BATCH, typename TO>
+__device__ __forceinline__ void join_cluster(const Operands& p, const float* sums, int split, int index, int first, int step, int m0, int n0) {
+    constexpr int PITCH = WIDTH + 4, PARTS = WIDTH / 4;
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-    cluster.sync();
-    const int rows = min(BN, p.M - m0);
-    for (int i = threadIdx.x; i < ((rows + split - 1) / split) * (BM / 4); i += THREADS) {
-        const int m = (i / (BM / 4)) * split + rank, c = (i % (BM / 4)) * 4, n = n0 + c;
-        if (m >= rows || n >= p.N) continue;
-        float4 v[MAX_SPLIT];  // asked for together: each takes some 700 cycles
+    const int rows = min(ROWS, p.M - m0), total = ((rows - index + split - 1) / split) * PARTS;  // this CTA's: rows index, index + split, ..
+    for (int i0 = threadIdx.x; i0 < total; i0 += THREADS * BATCH) {
+        float4 v[BATCH][MAX_SPLIT];
 #pragma unroll
-        for (int r = 0; r < MAX_SPLIT; ++r)
-            if (r < split) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + m * PITCH + c, r));
-        float y[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = min(i0 + b * THREADS, total - 1), m = (i / PARTS) * split + index, c = (i % PARTS) * 4;
 #pragma unroll
-        for (int r = 1; r < MAX_SPLIT; ++r)
-            if (r < split) {
-                y[0] += v[r].x;
-                y[1] += v[r].y;
-                y[2] += v[r].z;
-                y[3] += v[r].w;
+            for (int r = 0; r < MAX_SPLIT; ++r)
+                if (r < split) v[b][r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(sums + m * PITCH + c, first + step * r));
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = i0 + b * THREADS, m = (i / PARTS) * split + index, n = n0 + (i % PARTS) * 4;
+            if (i >= total || n >= p.N) continue;
+            float y[4] = {v[b][0].x, v[b][0].y, v[b][0].z, v[b][0].w};
+#pragma unroll
+            for (int r = 1; r < MAX_SPLIT; ++r)
+                if (r < split) {
+                    y[0] += v[b][r].x;
+                    y[1] += v[b][r].y;
+                    y[2] += v[b][r].z;
+                    y[3] += v[b][r].w;
+                }
+            TO* out = reinterpret_cast<TO*>(p.out) + (size_t)(m0 + m) * p.ldo + n;
+            if (n + 4 <= p.N && ((uintptr_t)out & (4 * sizeof(TO) - 1)) == 0) {
+                store4(out, y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < p.N) out[j] = from_float<TO>(y[j]);
             }
-        TO* out = reinterpret_cast<TO*>(p.out) + (size_t)(m0 + m) * p.ldo + n;
-        if (n + 4 <= p.N && ((uintptr_t)out & (4 * sizeof(TO) - 1)) == 0) {
-            store4(out, y);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.N) out[j] = from_float<TO>(y[j]);
         }
     }
     // nobody leaves while its sums are read (which has been done: nothing has to be made visible)

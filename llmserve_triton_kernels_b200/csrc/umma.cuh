@@ -69,10 +69,10 @@ __device__ __forceinline__ void mma_e4m3_scaled_pair(unsigned d_tmem, unsigned l
         "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((unsigned)accumulate) : "memory");
 }
-// Arrives at this barrier of both CTAs once the pair's products issued so far have ended.
-__device__ __forceinline__ void commit_pair(unsigned long long* bar) {
+// Arrives at this barrier of both CTAs once the pair's products issued so far have ended; `leader` is the first CTA's rank in its cluster.
+__device__ __forceinline__ void commit_pair(unsigned long long* bar, unsigned leader = 0) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
-                 ::"r"(tma::smem_addr(bar)), "h"((unsigned short)3) : "memory");
+                 ::"r"(tma::smem_addr(bar)), "h"((unsigned short)(3u << leader)) : "memory");
 }
 // The same product with the A operand in tensor memory: row m of A in lane m, its k values along the columns from
 // a_tmem on, two 16-bit values to a 32-bit column (the lower k in the lower half).

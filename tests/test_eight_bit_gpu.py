@@ -151,7 +151,7 @@ def test_linear_with_powers_of_two(n, k):
             check_scaled(got, x[:m], w, f"{m} rows, {out}")
 
 
-@pytest.mark.parametrize("m,n,k", [(1100, 2000, 272), (513, 9000, 400), (65, 20000, 144), (2049, 1500, 528), (300, 19000, 1040), (40, 24000, 656)])
+@pytest.mark.parametrize("m,n,k", [(1100, 2000, 272), (513, 9000, 400), (65, 20000, 144), (2049, 1500, 528), (300, 19000, 1040), (40, 24000, 656), (900, 1100, 4112), (513, 2304, 6000), (257, 4097, 4096)])
 def test_linear_of_many_tiles_with_powers_of_two(m, n, k):
     w = ops().quantize_weight(spread(n, k, 128, m))
     x = spread(m, k, 1, n).to(BF16)
