@@ -28,8 +28,10 @@
 // Cutting and joining cost 8 us and more, so short or many units of work go without: a CTA takes a tile of rows with all its keys, of two
 // warps instead of eight where there are many units of few keys, whose time is a CTA's 4 us of loads that wait for one another (q and
 // the page table, the pages, the warps' meeting) and not the bytes.  The host picks, from the longest context it is told.
-// Heads of 128 lanes, 32 over 8, requests of random lengths: 32 of up to 16,000 keys 137 us, 5.0 TB/s of pages; 64 of up to 4,000 93 us, 3.7
-// TB/s; 8 of up to 4,000 23 us, of which 10 are laying out, cutting and joining.
+// Heads of 128 lanes, 32 over 8, requests of random lengths: 32 of up to 8,191 keys 73 us, 4.8 TB/s of pages; 64 of up to 4,000 78 us, 4.4
+// TB/s; 8 of up to 4,000 20 us, of which 8 are laying out, cutting and joining.  It is not the memory that bounds the first (with all pages
+// in the L2 it took 5 % less) but the warps' own chains: 440 instructions a tile of 16 keys, issued in 59 % of the cycles with the
+// 4 warps that an SM's quarter has registers for.
 //
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
 // Where rows differ in what they see, NaN among the values is counted apart, so that it reaches the rows that see it alone.
@@ -39,6 +41,9 @@
 namespace {
 
 constexpr int TILE = 16, STAGES = 3;
+// What it costs a CTA to begin and end a segment, in tiles (q, the first copies, the warps' meeting: some 5,000 cycles): a unit counts for so
+// many tiles more than it has.  32 requests of up to 8,191 keys: 83 us with 0, 81 with 6, 79 with 12, 77 with 20, less with 28 than with 40.
+constexpr int UNIT_COST = 28;
 constexpr int JOIN_THREADS = 512;
 constexpr int MAX_REQUESTS = 1024;  // of a step whose work is counted tile by tile
 
@@ -151,7 +156,7 @@ template <int ROWS>
 __device__ __forceinline__ void lay_out(const Attn8Params& p, long long* begins) {
     for (int r = threadIdx.x; r < p.requests; r += blockDim.x) {
         const Share s = share_of<ROWS>(p, r);
-        begins[r + 1] = (long long)p.KV * s.row_tiles * s.tiles;
+        begins[r + 1] = s.tiles ? (long long)p.KV * s.row_tiles * (UNIT_COST + s.tiles) : 0;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -224,14 +229,16 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
             r = lo;
             const Share s = share_of<ROWS>(p, r);
             const long long within = at - begins[r];
-            const int unit = (int)(within / s.tiles), off = (int)(within - (long long)unit * s.tiles);
-            const int take = (int)min((long long)(s.tiles - off), end - at);
+            // a unit is UNIT_COST places without tiles, then its tiles
+            const int places = UNIT_COST + s.tiles, unit = (int)(within / places), off = (int)(within - (long long)unit * places);
+            const int to = (int)min((long long)places, off + end - at), skip = max(0, off - UNIT_COST), take = to - UNIT_COST - skip;
+            at += to - off;
+            if (take <= 0) continue;
             h = unit / s.row_tiles;
             row0 = (unit - h * s.row_tiles) * ROWS;
-            tile_lo = s.first_tile + off;
+            tile_lo = s.first_tile + skip;
             tile_hi = tile_lo + take;
-            if (take < s.tiles) part = blockIdx.x * 2 + (off == 0);
-            at += take;
+            if (take < s.tiles) part = blockIdx.x * 2 + (skip == 0);
         } else {
             r = blockIdx.x / p.KV;
             h = blockIdx.x - r * p.KV;
@@ -396,33 +403,25 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
             const unsigned char* stage = ring + slot * S::BYTES;
 
             // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
-            // (four sums of products each, so that none waits for another for long)
+            // (one sum: four, so that no product waits for another, need registers that the SM's other warps then lack: 2 us of 75)
             float s[NT][4];
-            {
-                float c[NT][4][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) c[nt][k][e] = 0.f;
+            for (int x = 0; x < D / 64; ++x) {
+                const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
+                const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
+                const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
-                for (int x = 0; x < D / 64; ++x) {
-                    const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
-                    const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
-                    const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_e4m3(c[nt][0], a0, qb[nt][2 * x][0][0], qb[nt][2 * x][0][1]);
-                        mma_e4m3(c[nt][1], a0, qb[nt][2 * x][1][0], qb[nt][2 * x][1][1]);
-                        mma_e4m3(c[nt][2], a1, qb[nt][2 * x + 1][0][0], qb[nt][2 * x + 1][0][1]);
-                        mma_e4m3(c[nt][3], a1, qb[nt][2 * x + 1][1][0], qb[nt][2 * x + 1][1][1]);
-                    }
-                }
+                    for (int nt = 0; nt < NT; ++nt) mma_e4m3(s[nt], a0, qb[nt][2 * x][part][0], qb[nt][2 * x][part][1]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nt][e] = (c[nt][0][e] + c[nt][2][e]) + (c[nt][1][e] + c[nt][3][e]);
+                    for (int nt = 0; nt < NT; ++nt) mma_e4m3(s[nt], a1, qb[nt][2 * x + 1][part][0], qb[nt][2 * x + 1][part][1]);
             }
             unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
@@ -637,7 +636,7 @@ attention8_join_kernel(const Attn8Params p) {
     const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = p.below && n >= p.below ? 0 : n * p.G, live_rows = min(ROWS, rows - row0);
     const Share share = share_of<ROWS>(p, r);
     lay_out<ROWS>(p, begins);
-    const long long total = begins[p.requests], from = begins[r] + (long long)(h * share.row_tiles + blockIdx.y) * share.tiles;
+    const long long total = begins[p.requests], from = begins[r] + (long long)(h * share.row_tiles + blockIdx.y) * (UNIT_COST + share.tiles) + UNIT_COST;
     int c0 = 0, c1 = -1;  // the stretches that hold a tile of these rows
     if (live_rows > 0 && share.tiles) {
         const int count = stretches(p, total);

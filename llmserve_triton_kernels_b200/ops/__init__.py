@@ -2551,12 +2551,13 @@ def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_d
 
     A unit is a tile of 8 or 16 rows of a request and a key head, with at most ``keys`` keys.  Without stretches (0) a CTA takes a unit; with
     them the keys of all units are dealt out evenly and a second kernel joins what was cut.  Measured on 148 SMs with heads of 128 lanes
-    (64 lanes: two thirds of what goes by keys), CTAs of 8 warps, requests of random lengths up to k thousands of keys, u units an SM: a CTA by itself takes 4 + 8 k us
-    and an SM 2 + 6 k us a unit, against 12 + u (6 + 5 k) us for stretches.  64 units of 4,000 keys: 36.5 us, in stretches 23.2; 256 of 8,191:
-    106 and 83; 256 of 1,000: 18.3 and 27.9; 1,024 of 2,000: 84 and 109.  Stretches are as many as CTAs find room at once, or half of them
-    where there is little for each, which leaves less to join: 8 units of 8,000 keys 17.4 us instead of 22.8, 64 of 4,000 28.3
-    instead of 23.2.  Many short units are better off with CTAs of 2 warps, of which there is room for four times as many: 1,824 units of
-    20 keys take 13.3 us instead of 32.7, of 250 keys 29 instead of 44; 256 units of 1,000 30 instead of 18."""
+    (64 lanes: two thirds of what goes by keys), CTAs of 8 warps, requests of random lengths up to k thousands of keys, u units an SM: a
+    CTA takes 4 + 8 k us and all (u + 1) (2 + 4.2 k) us, in stretches 10 + u (2.5 + 4.4 k) us.  64 units of 4,000 keys: 36.5 us, in
+    stretches 20.0; 256 of 8,191: 104 and 73; 256 of 1,000: 17.8 and 20.9; 1,024 of 2,000: 80 and 87.  Stretches are as many as CTAs find
+    room at once, or half of them where there is little for each and few units, which leaves less to join: 8 units of 16,000 keys 19.1 us
+    instead of 21.8, 64 of 2,000 18.6 instead of 15.3, 64 of 4,000 25.9 instead of 20.0.  Many short units are better off with CTAs of 2 warps, of
+    which there is room for four times as many: 1,824 units of 20 keys take 13.3 us instead of 32.7, of 250 keys 29 instead of 44; 256
+    units of 1,000 30 instead of 18."""
     if _ATTENTION8_SPLIT is not None:
         return _ATTENTION8_SPLIT
     height = 8 if rows <= 8 else 16
@@ -2566,6 +2567,6 @@ def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_d
     if keys <= 256 or requests > 1024:  # (the list of requests' shares is held in shared memory)
         return 8, 0
     k = keys * (head_dim + 64) / 192e3
-    if max(4 + 8 * k, -(-units // sms) * (2 + 6 * k)) <= 12 + units / sms * (6 + 5 * k):
+    if max(4 + 8 * k, (units / sms + 1) * (2 + 4.2 * k)) <= 10 + units / sms * (2.5 + 4.4 * k):
         return 8, 0
-    return 8, sms * (2 if height == 8 and units * keys >= 1700 * sms else 1)
+    return 8, sms * (2 if height == 8 and (units * keys >= 1700 * sms or units * 3 >= sms) else 1)
