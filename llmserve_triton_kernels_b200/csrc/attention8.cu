@@ -44,6 +44,8 @@ constexpr int TILE = 16, STAGES = 3;
 // What it costs a CTA to begin and end a segment, in tiles (q, the first copies, the warps' meeting: some 5,000 cycles): a unit counts for so
 // many tiles more than it has.  32 requests of up to 8,191 keys: 83 us with 0, 81 with 6, 79 with 12, 77 with 20, less with 28 than with 40.
 constexpr int UNIT_COST = 28;
+// Tiles of keys up to which a CTA takes a unit whole (8 requests of 500 keys, 8 key heads: 10.7 us instead of 12.3; of 100: 7.7 instead of 10).
+constexpr int WHOLE = 32;
 constexpr int JOIN_THREADS = 512;
 constexpr int MAX_REQUESTS = 1024;  // of a step whose work is counted tile by tile
 
@@ -151,12 +153,17 @@ __device__ __forceinline__ Share share_of(const Attn8Params& p, int r) {
     return s;
 }
 
-// Where the requests' shares begin in the list, [requests + 1], by the whole block.
+// Where the requests' shares begin in the list, [requests + 1], by the whole block.  Returns whether units are cut: a captured step is laid
+// out for the longest context there may be, and where no request holds more than WHOLE tiles of keys by now, a unit counts as one place,
+// which some CTA takes with all its keys.
 template <int ROWS>
-__device__ __forceinline__ void lay_out(const Attn8Params& p, long long* begins) {
+__device__ __forceinline__ bool lay_out(const Attn8Params& p, long long* begins) {
+    int most = 0;
+    for (int r = threadIdx.x; r < p.requests; r += blockDim.x) most = max(most, share_of<ROWS>(p, r).tiles);
+    const bool cut = __syncthreads_or(most > WHOLE);
     for (int r = threadIdx.x; r < p.requests; r += blockDim.x) {
         const Share s = share_of<ROWS>(p, r);
-        begins[r + 1] = s.tiles ? (long long)p.KV * s.row_tiles * (UNIT_COST + s.tiles) : 0;
+        begins[r + 1] = s.tiles ? (long long)p.KV * s.row_tiles * (cut ? UNIT_COST + s.tiles : 1) : 0;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -175,11 +182,12 @@ __device__ __forceinline__ void lay_out(const Attn8Params& p, long long* begins)
         if (threadIdx.x == 0) begins[0] = 0;
     }
     __syncthreads();
+    return cut;
 }
 
-// Stretches of a list of `total` tiles: no more than there are CTAs, none (but the last) shorter than a tile a warp.
-__device__ __forceinline__ int stretches(const Attn8Params& p, long long total) {
-    return (int)max(1LL, min((long long)p.ranges, total / p.warps));
+// Stretches of a list of `total` places: no more than there are CTAs, none (but the last) shorter than a tile a warp, or than a unit.
+__device__ __forceinline__ int stretches(const Attn8Params& p, long long total, bool cut) {
+    return (int)max(1LL, min((long long)p.ranges, cut ? total / p.warps : total));
 }
 
 // RUN: pages hold whole runs of 8 or 16 keys; 0: they do not, and the threads copy every key from its own place.
@@ -209,10 +217,11 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
     pdl_wait();
     pdl_trigger();
     long long at = 0, end = 1;
+    bool cut = false;
     if (p.ranges) {
-        lay_out<ROWS>(p, begins);
+        cut = lay_out<ROWS>(p, begins);
         const long long total = begins[p.requests];
-        const int count = stretches(p, total);
+        const int count = stretches(p, total, cut);
         if ((int)blockIdx.x >= count) return;
         at = total * blockIdx.x / count;
         end = total * (blockIdx.x + 1) / count;
@@ -229,9 +238,9 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
             r = lo;
             const Share s = share_of<ROWS>(p, r);
             const long long within = at - begins[r];
-            // a unit is UNIT_COST places without tiles, then its tiles
-            const int places = UNIT_COST + s.tiles, unit = (int)(within / places), off = (int)(within - (long long)unit * places);
-            const int to = (int)min((long long)places, off + end - at), skip = max(0, off - UNIT_COST), take = to - UNIT_COST - skip;
+            // a unit is UNIT_COST places without tiles, then its tiles; or one place
+            const int before = cut ? UNIT_COST : 1 - s.tiles, places = before + s.tiles, unit = (int)(within / places), off = (int)(within - (long long)unit * places);
+            const int to = (int)min((long long)places, off + end - at), skip = max(0, off - (cut ? UNIT_COST : 0)), take = to - before - skip;
             at += to - off;
             if (take <= 0) continue;
             h = unit / s.row_tiles;
@@ -635,11 +644,11 @@ attention8_join_kernel(const Attn8Params p) {
     // out while that one runs.
     const int first = p.cu_tokens[r], n = p.cu_tokens[r + 1] - first, rows = p.below && n >= p.below ? 0 : n * p.G, live_rows = min(ROWS, rows - row0);
     const Share share = share_of<ROWS>(p, r);
-    lay_out<ROWS>(p, begins);
+    const bool cut = lay_out<ROWS>(p, begins);
     const long long total = begins[p.requests], from = begins[r] + (long long)(h * share.row_tiles + blockIdx.y) * (UNIT_COST + share.tiles) + UNIT_COST;
     int c0 = 0, c1 = -1;  // the stretches that hold a tile of these rows
-    if (live_rows > 0 && share.tiles) {
-        const int count = stretches(p, total);
+    if (live_rows > 0 && share.tiles && cut) {
+        const int count = stretches(p, total, cut);
         c0 = (int)(from * count / total);
         while (total * (c0 + 1) / count <= from) ++c0;
         c1 = c0;
@@ -647,7 +656,7 @@ attention8_join_kernel(const Attn8Params p) {
     }
     pdl_wait();
     pdl_trigger();
-    if (live_rows <= 0 || (share.tiles && c0 == c1)) return;
+    if (live_rows <= 0 || (share.tiles && (!cut || c0 == c1))) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto place = [&](int k, int row) { return (size_t)(2 * k + (k == c0)) * ROWS + row; };
     for (int row = warp; row < live_rows; row += JOIN_THREADS / 32) {

@@ -54,7 +54,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
     unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ unsigned tmem_base;
-    __shared__ int gave_up;
+    __shared__ int gave_up, asked[2];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int kblocks = p.kblocks;
@@ -197,9 +197,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
-            if (!ok)  // nobody waits for the copies on their way any more
-                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
-                    if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+            if (lane == 0) asked[which] = it;
         } else {
             // ---- tensor-core issuers ----
             int it = 0, s = 0, turn = 0;
@@ -234,6 +232,10 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
+    if (warp < FIRST_ISSUER && failed()) {  // nobody waits for the copies on their way any more
+        for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
+            if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    }
     if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
@@ -255,7 +257,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
     unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [EPI_WARPS] pieces of the result
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ unsigned tmem_base;
-    __shared__ int gave_up;
+    __shared__ int gave_up, asked[2];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int kblocks = p.kblocks;
@@ -294,6 +296,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
 
     auto fail = [&]() {
         *(volatile int*)&gave_up = 1;
+        *(volatile int*)cg::this_cluster().map_shared_rank(&gave_up, place ^ 1) = 1;
         if (error_flag) atomicExch(error_flag, 1);
     };
     auto failed = [&]() { return *(volatile int*)&gave_up != 0; };
@@ -399,10 +402,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
                     if (++s == STAGES) s = 0, ++turn;
                 }
             }
-            // nobody waits for the copies on their way any more (they are counted at the first CTA, which outlives them: the CTAs leave together)
-            if (!ok && place == 0)
-                for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
-                    if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+            if (lane == 0) asked[which] = it;
         } else if (place == 0) {
             // ---- tensor-core issuers, for both CTAs ----
             int it = 0, s = 0, turn = 0;
@@ -437,6 +437,13 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
+    if (failed()) {  // (both CTAs know.)  Nobody waits for the copies on their way any more; they are counted at the first CTA, and the other's memory takes some
+        if (place == 0 && warp < FIRST_ISSUER) {
+            for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
+                if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        }
+        cg::this_cluster().sync();
+    }
     if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");

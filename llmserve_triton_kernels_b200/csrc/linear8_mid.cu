@@ -32,7 +32,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained[2];
     __shared__ __align__(16) float scales[EPI_WARPS][2][COLS];
     __shared__ unsigned tmem_base;
-    __shared__ int gave_up;
+    __shared__ int gave_up, asked[2];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % split, first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
@@ -113,9 +113,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
                 if (++s == STAGES) s = 0, ++turn;
             }
         }
-        if (!ok)  // nobody waits for the copies on their way any more
-            for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
-                if ((i & 1) == which) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        if (lane == 0) asked[which] = it;
     } else if (warp < FIRST_EPI) {
         // ---- tensor-core issuers ----
         int it = 0, s = 0, turn = 0;
@@ -232,6 +230,10 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
+    if (warp < FIRST_ISSUER && failed()) {  // nobody waits for the copies on their way any more
+        for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
+            if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    }
     if (warp == FIRST_ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");

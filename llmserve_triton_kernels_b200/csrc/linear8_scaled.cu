@@ -41,9 +41,11 @@ __device__ __forceinline__ unsigned exponents_of(float scale) { return (__float_
 // What the roles of both kernels share.
 struct Failing {
     int* gave_up;
+    int ctas;  // of the cluster, all of which are told; 0: this one alone
     int* error_flag;
     __device__ __forceinline__ void fail() const {
         *(volatile int*)gave_up = 1;
+        for (int r = 0; r < ctas; ++r) *(volatile int*)cg::this_cluster().map_shared_rank(gave_up, r) = 1;
         if (error_flag) atomicExch(error_flag, 1);
     }
     __device__ __forceinline__ bool failed() const { return *(volatile int*)gave_up != 0; }
@@ -68,7 +70,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], scales_full[GROUPS], scales_empty[GROUPS], drained;
     __shared__ unsigned tmem_base;
-    __shared__ int gave_up;
+    __shared__ int gave_up, asked[2];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % split, first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
@@ -108,7 +110,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         pdl_wait();
         pdl_trigger();
     }
-    const Failing f = {&gave_up, error_flag};
+    const Failing f = {&gave_up, 0, error_flag};
 
     if (warp < ISSUER) {
         // ---- producers ----
@@ -142,9 +144,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
                 if (++s == STAGES) s = 0, ++turn;
             }
         }
-        if (!ok)  // nobody waits for the copies on their way any more
-            for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
-                if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        if (lane == 0) asked[warp] = it;
     } else if (warp == ISSUER) {
         // ---- tensor-core issuer ----
         int s = 0, turn = 0, group = 0, round = 0;
@@ -251,6 +251,10 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
+    if (warp < ISSUER && f.failed()) {  // nobody waits for the copies on their way any more
+        for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
+            if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    }
     if (warp == ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(512) : "memory");
@@ -299,7 +303,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     unsigned char* staging = ring + (size_t)STAGES * SLOT_BYTES;  // [PAIR_EPI_WARPS] pieces of the result
     __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full, acc_empty, scales_full[GROUPS], scales_empty[GROUPS], drained;
     __shared__ unsigned tmem_base;
-    __shared__ int gave_up;
+    __shared__ int gave_up, asked[2];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     // `split` pairs (1 or 2, a cluster) share a tile's k-blocks; the pair's first CTA has rank `leader` in the cluster
@@ -338,7 +342,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
         pdl_wait();
         pdl_trigger();
     }
-    const Failing f = {&gave_up, error_flag};
+    const Failing f = {&gave_up, 2 * split, error_flag};
 
     if (warp < ISSUER) {
         // ---- producers ----
@@ -373,10 +377,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
                 if (++s == STAGES) s = 0, ++turn;
             }
         }
-        // nobody waits for the copies on their way any more (they are counted at the first CTA, which outlives them: the CTAs leave together)
-        if (!ok && place == 0)
-            for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i)
-                if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        if (lane == 0) asked[warp] = it;
     } else if (warp == ISSUER) {
         // ---- tensor-core issuer, for both CTAs ----
         if (place == 0) {
@@ -495,6 +496,13 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
+    if (f.failed()) {  // (the whole cluster knows.)  Nobody waits for the copies on their way any more; they are counted at the first CTA, and the other's memory takes some
+        if (place == 0 && warp < ISSUER) {
+            for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
+                if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+        }
+        cg::this_cluster().sync();
+    }
     if (warp == ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "n"(512) : "memory");

@@ -2384,7 +2384,8 @@ def _check8(code: int, what: str) -> None:
 
 def quantize_weight(w: torch.Tensor) -> Quantized:
     """A product's matrix ``[N, K]`` as :func:`linear8` takes it: a scale for every block of 128 x 128."""
-    _need(w.dim() == 2 and w.shape[1] >= 16 and w.shape[1] % 16 == 0, f"quantize_weight: a matrix with rows of a multiple of 16 values, not {list(w.shape)}")
+    _need(isinstance(w, torch.Tensor) and w.dim() == 2 and w.shape[1] >= 16 and w.shape[1] % 16 == 0,
+          f"quantize_weight: a matrix with rows of a multiple of 16 values, not {list(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__}")
     return quantize_blocks(w, rows=_BLOCK8)
 
 

@@ -391,8 +391,9 @@ def test_attention_of_prompt_portions(H, KV, D, page_size, counts, held, window)
 
 @pytest.mark.parametrize("split", [(2, 0), (8, 0), (8, 1), (8, 5), (8, 148), (2, 9)], ids=str)
 @pytest.mark.parametrize("H,KV,D,page_size", [(8, 2, 64, 16), (40, 4, 64, 8), (16, 2, 128, 24), (20, 1, 128, 16), (4, 4, 128, 5)])
-def test_attention_however_it_is_shared_out(monkeypatch, H, KV, D, page_size, split):
-    counts, held = [1, 1, 7, 0, 1, 30], [1, 900, 130, 40, 0, 600]
+@pytest.mark.parametrize("longest", [900, 512])  # 513 keys and more of some request: stretches cut; fewer: they hold whole units
+def test_attention_however_it_is_shared_out(monkeypatch, H, KV, D, page_size, split, longest):
+    counts, held = [1, 1, 7, 0, 1, 30], [1, longest, 130, 40, 0, min(600, longest)]
     monkeypatch.setattr(ops(), "_ATTENTION8_SPLIT", split)
     ctx, table, _, pages = a_step(counts, held, page_size, 5)
     pool, exps = pages8(pages, KV, page_size, D, 12)
