@@ -2370,11 +2370,13 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Quantized:
     code = _code(x.dtype)
     _here(x)
     m, k = shape
-    values = x.new_empty(shape, dtype=_E4M3)
+    values = x.new_empty((m, k), dtype=_E4M3)
     scales = x.new_empty((-(-m // rows), -(-k // _BLOCK8)), dtype=torch.float32)
     if m and k:
         _check8(_launch("llm_quantize_blocks", x.data_ptr(), code, x.stride(0), values.data_ptr(), scales.data_ptr(), m, k, rows, _stream()), "quantize_blocks")
-    return Quantized(values, scales, rows, powers_of_two=True)
+    q = object.__new__(Quantized)  # (what its constructor asks is so)
+    q.values, q.scales, q.rows, q.shape, q.powers_of_two = values, scales, rows, shape, True
+    return q
 
 
 def _check8(code: int, what: str) -> None:
@@ -2395,34 +2397,34 @@ def linear8(x, w: Quantized, out_dtype: torch.dtype | None = None) -> torch.Tens
     the tensor cores and enter 32-bit sums times both scales; scales that are powers of two on both sides (those of
     :func:`quantize_weight` are) the tensor cores may apply themselves, and sum over all blocks.  Few rows go to a kernel that
     streams the weights, more to tcgen05.  ``K`` is a multiple of 16.  ``out_dtype``: float32 or bfloat16 (default: that of ``x``, bfloat16 for a quantised one)."""
-    _need(isinstance(w, Quantized) and w.rows == _BLOCK8, "linear8: w is a Quantized matrix with a scale for every 128 rows")
+    if not isinstance(w, Quantized) or w.rows != _BLOCK8:
+        raise KernelError("linear8: w is a Quantized matrix with a scale for every 128 rows")
     if isinstance(x, NormedInput):
         x = x.materialize()
     given = isinstance(x, Quantized)
     xt = x.values if given else x
-    n, k = w.shape
-    if not (len(x.shape) == 2 and x.shape[1] == k and k % 16 == 0 and k >= 16 and xt.stride(1) == 1 and (not given or x.rows == 1)):
+    shape, (n, k) = x.shape, w.shape
+    if not (len(shape) == 2 and shape[1] == k and k % 16 == 0 and k >= 16 and xt.stride(1) == 1 and (not given or x.rows == 1)):
         _need(not given or x.rows == 1, "linear8: a quantised x has a scale for every row")
-        _need(len(x.shape) == 2 and x.shape[1] == k, f"linear8: shapes {tuple(x.shape)} and {tuple(w.shape)} do not match")
+        _need(len(shape) == 2 and shape[1] == k, f"linear8: shapes {tuple(shape)} and {tuple(w.shape)} do not match")
         _need(k >= 16 and k % 16 == 0, f"linear8: rows of {k} values; a multiple of 16 is needed")
         raise KernelError("linear8: x has unit inner stride")
-    m = x.shape[0]
+    m = shape[0]
     x_code = 0 if given else _code(x.dtype)
     out_dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
     code = _code(out_dtype)
-    _here(xt, w.values)
+    values = w.values
+    _here(xt, values)
     out = xt.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return out
-    if given:
-        xq = None
-        _need(xt.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
-    else:  # values and scales of the quantised x
-        blocks = -(-k // _BLOCK8)
-        xq = xt.new_empty((m * k + 4 * m * blocks,), dtype=torch.uint8)
-    _need(w.values.data_ptr() % 16 == 0, "linear8: 8-bit matrices start on 16 bytes")
-    _check8(_launch("llm_linear8", xt.data_ptr(), x_code, 0 if given else xt.stride(0), x.scales.data_ptr() if given else None, None if given else xq.data_ptr(),
-                    w.values.data_ptr(), w.scales.data_ptr(), w.powers_of_two and (not given or x.powers_of_two), out.data_ptr(), code, m, n, k, n, _error_flag_ptr(), _stream()), "linear8")
+    x_at, w_at = xt.data_ptr(), values.data_ptr()
+    if w_at % 16 or (given and x_at % 16):
+        raise KernelError("linear8: 8-bit matrices start on 16 bytes")
+    # values and scales of the quantised x
+    xq = None if given else xt.new_empty((m * (k - 4 * (-k // _BLOCK8)),), dtype=torch.uint8)
+    _check8(_launch("llm_linear8", x_at, x_code, 0 if given else xt.stride(0), x.scales.data_ptr() if given else None, None if given else xq.data_ptr(),
+                    w_at, w.scales.data_ptr(), w.powers_of_two and (not given or x.powers_of_two), out.data_ptr(), code, m, n, k, n, _error_flag_ptr(), _stream()), "linear8")
     if not given:
         add_launches(1)
     return out
@@ -2487,8 +2489,9 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     _i32(page_table, "page_table")
     _i32(cu_tokens, "cu_tokens")
     _i32(context_lens, "context_lens")
-    n, requests = q.shape[0], context_lens.numel()
-    _need(page_table.dim() == 2 and page_table.shape[0] == requests and cu_tokens.numel() == requests + 1, "paged_attention8: a row of the page table and a length for every request")
+    n, requests, places = q.shape[0], context_lens.numel(), page_table.shape
+    if len(places) != 2 or places[0] != requests or cu_tokens.numel() != requests + 1:
+        raise KernelError("paged_attention8: a row of the page table and a length for every request")
     _here(q, pool, exponents, page_table, cu_tokens, context_lens)
     out = q.new_empty((n, width))
     if n == 0 or requests == 0:
@@ -2508,7 +2511,7 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     if ranges:
         scratch = q.new_empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32)
         add_launches(1)
-    _check8(_launch("llm_attention8", q.data_ptr(), q.stride(0), out.data_ptr(), width, pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), page_table.shape[1],
+    _check8(_launch("llm_attention8", q.data_ptr(), q.stride(0), out.data_ptr(), width, pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), places[1],
                     cu_tokens.data_ptr(), context_lens.data_ptr(), requests, n, longest, below, num_heads, num_kv_heads, head_dim, pool.shape[3],
                     pool.shape[0], int(window or 0), float(scale), warps, ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
             "paged_attention8")
