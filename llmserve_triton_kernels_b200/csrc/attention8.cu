@@ -4,14 +4,14 @@
 //
 // Rows are (token, query head of the key head's group).  They ride along as the narrow side of both products: a tile of mma.sync is 16
 // keys (then: 16 lanes of the output) high and 8 rows wide, so that a group of up to 8 heads wastes nothing; a CTA takes one or two
-// such tiles of rows.  What bounds it is the pages' bytes, and behind them the instructions that unpack them, so there are few: with
-// the lanes of a head permuted alike in q and k (a dot product does not notice) a thread's 16-byte load of a key is the A operand of
-// two e4m3 products as it lies there.  q takes part as the sum of two e4m3 numbers, its row scaled to [128, 256): the first has a
-// value's upper 4 bits, the second the next 4, which is all that bfloat16 has (2^-18 of the row's largest value is what may be lost
-// of small ones).  Values become half precision (exact; one instruction for two): since the output's lanes may come in any order, a
-// thread's bytes of four values are the A elements of the second product.  Its weights stay in half precision, not in e4m3, whose
-// 18 powers of two would drop the many small weights of a long context.  They turn from the first product's result into the
-// second's operand by a transposition of 8 x 8 (movmatrix).
+// such tiles of rows.  What bounds it is the pages' bytes, and behind them the instructions that unpack them.  Both products are in
+// half precision, which holds every e4m3 number: with the lanes of a head permuted alike in q and k (a dot product does not
+// notice) a thread's 16 bytes of a key are the A elements of four products once they are converted, one instruction for two; and
+// since the output's lanes may come in any order, so are its bytes of four values, two by two interleaved, for the second product.
+// q, its row scaled to [128, 256), loses nothing but what lies 2^-22 and more below the row's largest value.  (Products of e4m3 would
+// save the conversion but for mma.sync, which converts by itself: q as two e4m3 numbers took 125 of 497 instructions a tile, q in half
+// precision takes 40 fewer.)  The weights stay in half precision too: e4m3's 18 powers of two would drop the many small weights of
+// a long context.  They turn from the first product's result into the second's operand by a transposition of 8 x 8 (movmatrix).
 //
 // A value's weight 2^(s_j + ev_j) has a running maximum of its own, apart from that of 2^(s_j): whatever the values' scales, the
 // weights that enter the half-precision product are at most one and the largest is one.
@@ -28,15 +28,17 @@
 // Cutting and joining cost 8 us and more, so short or many units of work go without: a CTA takes a tile of rows with all its keys, of two
 // warps instead of eight where there are many units of few keys, whose time is a CTA's 4 us of loads that wait for one another (q and
 // the page table, the pages, the warps' meeting) and not the bytes.  The host picks, from the longest context it is told.
-// Heads of 128 lanes, 32 over 8, requests of random lengths: 32 of up to 8,191 keys 73 us, 4.8 TB/s of pages; 64 of up to 4,000 78 us, 4.4
-// TB/s; 8 of up to 4,000 20 us, of which 8 are laying out, cutting and joining.  It is not the memory that bounds the first (with all pages
-// in the L2 it took 5 % less) but the warps' own chains: 440 instructions a tile of 16 keys, issued in 59 % of the cycles with the
-// 4 warps that an SM's quarter has registers for.
+// Heads of 128 lanes, requests of random lengths, 32 heads over 8: 32 of up to 8,191 keys 67 us, 5.2 TB/s of pages; 64 of up to 4,000 69 us,
+// 4.9 TB/s; 8 of up to 4,000 19 us, of which 8 are laying out, cutting and joining.  32 heads of their own: 64 of up to 4,000 219 us, 6.25 TB/s.
+// It is not the memory that bounds the first but the warps' own chains: 383 instructions a tile of 16 keys with the 4 warps that an SM's
+// quarter has registers for (500 instructions a tile took 73 us, the same pages all in the L2 5 % less).
 //
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
 // Where rows differ in what they see, NaN among the values is counted apart, so that it reaches the rows that see it alone.
 #include "fp8.cuh"
 #include "tma.cuh"
+
+#include <type_traits>
 
 namespace {
 
@@ -72,10 +74,6 @@ struct Attn8Params {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned half2_of(unsigned short v) {
@@ -338,8 +336,8 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
 
-        // ---- q: product j of a key takes lanes (D / 4) t + 8 j + 0 .. 7 of a row, as the keys' bytes lie ----
-        unsigned qb[NT][KSTEPS][2][2];  // [upper, lower bits][first, second four lanes]
+        // ---- q in half precision: product i of a key takes lanes (D / 4) t + 4 i + 0 .. 3 of a row, as the keys' bytes lie ----
+        unsigned qh[NT][D / 16][2];
         float factor[NT][2];  // of this thread's rows, which are 2 t and 2 t + 1 of every tile in the products' results
         int pos[NT][2];
 #pragma unroll
@@ -361,24 +359,9 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
 #pragma unroll
             for (int j = 0; j < KSTEPS; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        v[2 * i] = __uint_as_float(raw[nt][j][2 * e + i] << 16) * f0 * f1;
-                        v[2 * i + 1] = __uint_as_float(raw[nt][j][2 * e + i] & 0xffff0000u) * f0 * f1;
-                    }
-                    const unsigned upper = fp8::pack4(v[0], v[1], v[2], v[3], 1.f);
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const unsigned h2 = half2_of((unsigned short)(upper >> (16 * i)));
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-                        w[2 * i] = v[2 * i] - back.x;
-                        w[2 * i + 1] = v[2 * i + 1] - back.y;
-                    }
-                    qb[nt][j][0][e] = upper;
-                    qb[nt][j][1][e] = fp8::pack4(w[0], w[1], w[2], w[3], 1.f);
+                for (int e = 0; e < 4; ++e) {
+                    const float a = __uint_as_float(raw[nt][j][e] << 16) * f0 * f1, b = __uint_as_float(raw[nt][j][e] & 0xffff0000u) * f0 * f1;
+                    qh[nt][2 * j + (e >> 1)][e & 1] = pack_half(fmaf(a, 0.f, a), fmaf(b, 0.f, b));  // infinities become NaN
                 }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -411,159 +394,165 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
             const int j0 = (tile_lo + warp + i0 * WARPS) * TILE;
             const unsigned char* stage = ring + slot * S::BYTES;
 
-            // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
-            // (one sum: four, so that no product waits for another, need registers that the SM's other warps then lack: 2 us of 75)
-            float s[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) {
-                const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
-                const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
-                const unsigned a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
-#pragma unroll
-                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_e4m3(s[nt], a0, qb[nt][2 * x][part][0], qb[nt][2 * x][part][1]);
-#pragma unroll
-                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_e4m3(s[nt], a1, qb[nt][2 * x + 1][part][0], qb[nt][2 * x + 1][part][1]);
-            }
-            unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 2 * t + (e & 1) + 8 * (e >> 1);
-                if constexpr (D == 128) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(row, g));
-                    v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(stage + S::VALUES + S::key(row, g >> 1) + (g & 1) * 8);
-                    v[e][0] = w.x, v[e][1] = w.y;
-                }
-            }
-            float ev[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const unsigned char* at = scales[warp][slot] + g + 8 * x;
-                const float ks = __uint_as_float((unsigned)at[0] << 23);
-                ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
+            const auto work = [&](auto masked) {
+                // ---- scores: [key g | g + 8][row 2 t | 2 t + 1] of every tile of rows ----
+                float s[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) s[nt][2 * x + e] *= ks * factor[nt][e];
-            }
-            if (j0 < whole_from || j0 > whole_to) {
+                    for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) {
+                    const unsigned char* at = stage + S::key(g, (D / 64) * t + x);
+                    const uint4 k0 = *reinterpret_cast<const uint4*>(at), k1 = *reinterpret_cast<const uint4*>(at + S::SECOND);
+                    const unsigned w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned a[4] = {half2_of((unsigned short)w0[i]), half2_of((unsigned short)w1[i]), half2_of((unsigned short)(w0[i] >> 16)),
+                                               half2_of((unsigned short)(w1[i] >> 16))};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a, qh[nt][4 * x + i][0], qh[nt][4 * x + i][1]);
+                    }
+                }
+                unsigned v[4][D / 32];  // D / 8 bytes of the values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 2 * t + (e & 1) + 8 * (e >> 1);
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(row, g));
+                        v[e][0] = w.x, v[e][1] = w.y, v[e][2] = w.z, v[e][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(stage + S::VALUES + S::key(row, g >> 1) + (g & 1) * 8);
+                        v[e][0] = w.x, v[e][1] = w.y;
+                    }
+                }
+                float ev[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int j = j0 + g + 8 * x;
+                    const unsigned char* at = scales[warp][slot] + g + 8 * x;
+                    const float ks = __uint_as_float((unsigned)at[0] << 23);
+                    ev[x] = __uint_as_float(0x4b000000u | at[TILE]) - (8388608.f + 127.f);  // 2^23 + b has b as its lowest bits
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (j > pos[nt][e] || j >= key_end || (p.window > 0 && j <= pos[nt][e] - p.window)) s[nt][2 * x + e] = -INFINITY;
+                        for (int e = 0; e < 2; ++e) s[nt][2 * x + e] *= ks * factor[nt][e];
                 }
-                // a value that no row of the tile sees is nobody's
+                if constexpr (decltype(masked)::value) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
-                    if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
+                    for (int x = 0; x < 2; ++x) {
+                        const int j = j0 + g + 8 * x;
 #pragma unroll
-                        for (int w = 0; w < D / 32; ++w) v[e][w] = 0u;
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (j > pos[nt][e] || j >= key_end || (p.window > 0 && j <= pos[nt][e] - p.window)) s[nt][2 * x + e] = -INFINITY;
                     }
-                }
-                if (pos_min != pos_max) {
-                    // Some row may see a key that another does not, and NaN times a weight of zero is NaN: NaN among the values is taken out and
-                    // counted by a product of its own, of ones where a value is NaN and where a row sees a key.
-                    unsigned any = 0;
+                    // a value that no row of the tile sees is nobody's
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + 2 * t + (e & 1) + 8 * (e >> 1);
+                        if (j > pos_max || j >= key_end || (p.window > 0 && j <= pos_min - p.window)) {
 #pragma unroll
-                        for (int w = 0; w < D / 32; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                    if (__any_sync(0xffffffffu, any != 0)) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            unsigned seen[2];
-#pragma unroll
-                            for (int x = 0; x < 2; ++x)
-                                seen[x] = transpose((s[nt][2 * x] == -INFINITY ? 0u : 0x3c00u) | (s[nt][2 * x + 1] == -INFINITY ? 0u : 0x3c000000u));
-#pragma unroll
-                            for (int x = 0; x < MTILES; ++x) {
-                                unsigned bad[4];
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {  // lane byte 2 x + (q & 1), keys 2 t + 8 (q >> 1) and the next
-                                    const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
-                                    bad[q] = (((v[e][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c00u : 0u) |
-                                             (((v[e + 1][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c000000u : 0u);
-                                }
-                                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_f16(c, bad, seen[0], seen[1]);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (c[e] > 0.f) o[nt][x][e] = NAN;
-                            }
+                            for (int w = 0; w < D / 32; ++w) v[e][w] = 0u;
                         }
+                    }
+                    if (pos_min != pos_max) {
+                        // Some row may see a key that another does not, and NaN times a weight of zero is NaN: NaN among the values is taken out and
+                        // counted by a product of its own, of ones where a value is NaN and where a row sees a key.
+                        unsigned any = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
-                            for (int w = 0; w < D / 32; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                            for (int w = 0; w < D / 32; ++w) any |= __vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                unsigned seen[2];
+#pragma unroll
+                                for (int x = 0; x < 2; ++x)
+                                    seen[x] = transpose((s[nt][2 * x] == -INFINITY ? 0u : 0x3c00u) | (s[nt][2 * x + 1] == -INFINITY ? 0u : 0x3c000000u));
+#pragma unroll
+                                for (int x = 0; x < MTILES; ++x) {
+                                    unsigned bad[4];
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q) {  // lane byte 2 x + (q & 1), keys 2 t + 8 (q >> 1) and the next
+                                        const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
+                                        bad[q] = (((v[e][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c00u : 0u) |
+                                                 (((v[e + 1][b / 4] >> (8 * (b & 3))) & 0x7fu) == 0x7fu ? 0x3c000000u : 0u);
+                                    }
+                                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma_f16(c, bad, seen[0], seen[1]);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (c[e] > 0.f) o[nt][x][e] = NAN;
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int w = 0; w < D / 32; ++w) v[e][w] &= ~__vcmpeq4(v[e][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        }
                     }
                 }
-            }
-            // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
-            // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
-            unsigned pb[NT][2];
-            float u[NT][4];
-            bool behind = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    u[nt][e] = s[nt][e] + ev[e >> 1];
-                    behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
-                }
-            if (__any_sync(0xffffffffu, behind)) {
+                // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
+                // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
+                unsigned pb[NT][2];
+                float u[NT][4];
+                bool behind = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
-                        const float keep = exp2_fast(m2[nt][e] - b);
-                        sum[nt][e] *= exp2_fast(m1[nt][e] - a);
-                        m1[nt][e] = a;
-                        m2[nt][e] = b;
-#pragma unroll
-                        for (int x = 0; x < MTILES; ++x) {
-                            o[nt][x][e] *= keep;
-                            o[nt][x][2 + e] *= keep;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        u[nt][e] = s[nt][e] + ev[e >> 1];
+                        behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
                     }
-            }
+                if (__any_sync(0xffffffffu, behind)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    sum[nt][e] += exp2_fast(s[nt][e] - m1[nt][e]) + exp2_fast(s[nt][2 + e] - m1[nt][e]);
-                    u[nt][e] = exp2_fast(u[nt][e] - m2[nt][e]);
-                    u[nt][2 + e] = exp2_fast(u[nt][2 + e] - m2[nt][e]);
-                }
-                pb[nt][0] = transpose(pack_half(u[nt][0], u[nt][1]));
-                pb[nt][1] = transpose(pack_half(u[nt][2], u[nt][3]));
-            }
-            // ---- values: tile x takes bytes 2 x and 2 x + 1 of the thread's of every key ----
+                        for (int e = 0; e < 2; ++e) {
+                            const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
+                            const float keep = exp2_fast(m2[nt][e] - b);
+                            sum[nt][e] *= exp2_fast(m1[nt][e] - a);
+                            m1[nt][e] = a;
+                            m2[nt][e] = b;
 #pragma unroll
-            for (int x = 0; x < MTILES; ++x) {
-                unsigned a[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int b = 2 * x + (q & 1), e = 2 * (q >> 1);
-                    a[q] = half2_of((unsigned short)__byte_perm(v[e][b / 4], v[e + 1][b / 4], 0x0040u + 0x0011u * (b & 3)));
+                            for (int x = 0; x < MTILES; ++x) {
+                                o[nt][x][e] *= keep;
+                                o[nt][x][2 + e] *= keep;
+                            }
+                        }
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][x], a, pb[nt][0], pb[nt][1]);
-            }
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        sum[nt][e] += exp2_fast(s[nt][e] - m1[nt][e]) + exp2_fast(s[nt][2 + e] - m1[nt][e]);
+                        u[nt][e] = exp2_fast(u[nt][e] - m2[nt][e]);
+                        u[nt][2 + e] = exp2_fast(u[nt][2 + e] - m2[nt][e]);
+                    }
+                    pb[nt][0] = transpose(pack_half(u[nt][0], u[nt][1]));
+                    pb[nt][1] = transpose(pack_half(u[nt][2], u[nt][3]));
+                }
+                // ---- values: tile x takes bytes 2 x and 2 x + 1 of the thread's of every key ----
+#pragma unroll
+                for (int x = 0; x < MTILES; ++x) {
+                    unsigned a[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {  // lane bytes 2 x and 2 x + 1 of keys 2 t + 4 e and the next
+                        const unsigned w = __byte_perm(v[e][x / 2], v[e + 1][x / 2], x & 1 ? 0x7362u : 0x5140u);
+                        a[e] = half2_of((unsigned short)w);
+                        a[e + 1] = half2_of((unsigned short)(w >> 16));
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][x], a, pb[nt][0], pb[nt][1]);
+                }
+            };
+            // (written out twice: with the masks in the same code a tile took 57 instructions more)
+            if (j0 < whole_from || j0 > whole_to)
+                work(std::true_type{});
+            else
+                work(std::false_type{});
         }
 
         // ---- the warps meet, where the rings were ----

@@ -2485,10 +2485,12 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
         _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, f"paged_attention8: {num_heads} query heads over {num_kv_heads} key heads")
         raise KernelError("paged_attention8: a window holds a key at least")
     _pages8(pool, exponents, num_kv_heads, head_dim, "paged_attention8")
-    cu_tokens, context_lens = ctx.cu_tokens, ctx.context_lens
-    _i32(page_table, "page_table")
-    _i32(cu_tokens, "cu_tokens")
-    _i32(context_lens, "context_lens")
+    cu_tokens, context_lens, i32 = ctx.cu_tokens, ctx.context_lens, torch.int32
+    if not (page_table.dtype is i32 and cu_tokens.dtype is i32 and context_lens.dtype is i32 and page_table.is_contiguous() and cu_tokens.is_contiguous()
+            and context_lens.is_contiguous()):
+        _i32(page_table, "page_table")
+        _i32(cu_tokens, "cu_tokens")
+        _i32(context_lens, "context_lens")
     n, requests, places = q.shape[0], context_lens.numel(), page_table.shape
     if len(places) != 2 or places[0] != requests or cu_tokens.numel() != requests + 1:
         raise KernelError("paged_attention8: a row of the page table and a length for every request")
@@ -2556,10 +2558,10 @@ def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_d
     A unit is a tile of 8 or 16 rows of a request and a key head, with at most ``keys`` keys.  Without stretches (0) a CTA takes a unit; with
     them the keys of all units are dealt out evenly and a second kernel joins what was cut.  Measured on 148 SMs with heads of 128 lanes
     (64 lanes: two thirds of what goes by keys), CTAs of 8 warps, requests of random lengths up to k thousands of keys, u units an SM: a
-    CTA takes 4 + 8 k us and all (u + 1) (2 + 4.2 k) us, in stretches 10 + u (2.5 + 4.4 k) us.  64 units of 4,000 keys: 36.5 us, in
-    stretches 20.0; 256 of 8,191: 104 and 73; 256 of 1,000: 17.8 and 20.9; 1,024 of 2,000: 80 and 87.  Stretches are as many as CTAs find
-    room at once, or half of them where there is little for each and few units, which leaves less to join: 8 units of 16,000 keys 19.1 us
-    instead of 21.8, 64 of 2,000 18.6 instead of 15.3, 64 of 4,000 25.9 instead of 20.0.  Many short units are better off with CTAs of 2 warps, of
+    CTA takes 4 + 6.5 k us and all (u + 1) (1.8 + 3.5 k) us, in stretches 9.5 + u (2.5 + 3.9 k) us.  64 units of 4,000 keys: 30.4 us, in
+    stretches 19.2; 256 of 8,191: 82 and 67; 256 of 1,000: 15.3 and 19.3; 1,024 of 2,000: 69 and 75.  Stretches are as many as CTAs find
+    room at once, or half of them where there is little for each and few units, which leaves less to join: 8 units of 16,000 keys 17.6 us
+    instead of 20.7, 64 of 2,000 18.6 instead of 15.3, 64 of 4,000 25.9 instead of 20.0.  Many short units are better off with CTAs of 2 warps, of
     which there is room for four times as many: 1,824 units of 20 keys take 13.3 us instead of 32.7, of 250 keys 29 instead of 44; 256
     units of 1,000 30 instead of 18."""
     if _ATTENTION8_SPLIT is not None:
@@ -2571,6 +2573,6 @@ def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_d
     if keys <= 256 or requests > 1024:  # (the list of requests' shares is held in shared memory)
         return 8, 0
     k = keys * (head_dim + 64) / 192e3
-    if max(4 + 8 * k, (units / sms + 1) * (2 + 4.2 * k)) <= 10 + units / sms * (2.5 + 4.4 * k):
+    if max(4 + 6.5 * k, (units / sms + 1) * (1.8 + 3.5 * k)) <= 9.5 + units / sms * (2.5 + 3.9 * k):
         return 8, 0
     return 8, sms * (2 if height == 8 and (units * keys >= 1700 * sms or units * 3 >= sms) else 1)
