@@ -7,8 +7,8 @@
 // Where there are fewer tiles than SMs, `split` CTAs (a cluster) share a tile's k-blocks and add up in one another's shared memory.
 //
 // What bounds it: a k-block of 64 rows takes the sums' warps some 600 cycles (16 KB of weights in 0.33 us, 7.5 TB/s over all SMs), of 128
-// 850; and around them some 6 us of a launch, of first copies, and of the cluster's meeting and adding.  33 rows by 32,000 features of
-// 2,048: 19 us, by 4,096 of 14,336 16.9, by 4,096 of 4,096 9.8, each with x quantised in front.
+// 850; and around them some 6 us of a launch, of first copies, and of the cluster's meeting and adding.  With x quantised in front 33 rows by
+// 32,000 features of 2,048 take 20 us (250 tiles, two rounds), 32 rows by 4,096 of 14,336 16.9, by 4,096 of 4,096 9.8.
 #include "common.cuh"
 #include "linear8.h"
 #include "linear8_store.cuh"

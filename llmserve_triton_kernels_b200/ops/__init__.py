@@ -2311,8 +2311,8 @@ def delta_rule(y: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor, a_log: 
 
 
 # ------------------------------------------------------------------------------------------------
-# Numbers in 8 bits: matrices of e4m3 values with a scale for every block of 128 (csrc/fp8.cuh, quantize_blocks.cu,
-# linear8_few.cu, gemm8_tcgen05.cu), and pages of keys and values with one for every head's vector (rope_kv_write8.cu, attention8.cu).
+# Numbers in 8 bits: matrices of e4m3 values with a scale for every block of 128 (csrc/fp8.cuh, quantize_blocks.cu, linear8.cu and
+# what it calls), and pages of keys and values with one for every head's vector (rope_kv_write8.cu, attention8.cu).
 _E4M3 = torch.float8_e4m3fn
 _BLOCK8 = 128
 ATTENTION8_HEAD_DIMS = (64, 128)

@@ -568,6 +568,37 @@ def test_captured_replayed_and_beside_one_another():
             assert torch.equal(o, want[(turn + i) % 4])
 
 
+def test_large_calls_beside_one_another():
+    """Every kernel of the products and of the attention on two streams at once, with the results that each has alone."""
+    o = ops()
+    calls = []
+    for m, n, k, powers in ((3, 4000, 1024, True), (40, 3000, 1040, True), (40, 3000, 1040, False), (200, 1000, 2064, True), (200, 1000, 2064, False), (700, 9000, 528, True),
+                            (700, 9000, 528, False), (600, 1100, 4112, True), (500, 4000, 528, False)):
+        w = o.quantize_weight(spread(n, k, 128, m + k)) if powers else weights(n, k, m + k)
+        x = spread(m, k, 1, n).to(BF16)
+        calls.append(lambda x=x, w=w: o.linear8(x, w))
+    for H, KV, D, counts, held in ((16, 2, 128, [1] * 5, [3000, 20, 700, 1500, 1]), (8, 8, 64, [1] * 60, list(range(1, 61))), (8, 2, 64, [200, 1, 140], [500, 900, 140])):
+        ctx, table, _, pages = a_step(counts, held, 16, H)
+        cache = pages8(pages, KV, 16, D, H)
+        q = torch.randn(ctx.num_tokens, H * D, generator=gen(H), device=DEV).to(BF16)
+        calls.append(lambda q=q, cache=cache, table=table, ctx=ctx, heads=(H, KV, D): o.paged_attention8(
+            q, *cache, table, ctx, num_heads=heads[0], num_kv_heads=heads[1], head_dim=heads[2], scale=0.1))
+    want = [call().clone() for call in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for turn in range(8):
+        got = []
+        for i in range(len(calls)):
+            for j, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    at = (i * (1 + 4 * j) + turn * j) % len(calls)
+                    got.append((at, calls[at]()))
+        torch.cuda.synchronize()
+        for at, y in got:
+            assert torch.equal(y, want[at]), at
+    o.check_device_errors()
+
+
 def test_operands_on_the_host_are_refused():
     o = ops()
     x, w = torch.randn(4, 128, device=DEV).to(BF16), weights(64, 128, 1)
