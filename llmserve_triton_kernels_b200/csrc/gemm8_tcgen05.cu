@@ -15,9 +15,9 @@
 // a pair.  The roles that issue were the bound before they were two warps each: a k-block's waits, products and commits take one
 // warp 600 cycles (533 us for 4,096 x 28,672 x 4,096 with one, 459 with two: 2,096 TFLOP/s with x quantised in front).  Scales are read
 // where rows lie side by side (linear8.h): from [rows, blocks] the same product took 100 us more.
-// One CTA per SM walks 128 x 128 tiles, or a pair of CTAs 256 x 256, column tiles outermost, so that CTAs that run at the same time share their weights.  What lies beyond
-// the matrices arrives as zeros and is masked at the store.  Every wait is bounded; one that gives up sets *error_flag and the
-// roles run to their ends.
+// One CTA per SM walks 128 x 128 tiles, or a pair of CTAs 256 x 256, column tiles outermost, so that CTAs that run at the same time share
+// their weights.  What lies beyond the matrices arrives as zeros and is masked at the store.  Every wait is bounded; one that gives up
+// sets *error_flag and the roles run to their ends.
 #include "common.cuh"
 #include "linear8.h"
 #include "linear8_store.cuh"
@@ -437,7 +437,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
-    if (failed()) {  // (both CTAs know.)  Nobody waits for the copies on their way any more; they are counted at the first CTA, and the other's memory takes some
+    if (failed()) {  // (both CTAs know.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
         if (place == 0 && warp < FIRST_ISSUER) {
             for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
                 if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);

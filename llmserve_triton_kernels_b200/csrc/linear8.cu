@@ -6,14 +6,16 @@
 
 // x [M, K]: float32 or bfloat16 (x_dtype; row stride ldx, unit inner stride), quantised into `scratch` (16-byte aligned, M K + 4 M ceil(K / 128)
 // bytes); or, with sx [M, ceil(K / 128)] float32 (not null), e4m3, contiguous, on 16 bytes.  w [N, K] e4m3, contiguous, on 16 bytes; sw
-// [ceil(N / 128), ceil(K / 128)] float32; `powers`: these scales, and those of an x that comes quantised, are powers of two.  K a multiple of 16.  out [M, N] (row stride ldo), float32 or bfloat16.
+// [ceil(N / 128), ceil(K / 128)] float32; `powers`: these scales, and those of an x that comes quantised, are powers of two.  K a
+// multiple of 16.  out [M, N] (row stride ldo), float32 or bfloat16.
 LLM_EXPORT int llm_linear8(const void* x, int x_dtype, long long ldx, const float* sx, void* scratch, const void* w, const float* sw, int powers, void* out,
                            int out_dtype, int M, int N, int K, int ldo, int* error_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K < 16 || (K & 15) || ((uintptr_t)w & 15) || (out_dtype != LLM_F32 && out_dtype != LLM_BF16)) return LLM_ERR_BAD_ARGUMENT;
     const bool given = sx != nullptr;
     if (given ? ((uintptr_t)x & 15) != 0 : !scratch || ((uintptr_t)scratch & 15)) return LLM_ERR_BAD_ARGUMENT;
-    linear8::Operands p = {(const unsigned char*)x, sx, given ? (K + 127) / 128 : 1, given ? 1 : M, (const unsigned char*)w, sw, out, M, N, K, (K + 127) / 128, ldo, out_dtype};
+    linear8::Operands p = {(const unsigned char*)x, sx, given ? (K + 127) / 128 : 1, given ? 1 : M, (const unsigned char*)w, sw, out, M, N, K,
+                           (K + 127) / 128, ldo, out_dtype};
     if (!given) {
         unsigned char* values = (unsigned char*)scratch;
         float* scales = reinterpret_cast<float*>(values + (size_t)M * K);  // K is a multiple of 16

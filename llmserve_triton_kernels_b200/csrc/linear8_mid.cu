@@ -258,8 +258,8 @@ int launch(const linear8::Operands& p, int early, int* error_flag, cudaStream_t 
     const int sms = device_sms();
     int split = 1;  // doubled while all CTAs still run at once and none has fewer than four k-blocks
     while (split < MAX_SPLIT && tiles * split * 2 <= sms && p.kblocks >= 8 * split) split *= 2;
-    return linear8::launch_clusters(kernel, (unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms), (FIRST_EPI + EPI_WARPS) * 32, smem, split, stream, p, split, early, error_flag,
-                                    xmap, wmap);
+    return linear8::launch_clusters(kernel, (unsigned)(split > 1 ? tiles * split : tiles < sms ? tiles : sms), (FIRST_EPI + EPI_WARPS) * 32, smem,
+                                    split, stream, p, split, early, error_flag, xmap, wmap);
 }
 
 }  // namespace

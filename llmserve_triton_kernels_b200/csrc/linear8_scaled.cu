@@ -68,7 +68,8 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
     constexpr unsigned IDESC = umma::idesc_e4m3_scaled(BM, BN);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], scales_full[GROUPS], scales_empty[GROUPS], drained;
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], acc_full[NBUF], acc_empty[NBUF], drained;
+    __shared__ __align__(8) unsigned long long scales_full[GROUPS], scales_empty[GROUPS];
     __shared__ unsigned tmem_base;
     __shared__ int gave_up, asked[2];
 
@@ -295,7 +296,8 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     constexpr int COLS = BN / (PAIR_EPI_WARPS / 4);  // of an epilogue warp
     constexpr int KB_COLS = 16;                      // of a k-block's scales: 4 of the CTA's rows of x, 8 of the weights' rows, 4 unused
     constexpr int PITCH = BN + 4;
-    static_assert((size_t)BM * PITCH * 4 <= (size_t)STAGES * SLOT_BYTES + PAIR_EPI_WARPS * linear8::PIECE_BYTES<TO>, "a split tile's sums lie where ring and staging were");
+    static_assert((size_t)BM * PITCH * 4 <= (size_t)STAGES * SLOT_BYTES + PAIR_EPI_WARPS * linear8::PIECE_BYTES<TO>,
+                  "a split tile's sums lie where ring and staging were");
     static_assert(BN <= SCALES_AT && SCALES_AT + GROUPS * GROUP * KB_COLS <= 512, "tensor memory");
     constexpr unsigned IDESC = umma::idesc_e4m3_scaled(2 * BM, BN);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -496,7 +498,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
-    if (f.failed()) {  // (the whole cluster knows.)  Nobody waits for the copies on their way any more; they are counted at the first CTA, and the other's memory takes some
+    if (f.failed()) {  // (the whole cluster knows.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
         if (place == 0 && warp < ISSUER) {
             for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
                 if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);

@@ -88,7 +88,9 @@ int launch(void* qkv, long long row_stride, const int* positions, const float* t
 LLM_EXPORT int llm_rope_kv_write8(void* qkv, long long row_stride, const int* positions, const float* table, int table_rows, const int* slot_map,
                                   void* pool, unsigned char* exponents, int n, int H, int KV, int D, int page_size, int pages, cudaStream_t stream) {
     if (n <= 0) return 0;
-    if (H < 0 || KV <= 0 || page_size <= 0 || pages <= 0 || (table && table_rows <= 0) || (row_stride & 7) || ((uintptr_t)qkv & 15) || ((uintptr_t)table & 15) || ((uintptr_t)pool & 7)) return LLM_ERR_BAD_ARGUMENT;
+    if (H < 0 || KV <= 0 || page_size <= 0 || pages <= 0 || (table && table_rows <= 0) || (row_stride & 7) || ((uintptr_t)qkv & 15) ||
+        ((uintptr_t)table & 15) || ((uintptr_t)pool & 7))
+        return LLM_ERR_BAD_ARGUMENT;
     if (D == 64) return launch<64>(qkv, row_stride, positions, table, table_rows, slot_map, pool, exponents, n, H, KV, page_size, pages, stream);
     if (D == 128) return launch<128>(qkv, row_stride, positions, table, table_rows, slot_map, pool, exponents, n, H, KV, page_size, pages, stream);
     return LLM_ERR_UNSUPPORTED;
