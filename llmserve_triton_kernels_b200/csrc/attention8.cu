@@ -13,8 +13,11 @@
 // precision takes 40 fewer.)  The weights stay in half precision too: e4m3's 18 powers of two would drop the many small weights of
 // a long context.  They turn from the first product's result into the second's operand by a transposition of 8 x 8 (movmatrix).
 //
-// A value's weight 2^(s_j + ev_j) has a running maximum of its own, apart from that of 2^(s_j): whatever the values' scales, the
-// weights that enter the half-precision product are at most one and the largest is one.
+// A value's weight 2^(s_j + ev_j) has a running reference of its own, apart from that of 2^(s_j): what enters the half-precision product
+// is the weight over that reference, which is kept 2^ABOVE below the largest of some time ago, so that the largest lies in [2^11, 2^15]
+// once references have settled and every weight down to 2^-25 of the largest has all 11 bits of half precision.  A weight below that loses at
+// most 2^-36 of the largest, times its value: it shows only in lanes where the largest's own value is next to nothing.  Vectors of zeros,
+// which are written with a scale of one, have no part in the reference, however large their weights: they enter the weights' sum alone.
 //
 // Work is counted in tiles of 16 keys for one tile of rows: a step's tiles, request after request, form one list, and every CTA takes an
 // equal stretch of it, wherever requests begin and end (their lengths are the device's business: a captured step is replayed at any
@@ -124,14 +127,19 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
 
 // References start below every score; a row whose weights' sum is zero has seen nothing.
 constexpr float NOTHING = -3.4028234e38f;
+// In powers of two: how far the values' reference is put below the largest weight, and how far a weight may then lie above that largest before
+// the reference moves.  Together 15, half precision's range above one: each more of the first is a power of two more for small weights, each more of
+// the second fewer meetings of the lanes.
+constexpr float ABOVE = 11.f, LAG = 4.f;
 
 // Two lanes of a row's output, columns c and c + 1 of the sums: its sum over the weights' sum; zeros for a row that saw no key.
 template <int D>
 __device__ __forceinline__ void finish(const Attn8Params& p, int first, int h, int rho, int c, float a, float b, float total, float y0, float y1) {
-    const float f = total == 0.f ? 0.f : exp2f(b - a) / total;
+    // 2^(b - a) in two factors: beside the smallest and the largest scales of values it may leave 32 bits' exponents where the output does not
+    const float f = exp2f(0.5f * (b - a)), each = total == 0.f ? 0.f : f / total;
     const int token = rho / p.G, lane = (D / 8) * ((c & 15) >> 1) + 2 * (c >> 4);
     __nv_bfloat16* at = p.out + (first + token) * p.out_stride + (long long)(h * p.G + rho - token * p.G) * D + lane;
-    *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(y0 * f, y1 * f);
+    *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(y0 * f * each, y1 * f * each);
 }
 
 // A request's share of the list: tiles of rows for every key head, and the tiles of keys that any of its rows sees.
@@ -494,8 +502,8 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
                         }
                     }
                 }
-                // ---- weights.  The references m1 and m2 are maxima of some time ago: they move only when a score has left them 2^16 or 2^8
-                // behind, which half precision and the 32-bit sums bear, so that most tiles need no meeting of the lanes ----
+                // ---- weights.  The references m1 and m2 belong to maxima of some time ago: they move only when a score has left these 2^16 or 2^LAG
+                // behind, which the 32-bit sums and half precision bear, so that most tiles need no meeting of the lanes ----
                 unsigned pb[NT][2];
                 float u[NT][4];
                 bool behind = false;
@@ -504,14 +512,34 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         u[nt][e] = s[nt][e] + ev[e >> 1];
-                        behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + 8.f;
+                        behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + (ABOVE + LAG);
                     }
                 if (__any_sync(0xffffffffu, behind)) {
+                    // A vector of zeros is written with a scale of one.  (To look at the values of every tile that comes here takes 32 requests of up to
+                    // 2,000 keys with 32 key heads of 128 lanes from 68.9 us to 70.6, of 64 lanes and 4 heads 8 of 1,000 from 8.5 to 8.8.)
+                    if (__any_sync(0xffffffffu, ev[0] == 0.f || ev[1] == 0.f)) {
+                        unsigned some = 0;  // bit j: value j is no vector of zeros
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            unsigned bits = 0;
+#pragma unroll
+                            for (int w = 0; w < D / 32; ++w) bits |= v[e][w];
+                            some |= (bits & 0x7f7f7f7fu ? 1u : 0u) << (2 * t + (e & 1) + 8 * (e >> 1));
+                        }
+                        some = __reduce_or_sync(0xffffffffu, some);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (!(some >> (g + 8 * x) & 1u)) {  // (its weight might not be a number of half precision)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) u[nt][2 * x] = u[nt][2 * x + 1] = -INFINITY;
+                            }
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e]))), b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])));
+                            const float a = fmaxf(m1[nt][e], row_max(fmaxf(s[nt][e], s[nt][2 + e])));
+                            const float b = fmaxf(m2[nt][e], row_max(fmaxf(u[nt][e], u[nt][2 + e])) - ABOVE);
                             const float keep = exp2_fast(m2[nt][e] - b);
                             sum[nt][e] *= exp2_fast(m1[nt][e] - a);
                             m1[nt][e] = a;
