@@ -760,8 +760,8 @@ int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
 // Rows of a tile for `longest` tokens a request and G query heads a key head: the sums that a stretch leaves are [2][rows][D + 4 + 3] floats.
 LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longest * G <= 8 ? 8 : 16; }
 
-// q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, on 16
-// bytes; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
+// q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, the pool on 16
+// bytes, the exponents anywhere; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
 // most tokens a request brings; with `below` requests that bring so many or more are left out, and their
 // rows of out as they are.  out [n, H D].  window 0: none.  warps of a CTA: 2 or 8.  ranges: CTAs that share the step's keys evenly, with
 // scratch memory of ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and
@@ -773,15 +773,16 @@ LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long
     if (n <= 0 || requests <= 0) return 0;
     if (H <= 0 || KV <= 0 || H % KV || page_size <= 0 || pages <= 0 || table_width <= 0 || longest <= 0 || (warps != 2 && warps != 8) || ranges < 0 || window < 0 ||
         (ranges && (!scratch || requests > MAX_REQUESTS || ((uintptr_t)scratch & 15))) || (q_stride & 3) || ((uintptr_t)q & 7) ||
-        (out_stride & 3) || ((uintptr_t)out & 7) || ((uintptr_t)pool & 15) || ((uintptr_t)exponents & 15) ||
+        (out_stride & 3) || ((uintptr_t)out & 7) || ((uintptr_t)pool & 15) ||
         (long long)table_width * page_size > 0x7fff0000)
         return LLM_ERR_BAD_ARGUMENT;
     const int rows = llm_attention8_rows(longest, H / KV);
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
                      page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, below, error_flag, warps, ranges,
                      scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};
-    // a tensor map's rows are counted in 32 bits
-    const int run = (long long)pages * 2 * KV * page_size > 0x7fffffffLL ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 0;
+    // a tensor map's rows are counted in 32 bits, and runs' exponents are copied eight at a time (a cache's planes start on 16 bytes where pages
+    // hold runs, anywhere where they do not)
+    const int run = (long long)pages * 2 * KV * page_size > 0x7fffffffLL || ((uintptr_t)exponents & 7) ? 0 : page_size % 16 == 0 ? 16 : page_size % 8 == 0 ? 8 : 0;
 #define ATTENTION8(D_, NT_) \
     (run == 16 ? launch<D_, NT_, 16>(p, longest, stream) : run == 8 ? launch<D_, NT_, 8>(p, longest, stream) : launch<D_, NT_, 0>(p, longest, stream))
     if (D == 64) return rows == 8 ? ATTENTION8(64, 1) : ATTENTION8(64, 2);

@@ -60,7 +60,7 @@ expand_pages8_kernel(const unsigned char* __restrict__ pool, const unsigned char
 
 }  // namespace
 
-// pool and exponents as rope_kv_write8.cu leaves them (16-byte aligned).  out: bfloat16 [requests with at least `least` tokens x width pages, 2, KV,
+// pool and exponents as rope_kv_write8.cu leaves them (the pool on 16 bytes).  out: bfloat16 [requests with at least `least` tokens x width pages, 2, KV,
 // page_size, D]; out_table [requests, width].  window 0: none; else pages that no token's window reaches are left as they are.  D 64 or 128.
 LLM_EXPORT int llm_expand_pages8(const void* pool, const void* exponents, const int* page_table, int width, const int* cu_tokens,
                                  const int* context_lens, int requests, int KV, int D, int page_size, int pages, int window, int least, void* out,

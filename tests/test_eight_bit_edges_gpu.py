@@ -64,3 +64,50 @@ def test_values_at_both_ends_of_the_exponents(exponent):
     exps[:, 1] = exponent
     q = torch.randn(1, 8 * D, generator=gen(5), device=DEV).to(BF16)
     check_attention(attend(q, pool, exps, table, ctx, D), q, pool, exps, table, ctx, 8, D, 0.05, None)
+
+
+@pytest.mark.parametrize("KV,page_size,more_pages", [(1, 1, 0), (4, 3, 1), (2, 2, 0), (1, 4, 1), (3, 8, 1), (1, 16, 1)])
+@pytest.mark.parametrize("counts,held", [([1, 3], [60, 33]), ([1], [2500])], ids=str)
+def test_planes_of_a_cache(KV, page_size, more_pages, counts, held):
+    """A cache's layers lie one after another in one allocation: the second and third start wherever the one in front ends."""
+    D, H = 64, 2 * KV
+    ctx, table, slots, pages = a_step(counts, held, page_size, 6, more_pages)
+    if pages % 2 == 0:
+        pages += 1
+    pool, exps = pages8(3 * pages, KV, page_size, D, 7)
+    pool, exps = pool.view(3, pages, 2, KV, page_size, D), exps.view(3, pages, 2, KV, page_size)
+    qkv = torch.randn(ctx.num_tokens, (H + 2 * KV) * D, generator=gen(8), device=DEV).to(BF16)
+    for plane in range(3):
+        ops().rope_kv_write8(qkv, ctx.positions, None, slots, pool[plane], exps[plane], H, KV, D)
+        got = ops().paged_attention8(qkv, pool[plane], exps[plane], table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+        check_attention(got, qkv, pool[plane], exps[plane], table, ctx, H, D, 0.1, None, f"plane {plane}")
+
+
+def test_exponents_that_start_anywhere():
+    """... and a caller's own, at any byte, over pages that hold tiles whole."""
+    H, KV, D, page_size = 4, 2, 128, 16
+    ctx, table, _, pages = a_step([1, 2, 130], [900, 40, 200], page_size, 6)
+    pool, exps = pages8(pages, KV, page_size, D, 7)
+    q = torch.randn(ctx.num_tokens, H * D, generator=gen(8), device=DEV).to(BF16)
+    want = ops().paged_attention8(q, pool, exps, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+    for offset in (1, 4, 8):
+        room = torch.zeros(exps.numel() + offset, dtype=torch.uint8, device=DEV)
+        moved = room[offset:].view(exps.shape)
+        moved.copy_(exps)
+        got = ops().paged_attention8(q, pool, moved, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+        assert torch.equal(got, want), offset
+
+
+def test_small_pages_in_the_engine():
+    """Single-token pages, an odd number of them, two key heads: the second layer's exponents start on four bytes."""
+    from llmserve_triton_kernels_b200 import LLM, SamplingParams
+    from test_eight_bit_model_gpu import CONFIG
+
+    prompts = [[5, 17, 200, 9], list(range(30, 45))]
+    tokens = []
+    for block_size, num_blocks in ((1, 101), (16, 8)):
+        llm = LLM(CONFIG, seed=3, max_batch_size=2, block_size=block_size, num_blocks=num_blocks, cache_dtype="float8", freeze_gc=False)
+        tokens.append([o.token_ids for o in llm.generate(prompts, SamplingParams(max_new_tokens=4))])
+        llm.cache.check()
+    assert [[len(t) for t in each] for each in tokens] == [[4, 4], [4, 4]]
+    assert [t[0] for t in tokens[0]] == [t[0] for t in tokens[1]]
