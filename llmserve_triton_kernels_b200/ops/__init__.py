@@ -95,7 +95,8 @@ _SIGNATURES = {
     "llm_quantize_blocks": [_vp, _i, _ll, _vp, _vp, _i, _i, _i, _vp],
     "llm_linear8": [_vp, _i, _ll, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp],
     "llm_rope_kv_write8": [_vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    "llm_expand_pages8": [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp],
+    "llm_expand_pages8": [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp],
+    "llm_spread_nan8": [_vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp],
     "llm_attention8": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp],
     "llm_branch_norm_sum": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
 }
@@ -2499,13 +2500,24 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     if n == 0 or requests == 0:
         return out
     longest = getattr(ctx, "max_query_len", None) or max(_token_counts(ctx))
-    below = 0
+    group, below, marks = num_heads // num_kv_heads, 0, None
     if longest >= _TC_ATTENTION_MIN_TOKENS:
-        below = _attention8_portions(q, pool, exponents, page_table, ctx, out, num_heads, num_kv_heads, head_dim, float(scale), int(window or 0))
+        below, marks = _attention8_portions(q, pool, exponents, page_table, ctx, out, num_heads, num_kv_heads, head_dim, float(scale), int(window or 0))
         if below:
             longest = max((c for c in _token_counts(ctx) if c < below), default=0)
-            if not longest:
-                return out
+    if longest:
+        _attention8(q, pool, exponents, page_table, ctx, out, num_heads, num_kv_heads, head_dim, float(scale), window, longest, below)
+    if below:
+        _check8(_launch("llm_spread_nan8", pool.data_ptr(), page_table.data_ptr(), marks.data_ptr(), places[1], cu_tokens.data_ptr(), context_lens.data_ptr(),
+                        requests, num_kv_heads, group, head_dim, pool.shape[3], pool.shape[0], int(window or 0), out.data_ptr(), width, _stream()), "spread_nan8")
+    return out
+
+
+def _attention8(q, pool, exponents, page_table, ctx, out, num_heads: int, num_kv_heads: int, head_dim: int, scale: float, window: int | None, longest: int,
+                below: int) -> None:
+    """Requests of fewer than ``below`` tokens (0: all), of which the longest brings ``longest`` (csrc/attention8.cu)."""
+    context_lens, places, (n, width) = ctx.context_lens, page_table.shape, out.shape
+    requests = places[0]
     keys = getattr(ctx, "max_context_len", None) or int(context_lens.max())
     group = num_heads // num_kv_heads
     warps, ranges = _attention8_split(requests, num_kv_heads, longest * group, keys if window is None else min(keys, window + longest), head_dim)
@@ -2514,39 +2526,38 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
         scratch = q.new_empty((ranges * 2 * (8 if longest * group <= 8 else 16) * (head_dim + 7),), dtype=torch.float32)
         add_launches(1)
     _check8(_launch("llm_attention8", q.data_ptr(), q.stride(0), out.data_ptr(), width, pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), places[1],
-                    cu_tokens.data_ptr(), context_lens.data_ptr(), requests, n, longest, below, num_heads, num_kv_heads, head_dim, pool.shape[3],
-                    pool.shape[0], int(window or 0), float(scale), warps, ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
+                    ctx.cu_tokens.data_ptr(), context_lens.data_ptr(), requests, n, longest, below, num_heads, num_kv_heads, head_dim, pool.shape[3],
+                    pool.shape[0], int(window or 0), scale, warps, ranges, None if scratch is None else scratch.data_ptr(), _error_flag_ptr(), _stream()),
             "paged_attention8")
-    return out
 
 
 _EXPANDED_BYTES = 2 << 30  # most memory that a call's pages may take as bfloat16
 
 
-def _attention8_portions(q, pool, exponents, page_table, ctx, out, heads: int, kv_heads: int, dim: int, scale: float, window: int) -> int:
+def _attention8_portions(q, pool, exponents, page_table, ctx, out, heads: int, kv_heads: int, dim: int, scale: float, window: int) -> tuple:
     """Requests that bring many tokens, over their pages as bfloat16 (csrc/expand_pages8.cu) on tcgen05.  Returns how many tokens send a
-    request this way, 0 if this way was not taken (pages or rows that the kernel does not take, too much memory)."""
+    request this way, 0 if this way was not taken (pages or rows that the kernel does not take, too much memory), and the pages' marks."""
     page_size, width = pool.shape[3], page_table.shape[1]
     if page_size not in _TC_ATTENTION_PAGE_SIZES or not _TC_ATTENTION_ENABLED or not scale > 0.0:
-        return 0
+        return 0, None
     least = _tc_join_tokens(ctx, heads, dim, dim, _TC_ATTENTION_JOIN_CROWDED)
     counts = [c for c in _token_counts(ctx) if c >= least]
     pages = len(counts) * width
     if not counts or pages * 2 * kv_heads * page_size * dim * 2 > _EXPANDED_BYTES:
-        return 0
+        return 0, None
     wide = q.new_empty((pages, 2, kv_heads, page_size, dim))
-    table = page_table.new_empty(page_table.shape)
     requests = page_table.shape[0]
+    table, marks = page_table.new_empty((2, requests, width))
     _check8(_launch("llm_expand_pages8", pool.data_ptr(), exponents.data_ptr(), page_table.data_ptr(), width, ctx.cu_tokens.data_ptr(), ctx.context_lens.data_ptr(),
-                    requests, kv_heads, dim, page_size, pool.shape[0], window, least, wide.data_ptr(), table.data_ptr(), _stream()), "expand_pages8")
+                    requests, kv_heads, dim, page_size, pool.shape[0], window, least, wide.data_ptr(), table.data_ptr(), marks.data_ptr(), _stream()), "expand_pages8")
     code = _launch("llm_attention_tcgen05", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), wide.data_ptr(), pages, table.data_ptr(), width,
                    ctx.cu_tokens.data_ptr(), ctx.context_lens.data_ptr(), requests, q.shape[0], heads, kv_heads, dim, page_size, window, scale, least,
                    max(counts), _error_flag_ptr(), _stream())
     if code == 10002:  # rows or pages that it does not take
         add_launches(-1)
-        return 0
+        return 0, None
     _check(code, "paged_attention8 (portions)")
-    return least
+    return least, marks
 
 
 _ATTENTION8_SPLIT: tuple | None = None  # for tests and measurements: (warps, stretches) whatever the rule says

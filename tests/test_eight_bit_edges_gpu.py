@@ -2,7 +2,7 @@
 
 import pytest
 import torch
-from test_eight_bit_gpu import BF16, DEV, E4M3, a_step, check_attention, gen, ops, pages8
+from test_eight_bit_gpu import BF16, DEV, E4M3, a_step, check_attention, gen, ops, pages8, request_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -64,6 +64,71 @@ def test_values_at_both_ends_of_the_exponents(exponent):
     exps[:, 1] = exponent
     q = torch.randn(1, 8 * D, generator=gen(5), device=DEV).to(BF16)
     check_attention(attend(q, pool, exps, table, ctx, D), q, pool, exps, table, ctx, 8, D, 0.05, None)
+
+
+def nan_lanes(v, first, n, window):
+    """Which rows and lanes see a NaN: ``v [len, KV, D]`` -> ``[n, KV, D]``."""
+    bad, out = v.isnan(), []
+    for p in range(first, first + n):
+        out.append(bad[(0 if window is None else max(0, p - window + 1)) : p + 1].any(0))
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("D,page_size", [(64, 16), (128, 64), (128, 8), (64, 24)])
+@pytest.mark.parametrize("window", [None, 5, 90])
+def test_nan_reaches_the_rows_that_see_in_long_portions(D, page_size, window):
+    """Values: the lanes that are NaN, for the rows that see them; keys: all lanes of those rows.  All other bits stay as they were."""
+    H, KV, counts, held = 4, 2, [130, 1, 300, 40], [200, 70, 300, 50]
+    ctx, table, _, pages = a_step(counts, held, page_size, 5)
+    q = torch.randn(ctx.num_tokens, H * D, generator=gen(3), device=DEV).to(BF16)
+    call = dict(num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1, window=window)
+    clean = pages8(pages, KV, page_size, D, 12)
+    want = ops().paged_attention8(q, *clean, table, ctx, **call).view(-1, H, D)
+    # (request, position, key head, lane): seen by all of its rows, by some, by the last; two of one lane; beside a tile's end
+    for which, places in ((1, [(0, 100, 0, 9)]), (1, [(0, 37, 1, 0), (2, 63, 0, D - 1), (2, 64, 0, 3), (2, 299, 1, 17), (3, 30, 1, 2)]), (1, [(2, 20, 0, 5), (2, 250, 0, 5)]),
+                          (0, [(0, 150, 0, 9), (2, 299, 1, 1)]), (1, None)):
+        pool, exps = (t.clone() for t in clean)
+        if places is None:
+            pool.view(torch.uint8)[:, 1] = 0xFF  # nothing but NaN
+        for r, j, head, lane in places or ():
+            pool[int(table[r, j // page_size]), which, head, j % page_size, lane] = torch.nan
+        got = ops().paged_attention8(q, pool, exps, table, ctx, **call).view(-1, H, D)
+        spoilt = []
+        for r, n in enumerate(held):
+            bad = nan_lanes(request_rows(pool, exps, table[r], n)[which], n - counts[r], counts[r], window)
+            spoilt.append((bad if which else bad.any(-1, keepdim=True).expand_as(bad)).repeat_interleave(H // KV, 1))
+        spoilt = torch.cat(spoilt)
+        assert torch.equal(got.isnan(), spoilt) and torch.equal(got[~spoilt], want[~spoilt])
+
+
+def test_nan_in_long_portions_as_a_graph():
+    """Whether there is NaN is the device's business: a captured call finds it, and finds it gone."""
+    H, KV, D = 4, 2, 64
+    ctx, table, _, pages = a_step([200], [260], 16, 5)
+    q = torch.randn(200, H * D, generator=gen(3), device=DEV).to(BF16)
+    pool, exps = pages8(pages, KV, 16, D, 12)
+
+    def go():
+        return ops().paged_attention8(q, pool, exps, table, ctx, num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+
+    want = go().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        go()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = go()
+    place = (int(table[0, 100 // 16]), 1, 1, 100 % 16, 7)
+    kept = pool[place].clone()
+    for bad in (False, True, False):
+        pool[place] = torch.nan if bad else kept.float()
+        graph.replay()
+        torch.cuda.synchronize()
+        spoilt = torch.zeros(200, H, D, dtype=torch.bool, device=DEV)
+        spoilt[40:, 2:, 7] = bad
+        assert torch.equal(y.view(200, H, D).isnan(), spoilt) and torch.equal(y.view(200, H, D)[~spoilt], want.view(200, H, D)[~spoilt])
 
 
 @pytest.mark.parametrize("KV,page_size,more_pages", [(1, 1, 0), (4, 3, 1), (2, 2, 0), (1, 4, 1), (3, 8, 1), (1, 16, 1)])
