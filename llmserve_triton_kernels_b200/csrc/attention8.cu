@@ -219,7 +219,6 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
     }
     __syncwarp();
     int filled = 0;  // stages this warp has asked for: the barriers' phases go on from segment to segment
-    bool broken = false;
     pdl_wait();
     pdl_trigger();
     long long at = 0, end = 1;
@@ -392,10 +391,20 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
 
         // tiles that begin in here are seen whole by every row
         const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
+        bool broken = false;
         for (int i0 = 0; i0 < mine; ++i0, ++filled) {
             const int slot = filled % STAGES;
             asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
-            if (RUN && !broken && !tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1)) broken = true;
+            if (RUN) {
+                // one answer for all lanes: those that gave up would part from the others in the products
+                broken = !__all_sync(0xffffffffu, tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1));
+                if (broken) {  // nothing more is asked for; what is on its way (this tile and those behind it) must land before the CTA ends
+                    if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
+                    for (int i = 0; i < min(STAGES - 1, mine - i0); ++i)
+                        (void)tma::mbar_wait(&full[warp][(filled + i) % STAGES], ((filled + i) / STAGES) & 1);
+                    break;
+                }
+            }
             __syncwarp();  // copies by other lanes have arrived; and everyone has read the stage that is filled next
             if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
@@ -585,13 +594,12 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
 
         // ---- the warps meet, where the rings were ----
         asm volatile("cp.async.wait_all;\n" ::: "memory");
-        if (broken) {  // a wait gave up: the result is void; what is still on its way must land before the memory serves another end
-            if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
-            for (int i = max(0, filled - STAGES); i < filled; ++i) (void)tma::mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
-        }
         // the rings were written by the other proxy too, and will be: order what threads do to the same places
         if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        __syncthreads();
+        if (RUN == 0)
+            __syncthreads();
+        else if (__syncthreads_or(broken))
+            return;  // a wait gave up: the result is void
         float* merge = reinterpret_cast<float*>(smem);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)

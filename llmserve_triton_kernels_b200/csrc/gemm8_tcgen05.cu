@@ -21,6 +21,7 @@
 #include "common.cuh"
 #include "linear8.h"
 #include "linear8_store.cuh"
+#include "linear8_waits.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -90,11 +91,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
         pdl_trigger();
     }
 
-    auto fail = [&]() {
-        *(volatile int*)&gave_up = 1;
-        if (error_flag) atomicExch(error_flag, 1);
-    };
-    auto failed = [&]() { return *(volatile int*)&gave_up != 0; };
+    const linear8::Waits waits = {&gave_up, 0, error_flag};
 
     // (each role's share of the registers is set where the role begins: what follows a smaller share is compiled for it)
     if (warp >= FIRST_EPI) {
@@ -130,11 +127,8 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
                     if (k0 + i >= kblocks) break;
                     const int buf = it % NBUF;
                     const float scale = sx_now[i] * sw_now[i];
-                    ok = __all_sync(0xffffffffu, !failed() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
-                    if (!ok) {
-                        if (lane == 0) fail();
-                        break;
-                    }
+                    ok = waits.there_untold(&acc_full[buf], (it / NBUF) & 1);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
                     const unsigned long long both = umma::pair_of(__float_as_uint(scale), __float_as_uint(scale));
@@ -158,11 +152,6 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(FEW_REGISTERS));
-        auto there = [&](unsigned long long* bar, unsigned parity) {  // for the whole warp
-            if (__all_sync(0xffffffffu, tma::mbar_wait(bar, parity))) return true;
-            fail();
-            return false;
-        };
         const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
         if (warp < FIRST_ISSUER) {
             // ---- producers ----
@@ -182,7 +171,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
                 const int m0 = (tile % row_tiles) * BM, n0 = (tile / row_tiles) * BN;
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
                     if ((it & 1) == which) {
-                        if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                        if (it >= STAGES) ok = waits.there_untold(&empty[s], (turn - 1) & 1);
                         if (!ok) break;
                         unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
                         if (umma::elect_one()) {
@@ -206,7 +195,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
                     if ((it & 1) == which) {
                         const int buf = it % NBUF;
-                        ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
+                        ok = waits.there(&full[s], turn & 1) && (it < NBUF || waits.there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                         const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
@@ -232,7 +221,7 @@ gemm8_tcgen05_kernel(const linear8::Operands p, int early, int* error_flag, cons
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    if (warp < FIRST_ISSUER && failed()) {  // nobody waits for the copies on their way any more
+    if (warp < FIRST_ISSUER && waits.failed()) {  // nobody waits for the copies on their way any more
         for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
             if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
     }
@@ -294,12 +283,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
         pdl_trigger();
     }
 
-    auto fail = [&]() {
-        *(volatile int*)&gave_up = 1;
-        *(volatile int*)cg::this_cluster().map_shared_rank(&gave_up, place ^ 1) = 1;
-        if (error_flag) atomicExch(error_flag, 1);
-    };
-    auto failed = [&]() { return *(volatile int*)&gave_up != 0; };
+    const linear8::Waits waits = {&gave_up, 2, error_flag};
 
     // (each role's share of the registers is set where the role begins: what follows a smaller share is compiled for it)
     if (warp >= FIRST_EPI) {
@@ -335,9 +319,10 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
                     if (k0 + i >= kblocks) break;
                     const int buf = it % NBUF;
                     const float scale = sx_now[i] * sw_now[i];
-                    ok = __all_sync(0xffffffffu, !failed() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
+                    // (waits.there_untold here and in the producers takes 4,096 x 28,672 x 4,096 from 461 us to 492: fail() in the middle of the loop)
+                    ok = __all_sync(0xffffffffu, !waits.flag() && tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
                     if (!ok) {
-                        if (lane == 0) fail();
+                        if (lane == 0) waits.fail();
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -363,11 +348,6 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(FEW_REGISTERS));
-        auto there = [&](unsigned long long* bar, unsigned parity) {  // for the whole warp
-            if (__all_sync(0xffffffffu, tma::mbar_wait(bar, parity))) return true;
-            fail();
-            return false;
-        };
         const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
         if (warp < FIRST_ISSUER) {
             // ---- producers ----
@@ -387,7 +367,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
                 const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + place * (BN / 2);
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
                     if ((it & 1) == which) {
-                        if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                        if (it >= STAGES) ok = waits.there(&empty[s], (turn - 1) & 1) && !waits.failed();
                         if (!ok) break;
                         unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
                         if (umma::elect_one()) {
@@ -411,7 +391,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
                     if ((it & 1) == which) {
                         const int buf = it % NBUF;
-                        ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
+                        ok = waits.there(&full[s], turn & 1) && (it < NBUF || waits.there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                         const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
@@ -437,7 +417,7 @@ gemm8_pair_kernel(const linear8::Operands p, int early, int* error_flag, const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
-    if (failed()) {  // (both CTAs know.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
+    if (waits.failed()) {  // (both CTAs know.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
         if (place == 0 && warp < FIRST_ISSUER) {
             for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
                 if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);

@@ -12,6 +12,7 @@
 #include "common.cuh"
 #include "linear8.h"
 #include "linear8_store.cuh"
+#include "linear8_waits.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -69,16 +70,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
         pdl_trigger();
     }
 
-    auto fail = [&]() {
-        *(volatile int*)&gave_up = 1;
-        if (error_flag) atomicExch(error_flag, 1);
-    };
-    auto failed = [&]() { return *(volatile int*)&gave_up != 0; };
-    auto there = [&](unsigned long long* bar, unsigned parity) {  // for the whole warp
-        if (__all_sync(0xffffffffu, tma::mbar_wait(bar, parity))) return true;
-        fail();
-        return false;
-    };
+    const linear8::Waits waits = {&gave_up, 0, error_flag};
 
     const int which = warp & 1;  // of the two producers or issuers: its k-blocks are every other one
     if (warp < FIRST_ISSUER) {
@@ -98,7 +90,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 if ((it & 1) == which) {
-                    if (it >= STAGES) ok = there(&empty[s], (turn - 1) & 1) && !failed();
+                    if (it >= STAGES) ok = waits.there_untold(&empty[s], (turn - 1) & 1);
                     if (!ok) break;
                     unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
                     if (umma::elect_one()) {
@@ -122,7 +114,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 if ((it & 1) == which) {
                     const int buf = it % NBUF;
-                    ok = there(&full[s], turn & 1) && (it < NBUF || there(&acc_empty[buf], ((it / NBUF) - 1) & 1)) && !failed();
+                    ok = waits.there(&full[s], turn & 1) && (it < NBUF || waits.there(&acc_empty[buf], ((it / NBUF) - 1) & 1));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
@@ -183,12 +175,8 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
                     const int buf = it % NBUF;
 #pragma unroll
                     for (int u = 0; u < COLS / 32; ++u) mine[i & 1][32 * u + lane] = now[i][u];
-                    ok = !failed() && __all_sync(0xffffffffu, tma::mbar_wait(&acc_full[buf], (it / NBUF) & 1));
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) {
-                        if (lane == 0) fail();
-                        break;
-                    }
+                    ok = waits.there_untold(&acc_full[buf], (it / NBUF) & 1);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned base = tmem_base + buf * BN + part * COLS + ((unsigned)(quarter * 32) << 16);
 #pragma unroll
@@ -230,7 +218,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
-    if (warp < FIRST_ISSUER && failed()) {  // nobody waits for the copies on their way any more
+    if (warp < FIRST_ISSUER && waits.failed()) {  // nobody waits for the copies on their way any more
         for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
             if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
     }

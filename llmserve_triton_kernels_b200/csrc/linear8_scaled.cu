@@ -21,6 +21,7 @@
 #include "common.cuh"
 #include "linear8.h"
 #include "linear8_store.cuh"
+#include "linear8_waits.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -37,24 +38,6 @@ constexpr int MAX_SPLIT = 4;
 
 // A power of two's biased exponent, four times.
 __device__ __forceinline__ unsigned exponents_of(float scale) { return (__float_as_uint(scale) >> 23 & 0xffu) * 0x01010101u; }
-
-// What the roles of both kernels share.
-struct Failing {
-    int* gave_up;
-    int ctas;  // of the cluster, all of which are told; 0: this one alone
-    int* error_flag;
-    __device__ __forceinline__ void fail() const {
-        *(volatile int*)gave_up = 1;
-        for (int r = 0; r < ctas; ++r) *(volatile int*)cg::this_cluster().map_shared_rank(gave_up, r) = 1;
-        if (error_flag) atomicExch(error_flag, 1);
-    }
-    __device__ __forceinline__ bool failed() const { return *(volatile int*)gave_up != 0; }
-    __device__ __forceinline__ bool there(unsigned long long* bar, unsigned parity) const {  // for the whole warp
-        if (__all_sync(0xffffffffu, tma::mbar_wait(bar, parity))) return true;
-        fail();
-        return false;
-    }
-};
 
 template <int BN, int STAGES, typename TO>
 __global__ void __launch_bounds__(512, 1)
@@ -111,7 +94,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         pdl_wait();
         pdl_trigger();
     }
-    const Failing f = {&gave_up, 0, error_flag};
+    const linear8::Waits waits = {&gave_up, 0, error_flag};
 
     if (warp < ISSUER) {
         // ---- producers ----
@@ -130,7 +113,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 if ((it & 1) == warp) {
-                    if (it >= STAGES) ok = f.there(&empty[s], (turn - 1) & 1) && !f.failed();
+                    if (it >= STAGES) ok = waits.there_untold(&empty[s], (turn - 1) & 1);
                     if (!ok) break;
                     unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
                     if (umma::elect_one()) {
@@ -152,11 +135,11 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step, ++round) {
             const int buf = round % NBUF;
-            if (round >= NBUF) ok = f.there(&acc_empty[buf], (round / NBUF - 1) & 1);
+            if (round >= NBUF) ok = waits.there(&acc_empty[buf], (round / NBUF - 1) & 1);
             for (int kb = k_lo; kb < k_hi && ok; ++kb) {
                 const int j = (kb - k_lo) % GROUP, g = group % GROUPS;
                 const bool last = kb == k_hi - 1;
-                ok = (j != 0 || f.there(&scales_full[g], (group / GROUPS) & 1)) && f.there(&full[s], turn & 1) && !f.failed();
+                ok = (j != 0 || waits.there(&scales_full[g], (group / GROUPS) & 1)) && waits.there(&full[s], turn & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
@@ -211,8 +194,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
                     }
                 if (k0 + GROUP < k_hi) ask(k0 + GROUP);
                 const int g = group % GROUPS;
-                ok = !f.failed() && (group < GROUPS || f.there(&scales_empty[g], (group / GROUPS - 1) & 1));
-                ok = __all_sync(0xffffffffu, ok);
+                ok = !waits.failed() && (group < GROUPS || waits.there(&scales_empty[g], (group / GROUPS - 1) & 1));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 umma::tmem_st32(at + g * GROUP * KB_COLS, r);
@@ -227,7 +209,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
         int round = 0;
         for (int tile = first_tile; tile < tiles; tile += tile_step, ++round) {
             const int n = (tile % col_tiles) * BM + quarter * 32 + lane, m_first = (tile / col_tiles) * BN + part * COLS, buf = round % NBUF;
-            if (!f.there(&acc_full[buf], (round / NBUF) & 1)) break;
+            if (!waits.there(&acc_full[buf], (round / NBUF) & 1)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             unsigned v[COLS / 32][32];
 #pragma unroll
@@ -252,7 +234,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     if (split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
-    if (warp < ISSUER && f.failed()) {  // nobody waits for the copies on their way any more
+    if (warp < ISSUER && waits.failed()) {  // nobody waits for the copies on their way any more
         for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
             if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
     }
@@ -344,7 +326,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
         pdl_wait();
         pdl_trigger();
     }
-    const Failing f = {&gave_up, 2 * split, error_flag};
+    const linear8::Waits waits = {&gave_up, 2 * split, error_flag};
 
     if (warp < ISSUER) {
         // ---- producers ----
@@ -364,7 +346,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
             const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + place * (BN / 2);
             for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
                 if ((it & 1) == warp) {
-                    if (it >= STAGES) ok = f.there(&empty[s], (turn - 1) & 1) && !f.failed();
+                    if (it >= STAGES) ok = waits.there_untold(&empty[s], (turn - 1) & 1);
                     if (!ok) break;
                     unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
                     if (umma::elect_one()) {
@@ -386,11 +368,11 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
             int s = 0, turn = 0, group = 0, round = 0;
             bool ok = true;
             for (int tile = pair; tile < tiles && ok; tile += pairs, ++round) {
-                if (round > 0) ok = f.there(&acc_empty, (round - 1) & 1);
+                if (round > 0) ok = waits.there(&acc_empty, (round - 1) & 1);
                 for (int kb = k_lo; kb < k_hi && ok; ++kb) {
                     const int j = (kb - k_lo) % GROUP, g = group % GROUPS;
                     const bool last = kb == k_hi - 1;
-                    ok = (j != 0 || f.there(&scales_full[g], (group / GROUPS) & 1)) && f.there(&full[s], turn & 1) && !f.failed();
+                    ok = (j != 0 || waits.there(&scales_full[g], (group / GROUPS) & 1)) && waits.there(&full[s], turn & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                     const unsigned char* slot = ring + (size_t)s * SLOT_BYTES;
@@ -439,8 +421,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
             ask(k_lo);
             for (int k0 = k_lo; k0 < k_hi; k0 += GROUP, ++group) {
                 const int g = group % GROUPS;
-                ok = !f.failed() && (group < GROUPS || f.there(&scales_empty[g], (group / GROUPS - 1) & 1));
-                ok = __all_sync(0xffffffffu, ok);
+                ok = !waits.failed() && (group < GROUPS || waits.there(&scales_empty[g], (group / GROUPS - 1) & 1));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll
@@ -469,7 +450,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
         int round = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++round) {
             const int m0 = (tile % row_tiles) * 2 * BM + place * BM, n0 = (tile / row_tiles) * BN + part * COLS;
-            if (!f.there(&acc_full, round & 1)) break;
+            if (!waits.there(&acc_full, round & 1)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             unsigned v[COLS / 32][32];
 #pragma unroll
@@ -498,7 +479,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     cg::this_cluster().sync();  // neither leaves while the other reads its memory or arrives at its barriers
-    if (f.failed()) {  // (the whole cluster knows.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
+    if (waits.failed()) {  // (the whole cluster knows.)  Nobody waits for the copies on their way any more, which are counted at the first CTA
         if (place == 0 && warp < ISSUER) {
             for (int i = max(0, asked[warp] - STAGES); i < asked[warp]; ++i)
                 if ((i & 1) == warp) (void)tma::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
