@@ -2317,6 +2317,7 @@ def delta_rule(y: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor, a_log: 
 _E4M3 = torch.float8_e4m3fn
 _BLOCK8 = 128
 ATTENTION8_HEAD_DIMS = (64, 128)
+_MAX_CONTEXT8 = 0x7FFF0000  # keys of a request's page table at most
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -2496,6 +2497,8 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     if len(places) != 2 or places[0] != requests or cu_tokens.numel() != requests + 1:
         raise KernelError("paged_attention8: a row of the page table and a length for every request")
     _here(q, pool, exponents, page_table, cu_tokens, context_lens)
+    if window is not None:
+        window = min(int(window), _MAX_CONTEXT8)  # (no context fills more; the kernels count in 32 bits)
     out = q.new_empty((n, width))
     if n == 0 or requests == 0:
         return out

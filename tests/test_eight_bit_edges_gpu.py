@@ -176,3 +176,16 @@ def test_small_pages_in_the_engine():
         llm.cache.check()
     assert [[len(t) for t in each] for each in tokens] == [[4, 4], [4, 4]]
     assert [t[0] for t in tokens[0]] == [t[0] for t in tokens[1]]
+
+
+@pytest.mark.parametrize("counts,held", [([1, 3], [700, 33]), ([130], [200])], ids=str)
+def test_windows_beyond_32_bits(counts, held):
+    """A window that no context fills is none, however large the number."""
+    H, KV, D = 4, 2, 64
+    ctx, table, _, pages = a_step(counts, held, 16, 6)
+    pool, exps = pages8(pages, KV, 16, D, 7)
+    q = torch.randn(ctx.num_tokens, H * D, generator=gen(8), device=DEV).to(BF16)
+    call = dict(num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+    want = ops().paged_attention8(q, pool, exps, table, ctx, window=10_000, **call)
+    for window in (2**31 - 1, 2**31, 2**32 + 5, 2**40):
+        assert torch.equal(ops().paged_attention8(q, pool, exps, table, ctx, window=window, **call), want), window
