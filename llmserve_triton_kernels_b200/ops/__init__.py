@@ -2335,7 +2335,8 @@ class Quantized:
     """A matrix ``[M, K]`` in 8 bits: ``values`` (float8_e4m3fn, contiguous) times a float32 scale for every block of ``rows`` (1 or 128)
     rows and 128 columns, ``scales [ceil(M / rows), ceil(K / 128)]``.  Scales may be any positive numbers, such as a checkpoint's.
     ``powers_of_two`` says that they are powers of two from 2^-126 on, as :func:`quantize_blocks` makes them, which the tensor cores
-    take as they are: a product of many rows is faster with them."""
+    take as they are: a product of many rows is faster with them.  What is said is looked at once, here (the host waits for the device;
+    within a capture, where it cannot, it is believed)."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, rows: int = 1, powers_of_two: bool = False):
         shape = values.shape
@@ -2346,6 +2347,10 @@ class Quantized:
             _need(values.dtype == _E4M3 and len(shape) == 2 and values.is_contiguous(), "Quantized: values are a contiguous float8_e4m3fn matrix")
             _need(scales.device == values.device, "Quantized: values and scales lie on one device")
             raise KernelError(f"Quantized: scales are contiguous float32 {[-(-shape[0] // rows), -(-shape[1] // _BLOCK8)]}")
+        if powers_of_two and not (scales.is_cuda and torch.cuda.is_current_stream_capturing()):
+            bits = scales.view(torch.int32)  # no sign and no mantissa, an exponent that is neither the lowest nor the highest
+            _need(not ((bits & 0x7FFFFF != 0) | (bits < 1 << 23) | (bits >= 255 << 23)).any().item(),
+                  "Quantized: scales that are no powers of two from 2^-126 on; powers_of_two says that they are")
         self.values, self.scales, self.rows, self.shape, self.powers_of_two = values, scales, rows, shape, powers_of_two
 
     @property
