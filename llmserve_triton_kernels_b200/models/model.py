@@ -93,10 +93,14 @@ class Model:
 
     def quantize_weights(self) -> None:
         """The layers' matrices in 8 bits, after :meth:`bind` (the token table, the output matrix and everything that is no matrix stay as
-        they are).  ValueError if a part's kernels read bfloat16 matrices only: then the model is not to be used, some parts may
-        have changed."""
+        they are).  ValueError if a part's kernels read bfloat16 matrices only, or its matrices have no rows of 16 values: then the model
+        stays as it was."""
         if self.dtype != torch.bfloat16:
             raise ValueError(f"8-bit weights go with bfloat16 activations, not {self.dtype}")
+        for _, part in self._named_parts:
+            why = part.refuse_eight_bit_weights()
+            if why:
+                raise ValueError(why)
         for _, part in self._named_parts:
             part.quantize_weights()
 

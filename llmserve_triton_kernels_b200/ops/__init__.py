@@ -2391,10 +2391,17 @@ def _check8(code: int, what: str) -> None:
         _check(code, what)
 
 
+def refuse_quantize(w) -> str | None:
+    """Why :func:`quantize_weight` does not take ``w``, or None."""
+    if isinstance(w, torch.Tensor) and w.dim() == 2 and w.shape[1] >= 16 and w.shape[1] % 16 == 0:
+        return None
+    return f"8-bit weights: a matrix with rows of a multiple of 16 values, not {list(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__}"
+
+
 def quantize_weight(w: torch.Tensor) -> Quantized:
     """A product's matrix ``[N, K]`` as :func:`linear8` takes it: a scale for every block of 128 x 128."""
-    _need(isinstance(w, torch.Tensor) and w.dim() == 2 and w.shape[1] >= 16 and w.shape[1] % 16 == 0,
-          f"quantize_weight: a matrix with rows of a multiple of 16 values, not {list(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__}")
+    why = refuse_quantize(w)
+    _need(why is None, f"quantize_weight: {why}")
     return quantize_blocks(w, rows=_BLOCK8)
 
 

@@ -113,9 +113,13 @@ class PagedAttention(Mixer):
         if self.position is not None:
             self.position.bind({}, dtype, device)
 
-    def quantize_weights(self) -> None:
+    def refuse_eight_bit_weights(self) -> str | None:
         if self.general:
-            raise ValueError("8-bit weights are not built for attention with value_dim, qk_norm_eps or distance_bias")
+            return "8-bit weights are not built for attention with value_dim, qk_norm_eps or distance_bias"
+        return ops.refuse_quantize(self.w_in) or ops.refuse_quantize(self.w_out)
+
+    def quantize_weights(self) -> None:
+        super().quantize_weights()
         self.w_in, self.w_out = ops.quantize_weight(self.w_in), ops.quantize_weight(self.w_out)
 
     @property

@@ -119,11 +119,19 @@ class Part:
     def tensors(self) -> dict[str, TensorSpec]:
         return {}
 
+    def refuse_eight_bit_weights(self) -> str | None:
+        """Why :meth:`quantize_weights` would refuse, or None.  By default a part that has matrices has kernels for bfloat16 ones only,
+        unless it says how they are put into 8 bits."""
+        if type(self).quantize_weights is Part.quantize_weights and any(len(spec.shape) >= 2 for spec in self.tensors().values()):
+            return f"8-bit weights are not built for {type(self).__name__}"
+        return None
+
     def quantize_weights(self) -> None:
         """Put the matrices of this part's products, once bound, into 8 bits (``ops.quantize_blocks`` with a scale for every 128 x 128).  A
         part without matrices has nothing to do; one whose kernels read bfloat16 matrices only refuses."""
-        if any(len(spec.shape) >= 2 for spec in self.tensors().values()):
-            raise ValueError(f"8-bit weights are not built for {type(self).__name__}")
+        why = self.refuse_eight_bit_weights()
+        if why:
+            raise ValueError(why)
 
     def bind(self, tensors: dict[str, torch.Tensor], dtype: torch.dtype, device: torch.device) -> None:
         """Take ownership of the loaded tensors (keyed by local name), in the compute dtype."""

@@ -54,7 +54,11 @@ class GatedMLP(FeedForward):
             self.b_gate_up = torch.cat([tensors[self.names["gate_bias"]].to(dtype), tensors[self.names["up_bias"]].to(dtype)]).to(device).contiguous()
             self.b_down_32 = tensors[self.names["down_bias"]].to(device=device, dtype=torch.float32).contiguous()  # the sum it joins is 32-bit
 
+    def refuse_eight_bit_weights(self) -> str | None:
+        return ops.refuse_quantize(self.w_gate_up) or ops.refuse_quantize(self.w_down)
+
     def quantize_weights(self) -> None:
+        super().quantize_weights()
         self.w_gate_up, self.w_down = ops.quantize_weight(self.w_gate_up), ops.quantize_weight(self.w_down)
 
     accepts_sink = True
