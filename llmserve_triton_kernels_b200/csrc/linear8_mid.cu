@@ -38,7 +38,7 @@ linear8_mid_kernel(const linear8::Operands p, int split, int early, int* error_f
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % split, first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
     const int col_tiles = (p.N + BM - 1) / BM, tiles = col_tiles * ((p.M + BN - 1) / BN);
-    const int per = (p.kblocks + split - 1) / split, k_lo = min(p.kblocks, rank * per), k_hi = min(p.kblocks, k_lo + per);
+    const int k_lo = p.kblocks * rank / split, k_hi = p.kblocks * (rank + 1) / split;
 
     if (threadIdx.x == 0) {
 #pragma unroll

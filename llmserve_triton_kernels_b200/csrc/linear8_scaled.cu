@@ -59,7 +59,7 @@ linear8_scaled_kernel(const linear8::Operands p, int split, int early, int* erro
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % split, first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
     const int col_tiles = (p.N + BM - 1) / BM, tiles = col_tiles * ((p.M + BN - 1) / BN);
-    const int per = (p.kblocks + split - 1) / split, k_lo = min(p.kblocks, rank * per), k_hi = min(p.kblocks, k_lo + per);
+    const int k_lo = p.kblocks * rank / split, k_hi = p.kblocks * (rank + 1) / split;
 
     if (threadIdx.x == 0) {
 #pragma unroll
@@ -293,7 +293,7 @@ linear8_scaled_pair_kernel(const linear8::Operands p, int split, int early, int*
     // `split` pairs (1 or 2, a cluster) share a tile's k-blocks; the pair's first CTA has rank `leader` in the cluster
     const int place = blockIdx.x & 1, index = (blockIdx.x >> 1) % split, pair = (blockIdx.x >> 1) / split, pairs = (gridDim.x >> 1) / split;
     const unsigned leader = 2 * index;
-    const int per = (p.kblocks + split - 1) / split, k_lo = min(p.kblocks, index * per), k_hi = min(p.kblocks, k_lo + per);
+    const int k_lo = p.kblocks * index / split, k_hi = p.kblocks * (index + 1) / split;
     const int row_tiles = (p.M + 2 * BM - 1) / (2 * BM), tiles = row_tiles * ((p.N + BN - 1) / BN);
 
     if (threadIdx.x == 0) {

@@ -1,8 +1,10 @@
-"""Attention over 8-bit pages where its numbers and its pages end."""
+"""Attention over 8-bit pages where its numbers and its pages end; products whose work does not go round evenly."""
 
 import pytest
 import torch
-from test_eight_bit_gpu import BF16, DEV, E4M3, a_step, check_attention, gen, ops, pages8, request_rows
+from test_eight_bit_gpu import (
+    BF16, DEV, E4M3, a_step, check_attention, check_product, check_scaled, gen, ops, pages8, request_rows, spread, weights,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +191,15 @@ def test_windows_beyond_32_bits(counts, held):
     want = ops().paged_attention8(q, pool, exps, table, ctx, window=10_000, **call)
     for window in (2**31 - 1, 2**31, 2**32 + 5, 2**40):
         assert torch.equal(ops().paged_attention8(q, pool, exps, table, ctx, window=window, **call), want), window
+
+
+@pytest.mark.parametrize("k", [1040, 2064, 2640, 2944, 4112])
+@pytest.mark.parametrize("m", [20, 70, 300])
+def test_k_blocks_shared_out_unevenly(m, k):
+    """K-blocks that do not go evenly into the two or four CTAs, or the two pairs, of a tile: 9, 17, 21, 23 and 33."""
+    x = spread(m, k, 1, k).to(BF16)
+    for n in (130, 700):
+        w = weights(n, k, n)
+        check_product(ops().linear8(x, w), x, w, f"{n} features")
+        w = ops().quantize_weight(spread(n, k, 128, n))
+        check_scaled(ops().linear8(x, w), x, w, f"{n} features, powers of two")
