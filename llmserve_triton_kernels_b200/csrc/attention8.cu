@@ -68,7 +68,7 @@ struct Attn8Params {
     int requests, H, KV, G, page_size, pages, window;
     int below;          // requests that bring so many tokens or more are left out (0: none)
     int* error_flag;
-    int warps;          // of a CTA
+    int warps;          // of a CTA that takes a tile of rows with all its keys
     int ranges;         // stretches of the step's list of tiles at most; 0: a CTA takes a tile of rows with all its keys
     float scale;        // times log2 e
     float* part_sums;   // [ranges][2][ROWS][D + 4]: what a stretch holds of the rows at its beginning and at its end,
@@ -193,7 +193,7 @@ __device__ __forceinline__ bool lay_out(const Attn8Params& p, long long* begins)
 
 // Stretches of a list of `total` places: no more than there are CTAs, none (but the last) shorter than a tile a warp, or than a unit.
 __device__ __forceinline__ int stretches(const Attn8Params& p, long long total, bool cut) {
-    return (int)max(1LL, min((long long)p.ranges, cut ? total / p.warps : total));
+    return (int)max(1LL, min((long long)p.ranges, cut ? total / 8 : total));
 }
 
 // RUN: pages hold whole runs of 8 or 16 keys; 0: they do not, and the threads copy every key from its own place.
@@ -207,7 +207,7 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
     // the warps' rings; at a segment's end [WARPS][ROWS][PITCH] sums
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ float stats[WARPS][ROWS][3];  // largest score, largest score with the value's scale, sum of weights
-    __shared__ long long begins[MAX_REQUESTS + 1];
+    __shared__ long long begins[WARPS == 8 ? MAX_REQUESTS + 1 : 1];
     __shared__ __align__(16) unsigned char scales[WARPS][STAGES][2 * TILE];  // exponents of a stage's keys and values
     __shared__ __align__(8) unsigned long long full[WARPS][STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -223,7 +223,8 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
     pdl_trigger();
     long long at = 0, end = 1;
     bool cut = false;
-    if (p.ranges) {
+    const bool shared_out = WARPS == 8 && p.ranges;  // (stretches are CTAs of eight warps)
+    if (shared_out) {
         cut = lay_out<ROWS>(p, begins);
         const long long total = begins[p.requests];
         const int count = stretches(p, total, cut);
@@ -234,7 +235,7 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
     while (at < end) {
         // ---- the segment: request r, key head h, rows from row0 on, tiles tile_lo .. tile_hi - 1 ----
         int r, h, row0, tile_lo, tile_hi, part = -1;  // part: the place in scratch memory of a segment without all keys
-        if (p.ranges) {
+        if (shared_out) {
             int lo = 0, hi = p.requests;  // the last request whose share begins at or before `at`
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -760,20 +761,17 @@ int launch_warps(const Attn8Params& p, int longest, cudaStream_t stream) {
 
 template <int D, int NT, int RUN>
 int launch(const Attn8Params& p, int longest, cudaStream_t stream) {
-    return p.warps == 2 ? launch_warps<D, NT, RUN, 2>(p, longest, stream) : launch_warps<D, NT, RUN, 8>(p, longest, stream);
+    return p.warps == 2 && !p.ranges ? launch_warps<D, NT, RUN, 2>(p, longest, stream) : launch_warps<D, NT, RUN, 8>(p, longest, stream);
 }
 
 }  // namespace
 
-// Rows of a tile for `longest` tokens a request and G query heads a key head: the sums that a stretch leaves are [2][rows][D + 4 + 3] floats.
-LLM_EXPORT int llm_attention8_rows(int longest, int G) { return (long long)longest * G <= 8 ? 8 : 16; }
-
 // q rows [n, >= H D] bfloat16 (row stride a multiple of 4, 8-byte aligned); pool and exponents as rope_kv_write8.cu leaves them, the pool on 16
 // bytes, the exponents anywhere; request r's new tokens are rows cu_tokens[r] .. cu_tokens[r + 1] - 1, the last one at position context_lens[r] - 1; `longest`: the
 // most tokens a request brings; with `below` requests that bring so many or more are left out, and their
-// rows of out as they are.  out [n, H D].  window 0: none.  warps of a CTA: 2 or 8.  ranges: CTAs that share the step's keys evenly, with
-// scratch memory of ranges * 2 * llm_attention8_rows * (D + 7) floats on 16 bytes (at most 1,024 requests); 0: one for each key head and
-// tile of rows.  D 64 or 128.
+// rows of out as they are.  out [n, H D].  window 0: none.  ranges: CTAs of eight warps that share the step's keys evenly, with scratch
+// memory of ranges * 2 * R * (D + 7) floats on 16 bytes, R the rows of a tile (8 where the longest request has no more, else 16), at most 1,024
+// requests; 0: a CTA of `warps` (2 or 8) for each key head and tile of rows.  D 64 or 128.
 LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long long out_stride, const void* pool, const void* exponents,
                               const int* page_table, int table_width, const int* cu_tokens, const int* context_lens, int requests, int n,
                               int longest, int below, int H, int KV, int D, int page_size, int pages, int window, float scale, int warps, int ranges,
@@ -784,7 +782,7 @@ LLM_EXPORT int llm_attention8(const void* q, long long q_stride, void* out, long
         (out_stride & 3) || ((uintptr_t)out & 7) || ((uintptr_t)pool & 15) ||
         (long long)table_width * page_size > 0x7fff0000)
         return LLM_ERR_BAD_ARGUMENT;
-    const int rows = llm_attention8_rows(longest, H / KV);
+    const int rows = (long long)longest * (H / KV) <= 8 ? 8 : 16;
     Attn8Params p = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)pool, (const unsigned char*)exponents,
                      page_table, table_width, cu_tokens, context_lens, requests, H, KV, H / KV, page_size, pages, window, below, error_flag, warps, ranges,
                      scale * 1.4426950408889634f, scratch, ranges ? scratch + (size_t)ranges * 2 * rows * (D + 4) : nullptr};

@@ -2579,7 +2579,7 @@ _ATTENTION8_SPLIT: tuple | None = None  # for tests and measurements: (warps, st
 
 
 def _attention8_split(requests: int, kv_heads: int, rows: int, keys: int, head_dim: int) -> tuple:
-    """How :func:`paged_attention8` shares its work out: ``(warps of a CTA, stretches)``.
+    """How :func:`paged_attention8` shares its work out: ``(warps of a CTA, stretches)``; stretches are CTAs of eight warps.
 
     A unit is a tile of 8 or 16 rows of a request and a key head, with at most ``keys`` keys.  Without stretches (0) a CTA takes a unit; with
     them the keys of all units are dealt out evenly and a second kernel joins what was cut.  Measured on 148 SMs with heads of 128 lanes
