@@ -31,9 +31,9 @@
 // Cutting and joining cost 8 us and more, so short or many units of work go without: a CTA takes a tile of rows with all its keys, of two
 // warps instead of eight where there are many units of few keys, whose time is a CTA's 4 us of loads that wait for one another (q and
 // the page table, the pages, the warps' meeting) and not the bytes.  The host picks, from the longest context it is told.
-// Heads of 128 lanes, requests of random lengths, 32 heads over 8: 32 of up to 8,191 keys 67 us, 5.2 TB/s of pages; 64 of up to 4,000 69 us,
-// 4.9 TB/s; 8 of up to 4,000 19 us, of which 8 are laying out, cutting and joining.  32 heads of their own: 64 of up to 4,000 219 us, 6.25 TB/s.
-// It is not the memory that bounds the first but the warps' own chains: 383 instructions a tile of 16 keys with the 4 warps that an SM's
+// Heads of 128 lanes, requests of random lengths, 32 heads over 8: 32 of up to 8,191 keys 68 us, 5.2 TB/s of pages; 64 of up to 4,000 77 us,
+// 4.5 TB/s; 8 of up to 4,000 19 us, of which 8 are laying out, cutting and joining.  32 heads of their own: 64 of up to 4,000 227 us, 6.0 TB/s.
+// It is not the memory that bounds the first but the warps' own chains: some 390 instructions a tile of 16 keys with the 4 warps that an SM's
 // quarter has registers for (500 instructions a tile took 73 us, the same pages all in the L2 5 % less).
 //
 // Masks: a key that no row of the tile may see, or that lies behind the request's end, is never multiplied (its 8 bits may be NaN).
@@ -393,18 +393,15 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
         // tiles that begin in here are seen whole by every row
         const int whole_from = p.window > 0 ? pos_max - p.window + 1 : 0, whole_to = min(pos_min + 1, key_end) - TILE;
         bool broken = false;
-        for (int i0 = 0; i0 < mine; ++i0, ++filled) {
+        int i0 = 0;
+        for (; i0 < mine; ++i0, ++filled) {
             const int slot = filled % STAGES;
             asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
             if (RUN) {
-                // one answer for all lanes: those that gave up would part from the others in the products
+                // one answer for all lanes: those that gave up would part from the others in the products.  (The vote costs 0.2 us of 68; as part of the
+                // tile's other vote, below, 2.)
                 broken = !__all_sync(0xffffffffu, tma::mbar_wait(&full[warp][slot], (filled / STAGES) & 1));
-                if (broken) {  // nothing more is asked for; what is on its way (this tile and those behind it) must land before the CTA ends
-                    if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
-                    for (int i = 0; i < min(STAGES - 1, mine - i0); ++i)
-                        (void)tma::mbar_wait(&full[warp][(filled + i) % STAGES], ((filled + i) / STAGES) & 1);
-                    break;
-                }
+                if (broken) break;  // nothing more is asked for
             }
             __syncwarp();  // copies by other lanes have arrived; and everyone has read the stage that is filled next
             if (i0 + STAGES - 1 < mine) issue(i0 + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
@@ -525,18 +522,17 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
                         behind |= s[nt][e] > m1[nt][e & 1] + 16.f || u[nt][e] > m2[nt][e & 1] + (ABOVE + LAG);
                     }
                 if (__any_sync(0xffffffffu, behind)) {
-                    // A vector of zeros is written with a scale of one.  (To look at the values of every tile that comes here takes 32 requests of up to
-                    // 2,000 keys with 32 key heads of 128 lanes from 68.9 us to 70.6, of 64 lanes and 4 heads 8 of 1,000 from 8.5 to 8.8.)
+                    // A vector of zeros is written with a scale of one.  (To look at the values of every tile that comes here took 8 requests of up to 1,000 keys
+                    // with 4 key heads of 64 lanes 8.8 us, to look where a scale is one 8.5, as without.)
                     if (__any_sync(0xffffffffu, ev[0] == 0.f || ev[1] == 0.f)) {
-                        unsigned some = 0;  // bit j: value j is no vector of zeros
+                        unsigned bits = 0;  // half of value lane & 15, read anew: what is seldom done holds no registers
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            unsigned bits = 0;
-#pragma unroll
-                            for (int w = 0; w < D / 32; ++w) bits |= v[e][w];
-                            some |= (bits & 0x7f7f7f7fu ? 1u : 0u) << (2 * t + (e & 1) + 8 * (e >> 1));
+                        for (int c = 0; c < D / 32; ++c) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(stage + S::VALUES + S::key(lane & 15, (lane >> 4) * (D / 32) + c));
+                            bits |= w.x | w.y | w.z | w.w;
                         }
-                        some = __reduce_or_sync(0xffffffffu, some);
+                        unsigned some = __ballot_sync(0xffffffffu, (bits & 0x7f7f7f7fu) != 0u);
+                        some |= some >> 16;  // bit j: value j is no vector of zeros
 #pragma unroll
                         for (int x = 0; x < 2; ++x)
                             if (!(some >> (g + 8 * x) & 1u)) {  // (its weight might not be a number of half precision)
@@ -595,6 +591,10 @@ attention8_kernel(const Attn8Params p, const __grid_constant__ CUtensorMap map) 
 
         // ---- the warps meet, where the rings were ----
         asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (RUN && broken) {  // what is on its way (the tile that was waited for and those behind it) must land before the CTA ends
+            if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
+            for (int i = 0; i < min(STAGES - 1, mine - i0); ++i) (void)tma::mbar_wait(&full[warp][(filled + i) % STAGES], ((filled + i) / STAGES) & 1);
+        }
         // the rings were written by the other proxy too, and will be: order what threads do to the same places
         if (RUN) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         if (RUN == 0)
