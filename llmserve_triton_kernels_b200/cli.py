@@ -32,8 +32,8 @@ def parse_args(argv=None):
     ap.add_argument("--seed", type=int, default=None, help="sampling seed (and the weights' seed for a preset; default 0 there)")
     ap.add_argument("--device", default="cuda", help="a CUDA device; there is no CPU path")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
-    ap.add_argument("--weight-dtype", choices=["float8"], default=None, help="the layers' matrices in 8 bits (default: as --dtype)")
-    ap.add_argument("--cache-dtype", choices=["float8"], default=None, help="keys and values in 8-bit pages (default: as --dtype)")
+    ap.add_argument("--weight-dtype", choices=["float8"], default=None, help="the layers' matrices in 8 bits (default: as --dtype); for large models: small ones get slower")
+    ap.add_argument("--cache-dtype", choices=["float8"], default=None, help="keys and values in 8-bit pages (default: as --dtype); for large batches and long contexts")
     ap.add_argument("--block-size", type=int, default=16)
     ap.add_argument("--num-blocks", type=int, default=None)
     ap.add_argument("--kv-mem-mib", type=float, default=None, help="size the cache by memory instead of --num-blocks")

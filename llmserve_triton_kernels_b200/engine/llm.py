@@ -71,7 +71,10 @@ class LLM:
 
         ``weight_dtype`` "float8": the layers' matrices in 8 bits (e4m3, a scale for every 128 x 128; the activations are quantised row
         by row in front of every product).  ``cache_dtype`` "float8": keys and values in 8-bit pages (e4m3, a power of two for
-        every head's vector).  None: the compute type.  Both go with bfloat16 and the Llama architecture's layers.
+        every head's vector).  None: the compute type.  Both go with bfloat16 and the Llama architecture's layers.  They halve the
+        bytes, which pays for large models, batches and contexts; a small model's step is bound by launches, of which 8-bit layers have more
+        (one request, TinyLlama's sizes 0.88 ms instead of 0.69, Llama 3 8B's 2.52 instead of 2.73, and 2.59 with 8-bit pages too).
+        A long prompt's 8-bit pages are unpacked in up to 2 GiB of scratch memory, which must be left free beside the cache.
 
         ``freeze_gc``: once the engine stands, collect garbage and move everything that is alive to the collector's
         permanent generation (``gc.freeze()``).  A full collection otherwise walks the some 170,000 objects that the

@@ -2490,7 +2490,8 @@ def paged_attention8(q: torch.Tensor, pool: torch.Tensor, exponents: torch.Tenso
     heads; ``ctx`` and what a token sees are as there.  A row that sees no key comes out as zeros.  Where it pays the keys
     are spread evenly over the CTAs, wherever requests begin and end, and joined by a second kernel.  Requests that bring so many new tokens
     that :func:`paged_attention` would take them to tcgen05 have their pages unpacked to bfloat16 first, in scratch memory of at most 2 GiB,
-    and go the same way from there.  Returns bfloat16 ``[N, num_heads * head_dim]``."""
+    and go the same way from there.  NaN among the keys or values reaches the rows that see it and no other.  Returns bfloat16
+    ``[N, num_heads * head_dim]``."""
     width = num_heads * head_dim
     if not (q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= width and q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0
             and num_kv_heads > 0 and num_heads % num_kv_heads == 0 and (window is None or window >= 1)):
