@@ -1,9 +1,10 @@
 """Attention over 8-bit pages where its numbers and its pages end; products whose work does not go round evenly."""
 
+import plain_eight_bit as plain
 import pytest
 import torch
 from test_eight_bit_gpu import (
-    BF16, DEV, E4M3, a_step, check_attention, check_product, check_scaled, gen, ops, pages8, request_rows, spread, weights,
+    BF16, DEV, E4M3, F64, a_step, check_attention, check_product, check_scaled, gen, ops, pages8, request_rows, spread, weights,
 )
 
 pytestmark = pytest.mark.gpu
@@ -55,6 +56,60 @@ def test_a_lane_far_above_the_others(D, above, far, held, new):
     pool[page, 1, :, off, 5] = 448.0
     exps[page, 1, :, off] = 110 + far
     check_attention(attend(q, pool, exps, table, ctx, D), q, pool, exps, table, ctx, 8, D, 0.05, None)
+
+
+def small_weights_loss(q, pool, exps, table_row, length, new, H, D, scale, window):
+    """What weights far below a row's largest may lose, ``[new, H, 1]``: with their values' scales they are held in half precision relative to a
+    reference 2^11 to 2^15 below the largest, where a number has an error of 2^-25 at most: 2^-36 of the largest for every key, times a value of
+    448 at most."""
+    keys, _ = request_rows(pool, exps, table_row, length)
+    at = torch.arange(length, device=DEV)
+    ev = exps[table_row.long()[at // pool.shape[3]], 1, :, at % pool.shape[3]].to(F64) - 127  # [length, KV]
+    group, place = H // pool.shape[2], torch.arange(length - new, length, device=DEV)
+    s = torch.einsum("nhd,jhd->nhj", q[:, : H * D].view(new, H, D).to(F64), keys.repeat_interleave(group, 1)) * scale
+    hidden = at[None] > place[:, None]
+    if window is not None:
+        hidden |= at[None] <= place[:, None] - window
+    p = torch.softmax(s.masked_fill(hidden[:, None], -torch.inf), -1)
+    largest = (p * torch.exp2(ev).t().repeat_interleave(group, 0)).amax(-1, keepdim=True)
+    return length * 2.0**-36 * 448 * largest
+
+
+def check_far_apart(got, q, pool, exps, table, held, new, H, D, scale, window):
+    """As ``check_attention`` for one request, and what small weights may lose."""
+    keys, values = request_rows(pool, exps, table[0], held)
+    rows = q[:new, : H * D].view(new, H, D)
+    want, size = (plain.attention(rows, keys, v, held - new, scale, window) for v in (values, values.abs()))
+    off = (got[:new].view(new, H, D).to(F64) - want).abs()
+    assert (off <= (2.0**-11 + 2.0**-15) * size + 2.0**-8 * want.abs() + small_weights_loss(q[:new], pool, exps, table[0], held, new, H, D, scale, window)).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("above", [0, 6, 12])
+@pytest.mark.parametrize("far", [14, 30, 60, 120])
+@pytest.mark.parametrize("held,new", [(64, 1), (1500, 1), (90, 5), (700, 21)])
+def test_a_lane_beyond_half_precision(D, above, far, held, new):
+    """... and however far: what the others lose then is small beside that lane."""
+    q, pool, exps, table, ctx, page, off = a_token_that_draws(D, held, new, above, 10, held)
+    pool.view(torch.uint8)[page, 1, :, off] = 0
+    pool[page, 1, :, off, 5] = 448.0
+    exps[page, 1, :, off] = 110 + far
+    check_far_apart(attend(q, pool, exps, table, ctx, D), q, pool, exps, table, held, new, 8, D, 0.05, None)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("held,new", [(40, 1), (1500, 1), (90, 5), (700, 21)])
+@pytest.mark.parametrize("window", [None, 60])
+def test_values_of_one_lane_with_scales_of_their_own(D, held, new, window):
+    """Every value has one lane, and a scale anywhere in 2^-60 to 2^40: each lane's output is made of a few of them, whatever the others are."""
+    ctx, table, _, pages = a_step([new], [held], 16, 8)
+    pool, exps = pages8(pages, 2, 16, D, 9)
+    lanes = torch.randint(0, D, exps[:, 1].shape, generator=gen(10), device=DEV)
+    one = torch.nn.functional.one_hot(lanes, D).to(torch.bool)
+    pool[:, 1] = torch.where(one, pool[:, 1].float(), 0.0).to(E4M3)
+    exps[:, 1] = torch.randint(67, 167, exps[:, 1].shape, generator=gen(11), device=DEV).to(torch.uint8)
+    q = torch.randn(new, 8 * D, generator=gen(12), device=DEV).to(BF16)
+    check_far_apart(attend(q, pool, exps, table, ctx, D, window=window), q, pool, exps, table, held, new, 8, D, 0.05, window)
 
 
 @pytest.mark.parametrize("exponent", [2, 8, 230])
