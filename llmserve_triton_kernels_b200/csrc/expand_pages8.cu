@@ -1,6 +1,7 @@
 // Pages in 8 bits as bfloat16 pages, for requests that bring so many tokens that the products bound their attention: there the tcgen05
 // kernel over bfloat16 pages does it, and what every tile of rows would unpack anew is unpacked once.  A number e4m3 * 2^e is a bfloat16
-// number (but for the smallest of all), so nothing is rounded.
+// number, so nothing is rounded, but for the smallest of all and for 2^128, to which bfloat16's largest numbers are rounded in 8 bits: it becomes
+// the largest of bfloat16 again, 2^-8 less, because an infinity would make NaN of the rows that do not see it.
 //
 // Request r's pages lie one after another from page rank(r) * width on, rank counting the requests that bring at least `least` tokens.
 // Three portions of up to 301 tokens in contexts of up to 1,501 (32 query and 4 key heads of 64 lanes) take 43 us this way, and 128 by the
@@ -16,6 +17,12 @@
 namespace {
 
 constexpr int THREADS = 256;
+
+// Within bfloat16's numbers; a key's NaN stays one.
+__device__ __forceinline__ float held(float v) {
+    const float most = __uint_as_float(0x7f7f0000u);
+    return v > most ? most : v < -most ? -most : v;
+}
 
 template <int D>
 __global__ void __launch_bounds__(THREADS)
@@ -66,8 +73,8 @@ expand_pages8_kernel(const unsigned char* __restrict__ pool, const unsigned char
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float2 f = fp8::unpack2((unsigned short)(words[k] >> (16 * e)));
-                v[k >> 1][(k & 1) * 4 + 2 * e] = f.x * scale;
-                v[k >> 1][(k & 1) * 4 + 2 * e + 1] = f.y * scale;
+                v[k >> 1][(k & 1) * 4 + 2 * e] = held(f.x * scale);
+                v[k >> 1][(k & 1) * 4 + 2 * e + 1] = held(f.y * scale);
             }
         __nv_bfloat16* dst = out + (to * keys + key) * D + c;
         fp8::store8(dst, v[0]);

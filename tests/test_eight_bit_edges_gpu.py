@@ -258,3 +258,30 @@ def test_k_blocks_shared_out_unevenly(m, k):
         check_product(ops().linear8(x, w), x, w, f"{n} features")
         w = ops().quantize_weight(spread(n, k, 128, n))
         check_scaled(ops().linear8(x, w), x, w, f"{n} features, powers of two")
+
+
+@pytest.mark.parametrize("counts,held", [([130, 1], [200, 64]), ([40, 2], [200, 64])], ids=str)
+@pytest.mark.parametrize("lowest", [torch.finfo(BF16).min, torch.finfo(BF16).max, 3.32e38], ids=str)
+def test_values_of_the_types_lowest_number(counts, held, lowest):
+    """bfloat16's largest numbers come to 2^128 in 8 bits, which 32 bits do not hold: rows that do not see them stay as they were, rows that do
+    get their share.  (In long portions the largest bfloat16 number stands for 2^128: 2^-8 of it, as much as half a step of the output.)"""
+    H, KV, D, page_size, place = 4, 2, 64, 16, 180
+    ctx, table, _, pages = a_step(counts, held, page_size, 5)
+    q = torch.randn(ctx.num_tokens, H * D, generator=gen(3), device=DEV).to(BF16)
+    pool, exps = pages8(pages, KV, page_size, D, 12)
+    call = dict(num_heads=H, num_kv_heads=KV, head_dim=D, scale=0.1)
+    want = ops().paged_attention8(q, pool, exps, table, ctx, **call).view(-1, H, D)
+    one = torch.zeros(1, 3 * KV * D, dtype=BF16, device=DEV)  # a key of zeros, and a value of zeros but for one lane
+    one[0, 2 * KV * D + 7] = lowest
+    slot = table[0, place // page_size] * page_size + place % page_size
+    ops().rope_kv_write8(one, ctx.positions[:1], None, slot.view(1), pool, exps, KV, KV, D)
+    got = ops().paged_attention8(q, pool, exps, table, ctx, **call).view(-1, H, D)
+    first, last = held[0] - counts[0], place - (held[0] - counts[0])  # rows in front of `last` do not see the place
+    assert torch.equal(got[:last], want[:last]) and torch.equal(got[counts[0] :], want[counts[0] :]) and not got.isnan().any()
+    keys, values = request_rows(pool, exps, table[0], held[0])
+    rows = q[: counts[0]].view(-1, H, D)
+    exact, size = (plain.attention(rows, keys, v, first, 0.1, None) for v in (values, values.abs()))
+    assert exact.abs().max() > 1e36
+    # (long portions: weights in bfloat16, 2^-8 with the largest number's 2^-8; short ones: what small weights lose)
+    loss = 0.0 if counts[0] >= 128 else small_weights_loss(q[: counts[0]], pool, exps, table[0], held[0], counts[0], H, D, 0.1, None)
+    assert ((got[: counts[0]].to(F64) - exact).abs() <= (2.0**-7 + 2.0**-14) * size + 2.0**-8 * exact.abs() + loss).all()
