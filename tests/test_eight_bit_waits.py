@@ -1,4 +1,5 @@
-"""Waits of the 8-bit kernels that give up.  No launch makes one give up, so the sources are held to the form that is safe: a wait's outcome, and the flag that tells of one, reach a warp's lanes as one answer.  A lane that left a loop alone would leave the others at a vote, an
+"""Waits of the 8-bit kernels that give up.  No launch makes one give up, so the sources are held to the form that is safe: a wait's
+outcome, and the flag that tells of one, reach a warp's lanes as one answer.  A lane that left a loop alone would leave the others at a vote, an
 election or a load of tensor memory that is for all of them."""
 
 import re
